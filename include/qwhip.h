@@ -300,6 +300,116 @@ int32_t qwh_kv_append_q8(qwh_ctx *ctx, const float *key_dev, const float *value_
  * unless a later value compares greater). The decoder step's argmax. */
 int32_t qwh_argmax_rows(qwh_ctx *ctx, const float *logits_dev, uint32_t rows, uint32_t count, uint32_t *ids_dev);
 
+/* temperature, top-k, top-p and min-p of one row. */
+typedef struct {
+    float temperature; /* not above 0 (or NaN): the largest logit */
+    uint32_t top_k;    /* 0, or count and more: off */
+    float top_p;       /* 1 and more (or NaN): off */
+    float min_p;       /* not above 0 (or NaN): off */
+} qwh_sampling;
+
+/* Draws one token from each of `rows` rows of `count` logits (rows back to
+ * back), beside qwh_argmax_rows; the reference decodes greedily and has no
+ * counterpart. With x_i = (l_i - max l) / temperature and w_i = exp(x_i), the
+ * row is ordered by logit, the largest first and the lower index first among
+ * equal ones; the first top_k of it are kept, of those a token while the sum
+ * before it is below top_p times their sum (the first token always), of those
+ * the ones with w_i >= min_p (min_p at most 1). ids_dev[r] = the first kept
+ * token, in that order, whose running sum exceeds uniform_dev[r] times the
+ * kept sum: uniform_dev holds given numbers in [0, 1) (below 0 and NaN count
+ * as 0, from 1 on the last kept token with a weight). A NaN logit is never
+ * drawn, nor one of -infinity beside a larger one; where the largest is
+ * +infinity, only those are drawn, evenly. A row with nothing but NaN and
+ * -infinity gives 0. params_dev: one record per row. Weights are sums of
+ * whole multiples of 2^-s (s = 62 less the bits of count), so that the draw
+ * does not depend on the order of sums; a token below half of that beside the
+ * largest is not drawn. At most 65535 rows and 2^26 logits a row. */
+int32_t qwh_sample_rows(qwh_ctx *ctx, const float *logits_dev, uint32_t rows, uint32_t count,
+                        const qwh_sampling *params_dev, const float *uniform_dev, uint32_t *ids_dev);
+
+/* ---------------------------------------------------------------------- */
+/* A q8 key/value cache in pages, shared by many sequences                 */
+/* ---------------------------------------------------------------------- */
+
+/* The reference keeps one block of max_positions rows per decoder
+ * (decoder.zig:58-65); a server keeps one pool of pages for all its
+ * sequences. A pool's four planes are [layers][pages][page_size] rows of that
+ * cache's layout (k / v scales [kv_heads*head_dim/64] f16, k / v codes
+ * [kv_heads*head_dim] u8), device memory of the caller: code planes 16-byte,
+ * scale planes 4-byte aligned. page_size is any number of positions from 1,
+ * pages * page_size below 2^32 - 1, head_dim 64, 128, 192 or 256. */
+typedef struct {
+    uint32_t layers, pages, page_size, kv_heads, head_dim;
+    uint8_t *k_scales, *k_codes, *v_scales, *v_codes;
+} qwh_paged_cache;
+
+/* A page table's entry for positions that have no page (any value from
+ * `pages` on means the same). */
+#define QWH_PAGE_NONE 0xffffffffu
+
+/* One call's new tokens: rows of the row buffers, ragged over `batch`
+ * sequences (device arrays, read when the call's kernels run). Sequence b's
+ * new tokens are the rows row_starts[b] .. row_starts[b + 1] - 1 (row_starts:
+ * batch + 1 values that never fall; NULL: row b alone), at its positions
+ * first[b], first[b] + 1, ...; its position p lives in row p % page_size of
+ * page tables[b][p / page_size]. `rows` is the number of rows the buffers
+ * hold: rows behind the last sequence's are left as they are, and no row from
+ * `rows` on is touched whatever row_starts holds. At most 65535 sequences and
+ * 2^20 rows. */
+typedef struct {
+    uint32_t batch, rows, table_pages;
+    const uint32_t *row_starts; /* [batch + 1] or NULL */
+    const uint32_t *first;      /* [batch] */
+    const uint32_t *tables;     /* [batch][table_pages] */
+} qwh_paged_batch;
+
+/* decoder.zig:180-216 between the q | k | v projection and the attention, for
+ * the new tokens of many sequences in one launch. Row i of qkv_dev (qkv_stride
+ * floats apart: heads, then kv_heads, then kv_heads head rows) holds a token's
+ * projections: each query and key head row gets RMSNorm (q_norm_dev /
+ * k_norm_dev, head_dim weights) and the rotation of its position (row p of
+ * rope_cos_dev / rope_sin_dev, [rope_positions][head_dim/2], qwh_rope_tables);
+ * the query goes to row i of query_dev (query_stride floats apart; query_dev
+ * may be qkv_dev with its stride), key and value to layer `layer`'s row of the
+ * position, as qwh_kv_append_q8 stores them. Norm and rotation are held in 64
+ * bits and rounded to f32 once, so that a stored code does not depend on how
+ * a sum is split. A token whose position has no page gets its query row
+ * only; a token at or past the end of its page table or of the tables' rows
+ * is left out. Two tokens of a call must not share a pool row. qkv_dev and
+ * query_dev 16-byte aligned, strides multiples of 4. */
+int32_t qwh_paged_append(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t layer, const qwh_paged_batch *batch,
+                         const float *qkv_dev, uint32_t qkv_stride, uint32_t heads, const float *q_norm_dev,
+                         const float *k_norm_dev, float eps, const float *rope_cos_dev, const float *rope_sin_dev,
+                         uint32_t rope_positions, float *query_dev, uint32_t query_stride);
+
+/* decodeAttentionStepQ8 (kernels.zig:697-767) of every new token over its own
+ * sequence's pages of layer `layer`: the token at position p attends to the
+ * stored positions up to p, its own among them (append first). Positions
+ * without a page are skipped; a row with none left is zeros. Row i of
+ * query_dev (query_stride floats apart, heads * head_dim values) gives row i
+ * of out_dev (heads * head_dim values, back to back); rows of no sequence are
+ * left as they are. Any number of new tokens per sequence, one among them,
+ * and any heads / kv_heads ratio. query_dev and out_dev 16-byte aligned and
+ * apart, query_stride a multiple of 4. */
+int32_t qwh_paged_attention(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t layer, const qwh_paged_batch *batch,
+                            float *out_dev, const float *query_dev, uint32_t query_stride, uint32_t heads);
+
+/* Copies pages of a pool, every layer and plane: page dst_pages[i] receives
+ * what page src_pages[i] held before the call, for i < count (host arrays, not
+ * read after the call returns). One source may go to several pages (a fork),
+ * a page may be both source and destination (a compaction, a swap); a page
+ * named as destination twice, or one from `pages` on, gives
+ * QWH_E_INVALID_ARGUMENT, before any copy. */
+int32_t qwh_paged_copy(qwh_ctx *ctx, const qwh_paged_cache *cache, const uint32_t *src_pages,
+                       const uint32_t *dst_pages, uint32_t count);
+
+/* kernels.zig:534-564 buildRopeTables for positions 0 .. positions - 1, as a
+ * decoder builds its own: cos_dev and sin_dev receive [positions][head_dim/2]
+ * f32. Built on the host and copied; returns when the copy has ended.
+ * head_dim even and at least 2, theta above 0. */
+int32_t qwh_rope_tables(qwh_ctx *ctx, uint32_t head_dim, uint32_t positions, float theta, float *cos_dev,
+                        float *sin_dev);
+
 /* ---------------------------------------------------------------------- */
 /* Audio tower and projector (model.zig:646-735)                           */
 /* ---------------------------------------------------------------------- */
@@ -555,6 +665,13 @@ int32_t qwh_decoder_generate(qwh_decoder *decoder, const uint32_t *tokens, uint3
 int32_t qwh_decoder_generate_until(qwh_decoder *decoder, const uint32_t *tokens, uint32_t max_tokens,
                                    const uint32_t *stop_tokens, uint32_t stop_count, uint32_t *ids_out,
                                    uint32_t *counts_out);
+/* Draws a token for every sequence from its last logits (those that
+ * qwh_decoder_forward, _forward_rows with want_logits or _step left on the
+ * device) by qwh_sample_rows: params and uniform are host arrays of batch
+ * records and numbers, ids_out receives batch ids. The decoder's state does
+ * not change: the caller feeds the ids to its next forward. */
+int32_t qwh_decoder_sample(qwh_decoder *decoder, const qwh_sampling *params, const float *uniform,
+                           uint32_t *ids_out);
 /* Copies sequence `seq`'s last logits (vocab f32) to the host. */
 int32_t qwh_decoder_logits(qwh_decoder *decoder, uint32_t seq, float *out, uint32_t count);
 

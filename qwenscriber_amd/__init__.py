@@ -24,7 +24,11 @@ from ._lib import (  # noqa: F401
     DecoderConfig,
     DeviceBuffer,
     ModelConfig,
+    PAGE_NONE,
+    PagedBatch,
+    PagedCache,
     QwhError,
+    Sampling,
     T_ATTN_NORM,
     T_DOWN,
     T_EMBED,

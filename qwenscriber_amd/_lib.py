@@ -22,6 +22,7 @@ DATA_BYTES = {FORMAT_Q4: 32, FORMAT_Q5: 40, FORMAT_Q8: 64}
 T_EMBED, T_Q, T_K, T_V, T_O, T_GATE, T_UP, T_DOWN, T_LM_HEAD = range(9)
 T_ATTN_NORM, T_Q_NORM, T_K_NORM, T_FFN_NORM, T_FINAL_NORM = 16, 17, 18, 19, 20
 CACHE_F32, CACHE_Q8 = 0, 1
+PAGE_NONE = 0xFFFFFFFF
 
 class AudioLayerWeights(ctypes.Structure):
     """qwh_audio_layer_weights (model.zig AudioLayer): matrix handles and
@@ -31,6 +32,28 @@ class AudioLayerWeights(ctypes.Structure):
     VECTORS = ("q_bias", "k_bias", "v_bias", "o_bias", "ffn_in_bias", "ffn_out_bias", "attention_norm_weight",
                "attention_norm_bias", "final_norm_weight", "final_norm_bias")
     _fields_ = [(name, ctypes.c_uint64) for name in MATRICES] + [(name, ctypes.c_void_p) for name in VECTORS]
+
+
+class PagedCache(ctypes.Structure):
+    """qwh_paged_cache: a pool of pages of the q8 cache, planes by device address."""
+
+    _fields_ = [(name, ctypes.c_uint32) for name in ("layers", "pages", "page_size", "kv_heads", "head_dim")] + [
+        (name, ctypes.c_void_p) for name in ("k_scales", "k_codes", "v_scales", "v_codes")]
+
+
+class PagedBatch(ctypes.Structure):
+    """qwh_paged_batch: one call's new tokens, device addresses of its arrays
+    (row_starts None: one row per sequence)."""
+
+    _fields_ = [(name, ctypes.c_uint32) for name in ("batch", "rows", "table_pages")] + [
+        (name, ctypes.c_void_p) for name in ("row_starts", "first", "tables")]
+
+
+class Sampling(ctypes.Structure):
+    """qwh_sampling: one row's temperature, top-k, top-p and min-p."""
+
+    _fields_ = [("temperature", ctypes.c_float), ("top_k", ctypes.c_uint32), ("top_p", ctypes.c_float),
+                ("min_p", ctypes.c_float)]
 
 
 class AudioFrontendWeights(ctypes.Structure):
@@ -150,6 +173,13 @@ SIGNATURES = {
     "qwh_decode_attention_q8": (_I32, [_P, _P, _P, _P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _U64, _U64]),
     "qwh_kv_append_q8": (_I32, [_P, _P, _P, _U32, _U32, _P, _P, _P, _P]),
     "qwh_argmax_rows": (_I32, [_P, _P, _U32, _U32, _P]),
+    "qwh_sample_rows": (_I32, [_P, _P, _U32, _U32, _P, _P, _P]),
+    "qwh_paged_append": (_I32, [_P, ctypes.POINTER(PagedCache), _U32, ctypes.POINTER(PagedBatch), _P, _U32, _U32, _P, _P,
+                                _F, _P, _P, _U32, _P, _U32]),
+    "qwh_paged_attention": (_I32, [_P, ctypes.POINTER(PagedCache), _U32, ctypes.POINTER(PagedBatch), _P, _P, _U32, _U32]),
+    "qwh_paged_copy": (_I32, [_P, ctypes.POINTER(PagedCache), _P, _P, _U32]),
+    "qwh_rope_tables": (_I32, [_P, _U32, _U32, _F, _P, _P]),
+    "qwh_decoder_sample": (_I32, [_P, ctypes.POINTER(Sampling), _P, _P]),
     "qwh_layer_norm": (_I32, [_P, _P, _P, _P, _P, _U32, _U32, _F]),
     "qwh_add_bias": (_I32, [_P, _P, _P, _U32, _U32]),
     "qwh_gelu": (_I32, [_P, _P, _U64]),
@@ -512,6 +542,41 @@ class Context:
         """decoder.zig:290-301 argmaxLogits of each of `rows` rows (qwh_argmax_rows)."""
         self._check(self.lib.qwh_argmax_rows(self.handle, logits_dev, rows, count, ids_dev))
 
+    def sample_rows(self, logits_dev: int, rows: int, count: int, params_dev: int, uniform_dev: int,
+                    ids_dev: int) -> None:
+        """One token of each row by temperature, top-k, top-p and min-p from
+        given uniform numbers (qwh_sample_rows); params_dev: rows Sampling records."""
+        self._check(self.lib.qwh_sample_rows(self.handle, logits_dev, rows, count, params_dev, uniform_dev, ids_dev))
+
+    # -- a q8 cache in pages -------------------------------------------------
+    def paged_append(self, cache: "PagedCache", layer: int, batch: "PagedBatch", qkv_dev: int, qkv_stride: int,
+                     heads: int, q_norm_dev: int, k_norm_dev: int, eps: float, rope_cos_dev: int, rope_sin_dev: int,
+                     rope_positions: int, query_dev: int, query_stride: int) -> None:
+        """Norm and rotation of the new tokens' queries and keys, keys and
+        values stored in their pages (qwh_paged_append)."""
+        self._check(self.lib.qwh_paged_append(self.handle, cache, layer, batch, qkv_dev, qkv_stride, heads, q_norm_dev,
+                                              k_norm_dev, eps, rope_cos_dev, rope_sin_dev, rope_positions, query_dev,
+                                              query_stride))
+
+    def paged_attention(self, cache: "PagedCache", layer: int, batch: "PagedBatch", out_dev: int, query_dev: int,
+                        query_stride: int, heads: int) -> None:
+        """Attention of the new tokens over their sequences' pages (qwh_paged_attention)."""
+        self._check(self.lib.qwh_paged_attention(self.handle, cache, layer, batch, out_dev, query_dev, query_stride,
+                                                 heads))
+
+    def paged_copy(self, cache: "PagedCache", src_pages, dst_pages) -> None:
+        """Page dst_pages[i] receives what page src_pages[i] held before the
+        call, in every layer (qwh_paged_copy)."""
+        src = np.ascontiguousarray(src_pages, np.uint32)
+        dst = np.ascontiguousarray(dst_pages, np.uint32)
+        if src.ndim != 1 or src.shape != dst.shape:
+            raise ValueError("one destination page for each source page")
+        self._check(self.lib.qwh_paged_copy(self.handle, cache, _ptr(src), _ptr(dst), src.size))
+
+    def rope_tables(self, head_dim: int, positions: int, theta: float, cos_dev: int, sin_dev: int) -> None:
+        """kernels.zig buildRopeTables into device memory (qwh_rope_tables)."""
+        self._check(self.lib.qwh_rope_tables(self.handle, head_dim, positions, theta, cos_dev, sin_dev))
+
 
 class Decoder:
     """decoder.zig Decoder over `batch` sequences (qwh_decoder_*), with a q8
@@ -613,6 +678,21 @@ class Decoder:
         self._check(self.ctx.lib.qwh_decoder_generate_until(self.handle, _ptr(tokens), max_tokens, _ptr(stops),
                                                             len(stop_tokens), _ptr(ids), _ptr(counts)))
         return ids[: max_tokens * self.batch].reshape(max_tokens, self.batch), counts
+
+    def sample(self, params, uniform) -> np.ndarray:
+        """A token for every sequence from its last logits
+        (qwh_decoder_sample): `params` one Sampling for all sequences or one
+        for each, `uniform` a number in [0, 1) for each."""
+        if isinstance(params, Sampling):
+            params = [params] * self.batch
+        params = list(params)
+        uniform = np.ascontiguousarray(uniform, np.float32).reshape(-1)
+        if len(params) != self.batch or uniform.size != self.batch:
+            raise ValueError("one Sampling record and one number for each sequence")
+        out = np.zeros(self.batch, np.uint32)
+        self._check(self.ctx.lib.qwh_decoder_sample(self.handle, (Sampling * self.batch)(*params), _ptr(uniform),
+                                                    _ptr(out)))
+        return out
 
     def logits(self, seq: int) -> np.ndarray:
         out = np.zeros(self.config.vocab, np.float32)

@@ -1256,6 +1256,27 @@ int32_t qwh_argmax_rows(qwh_ctx *ctx, const float *logits_dev, uint32_t rows, ui
                      "argmax");
 }
 
+int32_t qwh_sample_rows(qwh_ctx *ctx, const float *logits_dev, uint32_t rows, uint32_t count, const qwh_sampling *params_dev,
+                        const float *uniform_dev, uint32_t *ids_dev) {
+    if (!ctx) return QWH_E_INVALID_ARGUMENT;
+    if (rows == 0) return QWH_OK;
+    if (count == 0) return fail(ctx, QWH_E_INVALID_ARGUMENT, "a draw from an empty row");
+    if (rows > 65535) return fail(ctx, QWH_E_LIMIT_EXCEEDED, "rows %u > 65535", rows);
+    if (count > kSampleMaxCount) return fail(ctx, QWH_E_LIMIT_EXCEEDED, "count %u > 2^26", count);
+    QWH_TRY(check_device_ptr(ctx, logits_dev, "logits"));
+    QWH_TRY(check_device_ptr(ctx, params_dev, "params"));
+    QWH_TRY(check_device_ptr(ctx, uniform_dev, "uniform"));
+    QWH_TRY(check_device_ptr(ctx, ids_dev, "ids"));
+    if (((uintptr_t)logits_dev | (uintptr_t)params_dev | (uintptr_t)uniform_dev | (uintptr_t)ids_dev) & 3u)
+        return fail(ctx, QWH_E_INVALID_ARGUMENT, "logits, params, uniform and ids must be 4-byte aligned");
+    OnDevice device(ctx->device);
+    QWH_TRY(on_device(ctx, device));
+    QWH_TRY(ensure_workspace(ctx, ctx->scratch, sample_scratch_bytes(rows, count)));
+    return check_hip(ctx, launch_sample_rows(ctx->stream, logits_dev, rows, count, params_dev, uniform_dev, ctx->scratch.ptr,
+                                             ids_dev),
+                     "sample");
+}
+
 int32_t qwh_audio_projector(qwh_ctx *ctx, uint64_t in_matrix, const float *in_bias_dev, uint64_t out_matrix,
                             const float *out_bias_dev, const float *encoder_dev, uint32_t steps, float *out_dev) {
     if (!ctx) return QWH_E_INVALID_ARGUMENT;

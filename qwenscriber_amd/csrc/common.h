@@ -95,6 +95,27 @@ int32_t fail(qwh_ctx *ctx, int32_t status, const char *fmt, ...);
 // Maps a HIP error to QWH_E_DEVICE with a message, or returns QWH_OK.
 int32_t check_hip(qwh_ctx *ctx, hipError_t err, const char *what);
 int32_t ensure_workspace(qwh_ctx *ctx, Workspace &ws, size_t bytes);
+// The context's device for the length of a call, and the caller's afterwards.
+class OnDevice {
+  public:
+    explicit OnDevice(int device) {
+        if (hipGetDevice(&before_) != hipSuccess) before_ = device;
+        if (before_ != device) ok_ = hipSetDevice(device) == hipSuccess;
+        device_ = device;
+    }
+    ~OnDevice() {
+        if (before_ != device_) (void)hipSetDevice(before_);
+    }
+    bool ok() const { return ok_; }
+
+  private:
+    int before_ = 0, device_ = 0;
+    bool ok_ = true;
+};
+
+inline int32_t on_device(qwh_ctx *ctx, const OnDevice &d) {
+    return d.ok() ? QWH_OK : fail(ctx, QWH_E_DEVICE, "device %d could not be made current", ctx->device);
+}
 const Matrix *find_matrix(qwh_ctx *ctx, uint64_t handle);
 // Registers a matrix on the context and returns its handle.
 uint64_t add_matrix(qwh_ctx *ctx, const Matrix &m);
@@ -331,6 +352,14 @@ bool attention_generic_supported(uint32_t head_dim);
 size_t argmax_scratch_bytes(uint32_t rows, uint32_t count);
 hipError_t launch_argmax_rows(hipStream_t s, const float *logits, uint32_t rows, uint32_t count, void *scratch,
                               uint32_t *ids);
+// Draws of qwh_sample_rows (sample.hip); scratch holds sample_scratch_bytes.
+constexpr uint32_t kSampleMaxCount = 1u << 26;
+size_t sample_scratch_bytes(uint32_t rows, uint32_t count);
+hipError_t launch_sample_rows(hipStream_t s, const float *logits, uint32_t rows, uint32_t count,
+                              const qwh_sampling *params, const float *uniform, void *scratch, uint32_t *ids);
+// kernels.zig:534-564 buildRopeTables on the host (decoder.hip).
+void build_rope_tables(std::vector<float> &cos_t, std::vector<float> &sin_t, uint32_t half, float theta,
+                       uint32_t max_positions);
 // Scratch bytes for the range records of either form of the attention.
 size_t attention_scratch_bytes(int cus, const AttentionArgs &a);
 // Fails with hipErrorInvalidValue, launching nothing, when scratch_bytes

@@ -832,24 +832,6 @@ int32_t run_step(qwh_decoder *d, bool want_logits) {
     return check_hip(ctx, hipGraphLaunch(exec, ctx->stream), "graph launch");
 }
 
-// kernels.zig:534-564 buildRopeTables / inverseFrequency, in f32 on the host
-// as model.zig:400-407 does at load time.
-void build_rope_tables(std::vector<float> &cos_t, std::vector<float> &sin_t, uint32_t half, float theta,
-                       uint32_t max_positions) {
-    const uint32_t head_dim = half * 2;
-    cos_t.assign((size_t)max_positions * half, 0.0f);
-    sin_t.assign((size_t)max_positions * half, 0.0f);
-    for (uint32_t p = 0; p < max_positions; ++p) {
-        for (uint32_t i = 0; i < half; ++i) {
-            const volatile float exponent = -2.0f * (float)i / (float)head_dim;
-            const float inv = powf(theta, exponent);
-            const volatile float angle = (float)p * inv;
-            cos_t[(size_t)p * half + i] = cosf(angle);
-            sin_t[(size_t)p * half + i] = sinf(angle);
-        }
-    }
-}
-
 // Copies src's rows to rows row_offset + i * stride of dst (stride 1: a
 // contiguous block; stride 2: every other row, for the gate / up pairs).
 int32_t copy_rows(qwh_decoder *d, Matrix &dst, uint32_t row_offset, const Matrix &src, uint32_t stride = 1) {
@@ -915,6 +897,24 @@ int32_t check_matrix(qwh_decoder *d, const Matrix *m, uint32_t rows, uint32_t co
 size_t argmax_scratch_bytes(uint32_t rows, uint32_t count) {
     const uint32_t parts = (count + kArgmaxPerBlock - 1) / kArgmaxPerBlock;
     return (size_t)rows * parts * (sizeof(float) + sizeof(uint32_t));
+}
+
+// kernels.zig:534-564 buildRopeTables / inverseFrequency, in f32 on the host
+// as model.zig:400-407 does at load time.
+void build_rope_tables(std::vector<float> &cos_t, std::vector<float> &sin_t, uint32_t half, float theta,
+                       uint32_t max_positions) {
+    const uint32_t head_dim = half * 2;
+    cos_t.assign((size_t)max_positions * half, 0.0f);
+    sin_t.assign((size_t)max_positions * half, 0.0f);
+    for (uint32_t p = 0; p < max_positions; ++p) {
+        for (uint32_t i = 0; i < half; ++i) {
+            const volatile float exponent = -2.0f * (float)i / (float)head_dim;
+            const float inv = powf(theta, exponent);
+            const volatile float angle = (float)p * inv;
+            cos_t[(size_t)p * half + i] = cosf(angle);
+            sin_t[(size_t)p * half + i] = sinf(angle);
+        }
+    }
 }
 
 hipError_t launch_argmax_rows(hipStream_t s, const float *logits, uint32_t rows, uint32_t count, void *scratch,
@@ -1973,6 +1973,31 @@ int32_t qwh_decoder_generate_until(qwh_decoder *d, const uint32_t *tokens, uint3
         for (uint32_t r = count[b]; r < max_tokens; ++r) ids_out[(size_t)r * B + b] = 0;
     }
     return QWH_OK;
+}
+
+int32_t qwh_decoder_sample(qwh_decoder *d, const qwh_sampling *params, const float *uniform, uint32_t *ids_out) {
+    if (!d || !params || !uniform || !ids_out) return QWH_E_INVALID_ARGUMENT;
+    qwh_ctx *ctx = d->ctx;
+    OnDevice device(ctx->device);
+    QWH_TRY(on_device(ctx, device));
+    // The records, the numbers and the ids in the context's scratch, before
+    // what the draw itself needs.
+    const size_t B = d->batch, head = (B * (sizeof(qwh_sampling) + 8) + 255) & ~(size_t)255;
+    QWH_TRY(ensure_workspace(ctx, ctx->scratch, head + sample_scratch_bytes(d->batch, d->c.vocab)));
+    uint8_t *base = static_cast<uint8_t *>(ctx->scratch.ptr);
+    qwh_sampling *params_dev = reinterpret_cast<qwh_sampling *>(base);
+    float *uniform_dev = reinterpret_cast<float *>(params_dev + B);
+    uint32_t *ids_dev = reinterpret_cast<uint32_t *>(uniform_dev + B);
+    QWH_TRY(check_hip(ctx, hipMemcpyAsync(params_dev, params, B * sizeof *params, hipMemcpyHostToDevice, ctx->stream), "params"));
+    int32_t st = check_hip(ctx, hipMemcpyAsync(uniform_dev, uniform, 4 * B, hipMemcpyHostToDevice, ctx->stream), "uniform");
+    if (st == QWH_OK)
+        st = check_hip(ctx, launch_sample_rows(ctx->stream, d->logits, d->batch, d->c.vocab, params_dev, uniform_dev, base + head,
+                                               ids_dev), "sample");
+    if (st == QWH_OK)
+        st = check_hip(ctx, hipMemcpyAsync(ids_out, ids_dev, 4 * B, hipMemcpyDeviceToHost, ctx->stream), "ids");
+    // (Also after a failure: the host arrays are the caller's again.)
+    const int32_t sync = check_hip(ctx, hipStreamSynchronize(ctx->stream), "sample sync");
+    return st != QWH_OK ? st : sync;
 }
 
 int32_t qwh_decoder_logits(qwh_decoder *d, uint32_t seq, float *out, uint32_t count) {
