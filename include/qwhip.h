@@ -337,7 +337,8 @@ int32_t qwh_sample_rows(qwh_ctx *ctx, const float *logits_dev, uint32_t rows, ui
  * cache's layout (k / v scales [kv_heads*head_dim/64] f16, k / v codes
  * [kv_heads*head_dim] u8), device memory of the caller: code planes 16-byte,
  * scale planes 4-byte aligned. page_size is any number of positions from 1,
- * pages * page_size below 2^32 - 1, head_dim 64, 128, 192 or 256. */
+ * pages * page_size below 2^32 - 1, a layer's code plane below 64 GiB,
+ * head_dim 64, 128, 192 or 256. */
 typedef struct {
     uint32_t layers, pages, page_size, kv_heads, head_dim;
     uint8_t *k_scales, *k_codes, *v_scales, *v_codes;
@@ -354,8 +355,9 @@ typedef struct {
  * first[b], first[b] + 1, ...; its position p lives in row p % page_size of
  * page tables[b][p / page_size]. `rows` is the number of rows the buffers
  * hold: rows behind the last sequence's are left as they are, and no row from
- * `rows` on is touched whatever row_starts holds. At most 65535 sequences and
- * 2^20 rows. */
+ * `rows` on is touched whatever row_starts holds. At most 65535 sequences,
+ * 2^20 rows, 2^23 rows times query heads, 512 query heads per key/value head,
+ * and page tables below 2^32 - 2^16 positions. */
 typedef struct {
     uint32_t batch, rows, table_pages;
     const uint32_t *row_starts; /* [batch + 1] or NULL */

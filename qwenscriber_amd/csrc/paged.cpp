@@ -31,6 +31,8 @@ int32_t qwh_paged_append(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t la
     QWH_REFUSE(paged::check_layer(*cache, layer));
     QWH_REFUSE(paged::check_batch(batch));
     QWH_REFUSE(paged::check_heads(*cache, heads));
+    QWH_REFUSE(paged::check_positions(*cache, *batch));
+    QWH_REFUSE(paged::check_row_heads(*batch, heads));
     if (!(eps >= 0.0f)) return fail(ctx, QWH_E_INVALID_ARGUMENT, "eps is not a number from 0 on");
     if (paged::nothing_to_do(*batch)) return QWH_OK;
     const uint64_t D = cache->head_dim;
@@ -68,7 +70,10 @@ int32_t qwh_paged_attention(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t
     QWH_REFUSE(paged::check_layer(*cache, layer));
     QWH_REFUSE(paged::check_batch(batch));
     QWH_REFUSE(paged::check_heads(*cache, heads));
+    QWH_REFUSE(paged::check_positions(*cache, *batch));
+    QWH_REFUSE(paged::check_row_heads(*batch, heads));
     if (paged::nothing_to_do(*batch)) return QWH_OK;
+    QWH_REFUSE(paged::check_units(*cache, *batch, heads));
     const uint64_t width = (uint64_t)heads * cache->head_dim;
     QWH_REFUSE(paged::check_rows(query_dev, query_stride, width, "query is null", "query_stride is smaller than a row"));
     QWH_REFUSE(paged::check_rows(out_dev, (uint32_t)width, width, "out is null", ""));

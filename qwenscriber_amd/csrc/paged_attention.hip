@@ -11,13 +11,13 @@
 // Sums are f32; the softmax keeps a running maximum and sum per query row, in
 // base 2.
 //
-// The positions of a sequence are split over workgroups, by as many units of
-// kUnit positions as give the device about `target` workgroups for the whole
-// batch whatever the lengths are: lengths are device values, so every
-// workgroup works out the same split from them (paged_work). A split that is
-// not alone leaves a record (maximum, sum, weighted values) per query row,
-// and a second launch joins the records in order.
-#include <cfloat>
+// The work is one line of units (kTileRows query rows by kUnit positions), a
+// sequence's row tiles one after another, and each workgroup takes an equal
+// stretch of it, whatever the lengths are. Lengths are device values, so every
+// workgroup works out the line from them (WorkLine). A stretch that begins or
+// ends inside a tile's positions leaves a record (maximum, sum, weighted
+// values) per query row, and a second launch joins the records in order.
+#include <cmath>
 
 #include "common.h"
 #include "paged.h"
@@ -26,24 +26,33 @@ namespace qwh {
 namespace {
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr uint32_t kUnit = 128;     // positions: one round of a workgroup
-constexpr uint32_t kTileRows = 16;  // query rows of a workgroup
+constexpr uint32_t kTileRows = 8;   // query rows of a workgroup
+constexpr uint32_t kDies = 8;
 
 struct KernelArgs {
     PagedAttentionArgs p;
     uint32_t held;          // positions a page table holds
     uint32_t ratio;         // query heads per key/value head
-    uint32_t target;        // workgroups wanted
+    uint32_t ratio_magic;   // floor(2^32 / ratio) + 1 (0: ratio 1)
+    uint32_t page_shift;    // log2 of page_size (32: not a power of two)
+    uint32_t stretches_most;  // stretches that the records are for
+    float inverse_stretches;
     float scaling;          // log2(e) / sqrt(head_dim)
     float *values, *sums;   // records: [record][row][D] and [record][row][2]
+    u4 *plan;               // per sequence: units of a stretch, its first unit, units of a tile
 };
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 
 // New tokens of sequence b (0 past the batch) and positions they see.
 __device__ __forceinline__ uint32_t new_tokens(const qwh_paged_batch &batch, uint32_t b) {
@@ -53,75 +62,81 @@ __device__ __forceinline__ uint32_t new_tokens(const qwh_paged_batch &batch, uin
     return end > begin ? end - begin : 0;
 }
 
-__device__ __forceinline__ uint32_t seen_positions(const KernelArgs &a, uint32_t b, uint32_t n) {
-    if (n == 0) return 0;
-    const uint64_t end = (uint64_t)a.p.batch.first[b] + n;
-    return end < a.held ? (uint32_t)end : a.held;
+__device__ __forceinline__ uint32_t row_tiles(const KernelArgs &a, uint32_t n) { return (n * a.ratio + kTileRows - 1) / kTileRows; }
+
+// f / ratio for f up to 2^23 + kTileRows (ratio at most 512).
+__device__ __forceinline__ uint32_t by_ratio(const KernelArgs &a, uint32_t f) {
+    return a.ratio_magic ? __umulhi(f, a.ratio_magic) : f;
 }
 
-// The whole batch's split: units of a workgroup, from the sum over the
-// sequences of row tiles times units. By a whole wavefront.
-__device__ __forceinline__ uint32_t split_units(const KernelArgs &a, int lane) {
-    uint64_t total = 0;
-    for (uint32_t base = 0; base < a.p.batch.batch; base += 64) {
-        const uint32_t b = base + lane, n = new_tokens(a.p.batch, b);
-        const uint64_t tiles = ((uint64_t)n * a.ratio + kTileRows - 1) / kTileRows;
-        total += tiles * ((seen_positions(a, b, n) + kUnit - 1) / kUnit);
+// The line's length is below this for starts that never fall (the host holds
+// rows and positions to it); sums stop here, so that others cannot wrap.
+constexpr uint32_t kMostUnits = 0x7fffffffu;
+
+__device__ __forceinline__ uint32_t add_units(uint32_t a, uint32_t b) { return min(a + b, kMostUnits); }
+
+// Inclusive sums over the wavefront, in lane order.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v = add_units(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, true));   // row_shr:1
+    v = add_units(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, true));   // row_shr:2
+    v = add_units(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, true));   // row_shr:4
+    v = add_units(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, true));   // row_shr:8
+    v = add_units(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false));  // row_bcast:15
+    v = add_units(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false));  // row_bcast:31
+    return v;
+}
+
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+
+// The line of units, 64 sequences of it at a time (a lane each). By a whole
+// wavefront; what is found is uniform.
+struct WorkLine {
+    uint32_t base = 0;            // the first of the 64 sequences
+    uint32_t before = 0;          // units before them
+    uint32_t n, first, units, upto;  // this lane's sequence: new tokens, its first position, units of a row tile, units up to its end
+
+    __device__ void load(const KernelArgs &a, int lane) {
+        const qwh_paged_batch &batch = a.p.batch;
+        const uint32_t b = base + lane;
+        n = new_tokens(batch, b);
+        first = b < batch.batch ? batch.first[b] : 0;
+        const uint64_t end = (uint64_t)first + n;
+        const uint32_t seen = n == 0 ? 0 : end < a.held ? (uint32_t)end : a.held;
+        units = (seen + kUnit - 1) / kUnit;
+        upto = wave_scan(row_tiles(a, n) * units);
     }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) total += __shfl_xor((unsigned long long)total, m, 64);
-    const uint64_t units = (total * a.p.cache.kv_heads + a.target - 1) / a.target;
-    return units > 1 ? (uint32_t)units : 1;
-}
-
-// A workgroup's part: query rows [tile * kTileRows, ...) of sequence b over
-// split `split` of `splits`; `record` counts the parts of the sequences with
-// more than one split.
-struct Work {
-    uint32_t b, n, tile, split, splits, record;
-};
-
-// Part number `item` (tiles of a sequence fastest, then its splits), or false
-// past the last. Every wavefront of the workgroup gets the same.
-__device__ __forceinline__ bool paged_work(const KernelArgs &a, uint32_t item, uint32_t units, int lane, Work &w) {
-    // (64 bits: starts that fall, against the interface, can name more rows
-    // than there are, and must not wrap into a part that is none.)
-    uint64_t before = 0;
-    uint32_t records = 0;
-    for (uint32_t base = 0; base < a.p.batch.batch; base += 64) {
-        const uint32_t b = base + lane, n = new_tokens(a.p.batch, b);
-        const uint32_t tiles = (uint32_t)(((uint64_t)n * a.ratio + kTileRows - 1) / kTileRows);
-        const uint32_t splits = ((seen_positions(a, b, n) + kUnit - 1) / kUnit + units - 1) / units;
-        const uint32_t items = tiles * splits, recorded = splits > 1 ? items : 0;
-        uint64_t sum = items;
-        uint32_t rec = recorded;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint64_t s2 = __shfl_up((unsigned long long)sum, d, 64);
-            const uint32_t r2 = __shfl_up(rec, d, 64);
-            if (lane >= d) {
-                sum += s2;
-                rec += r2;
+    // Units of the whole line (leaves the last 64 sequences loaded).
+    __device__ uint32_t length(const KernelArgs &a, int lane) {
+        load(a, lane);
+        uint32_t all = lane_of(upto, 63);
+        for (base = 64; base < a.p.batch.batch; base += 64) {
+            load(a, lane);
+            all = add_units(all, lane_of(upto, 63));
+        }
+        if (a.p.batch.batch > 64) {
+            base = 0;
+            load(a, lane);
+        } else {
+            base = 0;
+        }
+        return all;
+    }
+    // The lane of the sequence that unit `at` lies in, moving on to its 64
+    // (never back); false past the line.
+    __device__ bool find(const KernelArgs &a, uint32_t at, int lane, int &owner) {
+        for (;;) {
+            const uint64_t past = __ballot(add_units(before, upto) > at);
+            if (past) {
+                owner = __builtin_ctzll(past);
+                return true;
             }
+            before = add_units(before, lane_of(upto, 63));
+            base += 64;
+            if (base >= a.p.batch.batch) return false;
+            load(a, lane);
         }
-        const uint64_t past = __ballot(before + sum > item);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            const uint32_t rest = __shfl((uint32_t)(item - before - (sum - items)), at, 64);
-            const uint32_t t = __shfl(tiles, at, 64);
-            w.b = base + at;
-            w.n = __shfl(n, at, 64);
-            w.splits = __shfl(splits, at, 64);
-            w.split = rest / t;
-            w.tile = rest - w.split * t;
-            w.record = records + __shfl(rec - recorded, at, 64) + rest;
-            return true;
-        }
-        before += __shfl((unsigned long long)sum, 63, 64);
-        records += __shfl(rec, 63, 64);
     }
-    return false;
-}
+};
 
 // Eight codes (two words) as f16 (u - 128) * 2^-9: a byte in a 16-bit half is
 // u * 2^-24, a subnormal that the multiply-add takes as it is.
@@ -153,92 +168,180 @@ __device__ __forceinline__ h8 codes_across(const uint32_t (&w)[8]) {
 }
 
 // x as hi + lo, both f16 (rounded to nearest, together 2^-22 of x).
-__device__ __forceinline__ void two_terms(const float (&x)[8], h8 &hi, h8 &lo) {
+__device__ __forceinline__ void two_terms(const float (&x)[4], u2 &hi, u2 &lo) {
+    h4 h, l;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) hi[i] = (_Float16)x[i];
+    for (int i = 0; i < 4; ++i) h[i] = (_Float16)x[i];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) lo[i] = (_Float16)(x[i] - (float)hi[i]);
+    for (int i = 0; i < 4; ++i) l[i] = (_Float16)(x[i] - (float)h[i]);
+    hi = __builtin_bit_cast(u2, h);
+    lo = __builtin_bit_cast(u2, l);
 }
 
 __device__ __forceinline__ f4 mma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-// The largest of a value over the four lanes that share lane % 16.
-__device__ __forceinline__ float quarters_max(float v) {
+// Over the eight lanes of a query row: those that share lane % 8.
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, dev::xor_lane<8>(v));
     v = fmaxf(v, dev::xor_lane<16>(v));
     return fmaxf(v, dev::xor_lane<32>(v));
 }
 
-__device__ __forceinline__ float quarters_sum(float v) {
+__device__ __forceinline__ float row_sum(float v) {
+    v += dev::xor_lane<8>(v);
     v += dev::xor_lane<16>(v);
     return v + dev::xor_lane<32>(v);
 }
 
-// Sixteen query rows (columns of the products) over a range of positions.
-// Each of the four wavefronts takes every fourth 32 positions by itself, two
-// blocks of 16:
-//   scores  [position][row] = K [16 x 32 values] Q^T, lane l: row l % 16,
-//           positions 4 * (l / 16) .. + 3 of each block;
-//   values  [dimension][row] += V^T [16 x 32 positions] P^T: the weights a
-//           lane holds are the operand P^T of its own row, if the 32
-//           positions are counted in the order (quarter, block, four), so
-//           weights never leave their lane. V^T takes lane l % 16's four
-//           dimensions of a group (one word a position), a product for each.
-// Loads go straight to registers, the next tile's before this one's products.
+// `keep` in lanes whose bit 3 is HIGH's opposite, in the others `from` of
+// lane ^ 8 (a row rotation by 8 into half of the lanes).
+template <bool HIGH>
+__device__ __forceinline__ uint32_t take_other(uint32_t keep, uint32_t from) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)keep, (int)from, 0x128, 0xF, HIGH ? 0xC : 0x3, false);
+}
+
+// Eight query rows over a range of positions. A product's sixteen columns are
+// the rows' first and second terms (lane l: column l % 16, row l % 8, term
+// l / 8 % 2), so one product takes both. Each of the four wavefronts takes
+// every fourth 32 positions by itself, two blocks of 16:
+//   scores  [position][column] = K [16 x 32 values] Q^T, lane l: positions
+//           4 * (l / 16) .. + 3 of each block. The two terms' columns are
+//           added; the first term's lane goes on with block 0, the second's
+//           with block 1;
+//   values  [dimension][column] += V^T [16 x 32 positions] P^T, in whose 32
+//           positions the order is (l / 16, block, four): a lane's weights
+//           are half of its own column's operand and half of the other
+//           term's, and change lanes only with that one. V^T takes lane
+//           l % 16's four dimensions of a group (one word a position), a
+//           product for each. The terms' sums are added at the end.
+// Two tiles of registers: one in flight while the other is used.
 template <int D>
 __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
     constexpr int G = D / 64;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = lane & 15, quarter = lane >> 4;
+    constexpr uint32_t kPieces = D / 16;  // 16-byte pieces of a head row
+    const int lane = threadIdx.x & 63, wave = (int)uniform(threadIdx.x >> 6);
+    const int n = lane & 15, quarter = lane >> 4, term = lane >> 3 & 1;
     const qwh_paged_cache &c = a.p.cache;
-    const uint32_t kvh = blockIdx.x % c.kv_heads;
-    Work work;
-    const uint32_t units = split_units(a, lane);
-    if (!paged_work(a, blockIdx.x / c.kv_heads, units, lane, work)) return;
-    const uint32_t first = a.p.batch.first[work.b];
-    const uint32_t start = a.p.batch.row_starts ? a.p.batch.row_starts[work.b] : work.b;
+    // A stretch's heads one after another on a die.
+    const uint32_t kvh = blockIdx.x / kDies % c.kv_heads;
+    const uint32_t stretch = blockIdx.x / kDies / c.kv_heads * kDies + blockIdx.x % kDies;
+    WorkLine line;
+    const uint32_t length = line.length(a, lane);
+    // (Rounded up but for the last bits of the product: at most two stretches
+    // more than wanted.)
+    const float share = ceilf((float)length * a.inverse_stretches * 0.999999f);
+    const uint32_t per = uniform(share > 1.0f ? (uint32_t)share : 1);
+    if ((uint64_t)stretch * per >= length) return;
+    const uint32_t stretch_begin = stretch * per, stretch_end = min(stretch_begin + per, length);
+
+    __shared__ uint32_t lds_rows[4][32];
+    __shared__ float lds_scale[4][2][G][32];
+    // A tile's value codes, a row every D + 16 bytes: the four rows that the
+    // lane quarters read at once then lie on different banks.
+    __shared__ __attribute__((aligned(16))) uint8_t lds_values[4][32 * (D + 16)];
+    __shared__ float lds_acc[2][kTileRows][D + 4];
+    __shared__ float lds_state[2][2][kTileRows];
+
+    const uint32_t kv_width = c.kv_heads * D, gpr = kv_width / 64;
+    for (uint32_t at = stretch_begin; at < stretch_end;) {
+    int owner;
+    if (!line.find(a, at, lane, owner)) return;
+    const uint32_t b = line.base + owner, tokens = lane_of(line.n, owner), first = lane_of(line.first, owner);
+    const uint32_t units = lane_of(line.units, owner), tiles = row_tiles(a, tokens);
+    // The sequence's first unit, and this part of one of its row tiles.
+    const uint32_t seq_begin = add_units(line.before, lane_of(line.upto, owner)) - tiles * units;
+    const uint32_t tile = uniform((at - seq_begin) / units), from = (at - seq_begin) - tile * units;
+    if (tile >= tiles) return;  // (starts that fall)
+    const uint32_t count = min(units - from, stretch_end - at);
+    const bool alone = count == units;
+    const uint32_t record = 2 * stretch + (at == stretch_begin ? 0 : 1);
+    if (at == seq_begin && kvh == 0 && threadIdx.x == 0) a.plan[b] = u4{per, seq_begin, units, 0};  // for the join
+    at += count;
+    const uint32_t start = a.p.batch.row_starts ? a.p.batch.row_starts[b] : b;
     // This lane's query row: token t, head kvh * ratio + r; it sees positions
     // up to `limit`.
-    const uint32_t f = work.tile * kTileRows + n;
-    const uint32_t t = f / a.ratio, r = f - t * a.ratio;
-    const bool active = t < work.n;
-    const uint32_t last_t = min((work.tile * kTileRows + kTileRows - 1) / a.ratio, work.n - 1);
-    const uint32_t first_t = work.tile * kTileRows / a.ratio;
+    const uint32_t f = tile * kTileRows + (n & 7);
+    const uint32_t t = by_ratio(a, f), r = f - t * a.ratio;
+    const bool active = t < tokens;
+    const uint32_t last_t = min(by_ratio(a, tile * kTileRows + kTileRows - 1), tokens - 1);
+    const uint32_t first_t = by_ratio(a, tile * kTileRows);
     const auto place = [&](uint32_t token) {  // its position, at most the tables' last
         const uint64_t p = (uint64_t)first + token;
         return p < a.held ? (uint32_t)p : a.held - 1;
     };
-    const uint32_t limit = place(t), common = place(first_t);
-    const uint32_t begin = work.split * units * kUnit;
-    uint32_t end = place(last_t) + 1;
-    if (begin >= end) return;  // (no row of the tile sees this split)
-    if (end - begin > units * kUnit) end = begin + units * kUnit;
+    const uint32_t limit = place(t), common = uniform(place(first_t));
+    const uint32_t begin = from * kUnit;
+    uint32_t end = uniform(place(last_t)) + 1;
+    if (begin >= end) continue;  // (no row of the tile sees this part)
+    if (end - begin > count * kUnit) end = begin + count * kUnit;
 
-    __shared__ uint32_t lds_rows[4][32];
-    __shared__ float lds_scale[4][2][G][32];
-    __shared__ float lds_acc[2][kTileRows][D + 4];
-    __shared__ float lds_state[2][2][kTileRows];
+    const uint32_t *table = a.p.batch.tables + (size_t)b * a.p.batch.table_pages;
+    const uint8_t *k_base = c.k_codes + kvh * D + 16 * quarter;
+    const uint8_t *v_base = c.v_codes + kvh * D;
+    // Lanes 0..31 load the key scales of position lane, 32..63 the value scales.
+    const uint16_t *scale_base = reinterpret_cast<const uint16_t *>(lane < 32 ? c.k_scales : c.v_scales) + kvh * G;
 
-    // The query row in two terms, scaled by a power of two to below 2^8.
+    // The page of this lane's position (lane % 32) of the tile at `base`. Loads
+    // complete in order: a tile's pages are asked for a tile ahead of its
+    // rows, so that they do not wait for the loads between.
+    struct Place {
+        uint32_t page, within;
+    };
+    const auto lookup = [&](uint32_t base) {
+        const uint32_t p = min(base + (lane & 31), end - 1);
+        const uint32_t at = a.page_shift < 32 ? p >> a.page_shift : p / c.page_size;
+        return Place{table[at], p - at * c.page_size};
+    };
+    struct Tile {
+        uint4 k[2][G];
+        uint4 v[2 * G];  // 16-byte piece lane + 64 j of the tile's rows
+        uint16_t scale[G];
+        uint32_t there;  // of the 32 positions, those with a row
+    };
+    const auto load = [&](Tile &tile, const Place &at, uint32_t base) {
+        const bool has_row = (at.page < c.pages) & (base + (lane & 31) < end);
+        tile.there = (uint32_t)__ballot(has_row);
+        const uint32_t safe = has_row ? at.page * c.page_size + at.within : 0;
+        // (In 16-byte pieces: a layer's code plane is below 64 GiB.)
+        if (lane < 32) lds_rows[wave][lane] = safe * (kv_width / 16);
+#pragma unroll
+        for (int g = 0; g < G; ++g) tile.scale[g] = scale_base[(size_t)safe * gpr + g];
+        wave_fence();
+        const uint32_t k0 = lds_rows[wave][n], k1 = lds_rows[wave][16 + n];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            tile.k[0][g] = *reinterpret_cast<const uint4 *>(k_base + ((size_t)k0 << 4) + 64 * g);
+            tile.k[1][g] = *reinterpret_cast<const uint4 *>(k_base + ((size_t)k1 << 4) + 64 * g);
+        }
+#pragma unroll
+        for (int j = 0; j < 2 * G; ++j) {
+            const uint32_t at = lane + 64 * j, r = lds_rows[wave][at / kPieces];
+            tile.v[j] = *reinterpret_cast<const uint4 *>(v_base + ((size_t)r << 4) + 16 * (at % kPieces));
+        }
+        // Every load of a tile is asked for before the tile in hand is used.
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    uint32_t base = begin + 32 * wave;
+    Place ahead = lookup(base), after = lookup(base + kUnit);
+
+    // This lane's term of the query row, scaled by a power of two to below 2^8.
     const size_t row = (size_t)start + t;
-    h8 qh[G][2], ql[G][2];
+    h8 q[G][2];
     float qs;
     {
-        float q[G][16];
+        f4 x[G][4];
         float top = 0.0f;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             const f4 *src = reinterpret_cast<const f4 *>(a.p.query + (active ? row * a.p.query_stride + (kvh * a.ratio + r) * D + 64 * g + 16 * quarter : 0));
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f4 v = src[i];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    q[g][4 * i + k] = active ? v[k] : 0.0f;
-                    top = fmaxf(top, fabsf(q[g][4 * i + k]));
-                }
+                x[g][i] = active ? src[i] : f4{0.0f, 0.0f, 0.0f, 0.0f};
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(x[g][i].x), fabsf(x[g][i].y)), fmaxf(fabsf(x[g][i].z), fabsf(x[g][i].w))));
             }
         }
-        top = quarters_max(top);
+        top = row_max(top);
         int e = 0;
         if (top > 0.0f && top < INFINITY) (void)__builtin_frexpf(top, &e);
         e = e < -100 ? -100 : e;
@@ -247,56 +350,15 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                float x[8];
+            for (int i = 0; i < 4; ++i) {
+                const float y[4] = {x[g][i].x * up, x[g][i].y * up, x[g][i].z * up, x[g][i].w * up};
+                u2 hi, lo;
+                two_terms(y, hi, lo);
+                const h4 mine = __builtin_bit_cast(h4, term ? lo : hi);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = q[g][8 * k + i] * up;
-                two_terms(x, qh[g][k], ql[g][k]);
+                for (int j = 0; j < 4; ++j) q[g][i / 2][4 * (i & 1) + j] = mine[j];
             }
     }
-
-    const uint32_t kv_width = c.kv_heads * D, gpr = kv_width / 64;
-    const uint32_t *table = a.p.batch.tables + (size_t)work.b * a.p.batch.table_pages;
-    const uint8_t *k_base = c.k_codes + kvh * D + 16 * quarter;
-    const uint8_t *v_base = c.v_codes + kvh * D + 4 * n;
-    // Lanes 0..31 load the key scales of position lane, 32..63 the value scales.
-    const uint16_t *scale_base = reinterpret_cast<const uint16_t *>(lane < 32 ? c.k_scales : c.v_scales) + kvh * G;
-
-    struct Tile {
-        uint4 k[2][G];
-        uint32_t v[G][8];
-        uint16_t scale[G];
-        uint32_t there;  // of the 32 positions, those with a row
-    };
-    // The pool row of this lane's position (lane % 32) of the tile at `base`.
-    const auto lookup = [&](uint32_t base) {
-        const uint32_t p = base + (lane & 31);
-        return p < end ? paged_pool_row(c, table, p) : kNoRow;
-    };
-    const auto load = [&](Tile &tile, uint32_t pool_row) {
-        tile.there = (uint32_t)__ballot(pool_row != kNoRow);
-        const uint32_t safe = pool_row != kNoRow ? pool_row : 0;
-        if (lane < 32) lds_rows[wave][lane] = safe;
-        wave_fence();
-        const uint32_t k0 = lds_rows[wave][n], k1 = lds_rows[wave][16 + n];
-        const u4 v0 = *reinterpret_cast<const u4 *>(&lds_rows[wave][4 * quarter]);
-        const u4 v1 = *reinterpret_cast<const u4 *>(&lds_rows[wave][16 + 4 * quarter]);
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            tile.k[0][g] = *reinterpret_cast<const uint4 *>(k_base + (size_t)k0 * kv_width + 64 * g);
-            tile.k[1][g] = *reinterpret_cast<const uint4 *>(k_base + (size_t)k1 * kv_width + 64 * g);
-        }
-#pragma unroll
-        for (int g = 0; g < G; ++g) tile.scale[g] = scale_base[(size_t)safe * gpr + g];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                tile.v[g][i] = *reinterpret_cast<const uint32_t *>(v_base + (size_t)v0[i] * kv_width + 64 * g);
-                tile.v[g][4 + i] = *reinterpret_cast<const uint32_t *>(v_base + (size_t)v1[i] * kv_width + 64 * g);
-            }
-        wave_fence();
-    };
 
     float m = -INFINITY, l = 0.0f;
     float e_w = -100.0f;  // acc is in units of 2^e_w
@@ -310,147 +372,145 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
 #pragma unroll
         for (int g = 0; g < G; ++g) lds_scale[wave][lane >> 5][g][lane & 31] = dev::f16_bits_to_f32(tile.scale[g]);
         wave_fence();
-        f4 s[2];
+        f4 both[2];
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
-            s[blk] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            both[blk] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const uint4 w = tile.k[blk][g];
-                const h8 ka = codes8(w.x, w.y), kb = codes8(w.z, w.w);
-                f4 x = mma(ka, ql[g][0], f4{0.0f, 0.0f, 0.0f, 0.0f});
-                x = mma(kb, ql[g][1], x);
-                x = mma(ka, qh[g][0], x);
-                x = mma(kb, qh[g][1], x);
+                f4 x = mma(codes8(w.x, w.y), q[g][0], f4{0.0f, 0.0f, 0.0f, 0.0f});
+                x = mma(codes8(w.z, w.w), q[g][1], x);
                 const f4 ks = *reinterpret_cast<const f4 *>(&lds_scale[wave][0][g][16 * blk + 4 * quarter]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[blk][i] = fmaf(ks[i], x[i], s[blk][i]);
+                for (int i = 0; i < 4; ++i) both[blk][i] = fmaf(ks[i], x[i], both[blk][i]);
             }
         }
+        float s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float s0 = both[0][i] + dev::xor_lane<8>(both[0][i]), s1 = both[1][i] + dev::xor_lane<8>(both[1][i]);
+            s[i] = term ? s1 : s0;
+        }
         const bool whole = tile.there == 0xffffffffu && base + 31 <= common;
+        const int mine = 16 * term + 4 * quarter;  // this lane's first position of the tile
         if (!whole) {
 #pragma unroll
-            for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t at = 16 * blk + 4 * quarter + i;
-                    if (!(tile.there >> at & 1u) || base + at > limit) s[blk][i] = -INFINITY;
-                }
+            for (int i = 0; i < 4; ++i)
+                if (!(tile.there >> (mine + i) & 1u) || base + mine + i > limit) s[i] = -INFINITY;
         }
-        float mx = m;
-#pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[blk][i]);
-        mx = quarters_max(mx);
+        const float mx = row_max(fmaxf(fmaxf(m, fmaxf(s[0], s[1])), fmaxf(s[2], s[3])));
         // A row that has seen nothing yet: weights of 0 against any maximum.
         const float low = (mx == -INFINITY ? 0.0f : mx) * qs;
         const float turn = fmaf(m, qs, -low);  // log2 of what earlier weights lose
         m = mx;
-        float p[8];
+        float p[4];
 #pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[4 * blk + i] = exp2_fast(fmaf(s[blk][i], qs, -low));
+        for (int i = 0; i < 4; ++i) p[i] = exp2_fast(fmaf(s[i], qs, -low));
         // The weights with their value scales, and the power of two that
         // brings the row's largest (of earlier ones too) near f16's top.
-        float w[G][8], largest = 0.0f;
+        float w[G][4], largest = 0.0f;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            const f4 s0 = *reinterpret_cast<const f4 *>(&lds_scale[wave][1][g][4 * quarter]);
-            const f4 s1 = *reinterpret_cast<const f4 *>(&lds_scale[wave][1][g][16 + 4 * quarter]);
+            const f4 vs = *reinterpret_cast<const f4 *>(&lds_scale[wave][1][g][mine]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[g][i] = p[i] * s0[i];
-                w[g][4 + i] = p[4 + i] * s1[i];
-            }
+            for (int i = 0; i < 4; ++i) w[g][i] = p[i] * vs[i];
             if (!whole) {  // (a scale that is no number must not reach rows that do not see it)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[g][i] = s[i / 4][i & 3] == -INFINITY ? 0.0f : w[g][i];
+                for (int i = 0; i < 4; ++i) w[g][i] = s[i] == -INFINITY ? 0.0f : w[g][i];
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) largest = fmaxf(largest, w[g][i]);
+            for (int i = 0; i < 4; ++i) largest = fmaxf(largest, w[g][i]);
         }
-        largest = quarters_max(largest);
+        largest = row_max(largest);
         const float e_now = fmaxf(fmaxf(e_w + ceilf(turn), (float)((int)(__float_as_uint(largest) >> 23) - 126)), -100.0f);
         if (__ballot(turn != 0.0f || e_now != e_w)) {
             l *= exp2_fast(turn);
-            const float both = exp2_fast(turn + (e_w - e_now));
+            const float less = exp2_fast(turn + (e_w - e_now));
 #pragma unroll
             for (int g = 0; g < G; ++g)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[g][i] *= both;
+                for (int i = 0; i < 4; ++i) acc[g][i] *= less;
             e_w = e_now;
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) l += p[i];
+        l += (p[0] + p[1]) + (p[2] + p[3]);
         const float up = exp2_fast(12.0f - e_w);
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[g][i] *= up;
-            h8 ph, pl;
-            two_terms(w[g], ph, pl);
-            const h8 v0 = codes_across<0>(tile.v[g]), v1 = codes_across<1>(tile.v[g]);
-            const h8 v2 = codes_across<2>(tile.v[g]), v3 = codes_across<3>(tile.v[g]);
-            acc[g][0] = mma(v0, ph, mma(v0, pl, acc[g][0]));
-            acc[g][1] = mma(v1, ph, mma(v1, pl, acc[g][1]));
-            acc[g][2] = mma(v2, ph, mma(v2, pl, acc[g][2]));
-            acc[g][3] = mma(v3, ph, mma(v3, pl, acc[g][3]));
+        for (int j = 0; j < 2 * G; ++j) {
+            const uint32_t at = lane + 64 * j;
+            *reinterpret_cast<uint4 *>(&lds_values[wave][at / kPieces * (D + 16) + at % kPieces * 16]) = tile.v[j];
         }
         wave_fence();
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            uint32_t v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v[i] = *reinterpret_cast<const uint32_t *>(
+                    &lds_values[wave][(16 * (i / 4) + 4 * quarter + (i & 3)) * (D + 16) + 64 * g + 4 * n]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[g][i] *= up;
+            u2 hi, lo;
+            two_terms(w[g], hi, lo);
+            // Block 0's four positions, then block 1's: this column's own
+            // term of its own block and of the other lane's.
+            const u4 mixed = {take_other<true>(hi.x, lo.x), take_other<true>(hi.y, lo.y),
+                              take_other<false>(lo.x, hi.x), take_other<false>(lo.y, hi.y)};
+            const h8 weights = __builtin_bit_cast(h8, mixed);
+            acc[g][0] = mma(codes_across<0>(v), weights, acc[g][0]);
+            acc[g][1] = mma(codes_across<1>(v), weights, acc[g][1]);
+            acc[g][2] = mma(codes_across<2>(v), weights, acc[g][2]);
+            acc[g][3] = mma(codes_across<3>(v), weights, acc[g][3]);
+        }
     };
 
-    uint32_t base = begin + 32 * wave;
     if (base < end) {
+        // (The loads behind the range are of pool row 0; waits count on them.)
         Tile even, odd;
-        load(even, lookup(base));
-        uint32_t ahead = lookup(base + kUnit < end ? base + kUnit : base);
-        for (;;) {
-            const uint32_t second = base + kUnit;
-            if (second < end) {
-                load(odd, ahead);
-                ahead = lookup(second + kUnit < end ? second + kUnit : second);
-            }
+        load(even, ahead, base);
+        for (; base + kUnit < end; base += 2 * kUnit) {
+            ahead = lookup(base + 2 * kUnit);
+            load(odd, after, base + kUnit);
             use(even, base);
-            if (second >= end) break;
-            base = second + kUnit;
-            if (base < end) {
-                load(even, ahead);
-                ahead = lookup(base + kUnit < end ? base + kUnit : base);
-            }
-            use(odd, second);
-            if (base >= end) break;
+            after = lookup(base + 3 * kUnit);
+            load(even, ahead, base + 2 * kUnit);
+            use(odd, base + kUnit);
         }
+        if (base < end) use(even, base);
     }
 
-    // The four wavefronts' states into the first's: 2 and 3 hand theirs to 0
-    // and 1, then 1 to 0. Maxima in base 2, values without their powers of two.
-    l = quarters_sum(l);
-    float M = m == -INFINITY ? -INFINITY : m * qs;
+    // The terms' sums, and the lanes' of l.
+    l = row_sum(l);
     const float back = exp2_fast(e_w - 12.0f) * kCodeScale;
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[g][i] *= back;
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[g][i][j] = (acc[g][i][j] + dev::xor_lane<8>(acc[g][i][j])) * back;
+    float M = m == -INFINITY ? -INFINITY : m * qs;  // in base 2
+    const int slot_row = n & 7;
+    const bool writes = term == 0;
+    // The four wavefronts' states into the first's: 2 and 3 hand theirs to 0
+    // and 1, then 1 to 0.
 #pragma unroll
     for (int half = 2; half >= 1; half /= 2) {
-        if (wave >= half && wave < 2 * half) {
+        if (wave >= half && wave < 2 * half && writes) {
             const int slot = wave - half;
             if (quarter == 0) {
-                lds_state[slot][0][n] = M;
-                lds_state[slot][1][n] = l;
+                lds_state[slot][0][slot_row] = M;
+                lds_state[slot][1][slot_row] = l;
             }
 #pragma unroll
             for (int g = 0; g < G; ++g)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<f4 *>(&lds_acc[slot][n][64 * g + 16 * quarter + 4 * i]) =
+                    *reinterpret_cast<f4 *>(&lds_acc[slot][slot_row][64 * g + 16 * quarter + 4 * i]) =
                         f4{acc[g][0][i], acc[g][1][i], acc[g][2][i], acc[g][3][i]};
         }
         __syncthreads();
         if (wave < half) {
-            const float m2 = lds_state[wave][0][n], l2 = lds_state[wave][1][n];
+            const float m2 = lds_state[wave][0][slot_row], l2 = lds_state[wave][1][slot_row];
             const float top = fmaxf(M, m2), low = top == -INFINITY ? 0.0f : top;
             const float f1 = exp2_fast(M - low), f2 = exp2_fast(m2 - low);
             M = top;
@@ -459,16 +519,16 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
             for (int g = 0; g < G; ++g)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const f4 other = *reinterpret_cast<const f4 *>(&lds_acc[wave][n][64 * g + 16 * quarter + 4 * i]);
+                    const f4 other = *reinterpret_cast<const f4 *>(&lds_acc[wave][slot_row][64 * g + 16 * quarter + 4 * i]);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) acc[g][k][i] = acc[g][k][i] * f1 + other[k] * f2;
                 }
         }
         __syncthreads();
     }
-    if (wave != 0 || !active) return;
-    if (work.splits > 1) {
-        const size_t rec = ((size_t)work.record * c.kv_heads + kvh) * kTileRows + n;
+    if (wave != 0 || !active || !writes) continue;
+    if (!alone) {
+        const size_t rec = ((size_t)record * c.kv_heads + kvh) * kTileRows + slot_row;
         if (quarter == 0) {
             a.sums[2 * rec] = M;
             a.sums[2 * rec + 1] = l;
@@ -479,7 +539,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
             for (int i = 0; i < 4; ++i)
                 *reinterpret_cast<f4 *>(a.values + rec * D + 64 * g + 16 * quarter + 4 * i) =
                     f4{acc[g][0][i], acc[g][1][i], acc[g][2][i], acc[g][3][i]};
-        return;
+        continue;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     float *out = a.p.out + (row * a.p.heads + kvh * a.ratio + r) * D + 16 * quarter;
@@ -489,41 +549,35 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
         for (int i = 0; i < 4; ++i)
             *reinterpret_cast<f4 *>(out + 64 * g + 4 * i) =
                 f4{acc[g][0][i] * inv, acc[g][1][i] * inv, acc[g][2][i] * inv, acc[g][3][i] * inv};
+    }
 }
 
 // Joins the records of a query row (one wavefront) in the order of its
-// splits. Rows of sequences with one split were written by their workgroup.
+// positions. Rows whose tile one workgroup took whole were written by it.
 template <int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(const KernelArgs a, uint32_t rows) {
     constexpr int G = D / 64;
     const int lane = threadIdx.x & 63;
     const uint64_t unit = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const uint32_t row = (uint32_t)(unit / a.p.heads), h = (uint32_t)(unit % a.p.heads);
+    const uint32_t row = uniform((uint32_t)(unit / a.p.heads)), h = uniform((uint32_t)(unit % a.p.heads));
     if (row >= rows) return;
     uint32_t b, t;
     if (!paged_row(a.p.batch, row, lane, b, t)) return;
-    const uint32_t units = split_units(a, lane);
-    // The sequence's first record.
-    uint32_t records = 0, splits = 0, tiles = 0;
-    for (uint32_t base = 0; base <= b; base += 64) {
-        const uint32_t s = base + lane, n = new_tokens(a.p.batch, s);
-        const uint32_t s_tiles = (uint32_t)(((uint64_t)n * a.ratio + kTileRows - 1) / kTileRows);
-        const uint32_t s_splits = ((seen_positions(a, s, n) + kUnit - 1) / kUnit + units - 1) / units;
-        uint32_t mine = s < b && s_splits > 1 ? s_tiles * s_splits : 0;
-#pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) mine += __shfl_xor(mine, m, 64);
-        records += mine;
-        if (b - base < 64) {
-            splits = (uint32_t)__builtin_amdgcn_readlane((int)s_splits, (int)(b - base));
-            tiles = (uint32_t)__builtin_amdgcn_readlane((int)s_tiles, (int)(b - base));
-        }
-    }
-    if (splits <= 1) return;
+    b = uniform(b);
+    t = uniform(t);
+    const u4 plan = a.plan[b];
+    const uint64_t seen64 = (uint64_t)a.p.batch.first[b] + t + 1;
+    const uint32_t seen = seen64 < a.held ? (uint32_t)seen64 : a.held;
+    // (Starts that fall can leave a sequence without a plan: whatever stands
+    // there, only records are read.)
+    const uint32_t per = max(plan.x, 1u), units = plan.z;
     const uint32_t kvh = h / a.ratio, f = t * a.ratio + (h - kvh * a.ratio);
-    const uint32_t tile = f / kTileRows, n = f - tile * kTileRows;
-    const uint64_t seen = (uint64_t)a.p.batch.first[b] + t + 1;
-    const uint32_t span = units * kUnit;
-    const uint32_t used = ((seen < a.held ? (uint32_t)seen : a.held) + span - 1) / span;
+    const uint32_t tile = f / kTileRows, slot = f - tile * kTileRows;
+    const uint32_t begin = plan.y + tile * units;  // the tile's units
+    const uint32_t first = begin / per, last = (begin + units - 1) / per;
+    if (first == last) return;
+    // Stretches that hold positions this row sees.
+    const uint32_t used = min(min(last, (begin + (seen - 1) / kUnit) / per) - first + 1, a.stretches_most);
     float M = -INFINITY, L = 0.0f, acc[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) acc[g] = 0.0f;
@@ -531,8 +585,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const KernelArgs a, uin
         float m[4], l[4], v[4][G];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const uint32_t s = min(s0 + k, used - 1);
-            const size_t rec = ((size_t)(records + s * tiles + tile) * a.p.cache.kv_heads + kvh) * kTileRows + n;
+            const uint32_t s = min(first + min(s0 + k, used - 1), a.stretches_most - 1);
+            const size_t rec = ((size_t)(2 * s + (s * per < begin ? 1 : 0)) * a.p.cache.kv_heads + kvh) * kTileRows + slot;
             m[k] = a.sums[2 * rec];
             l[k] = a.sums[2 * rec + 1];
 #pragma unroll
@@ -554,27 +608,30 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const KernelArgs a, uin
     for (int g = 0; g < G; ++g) a.p.out[((size_t)row * a.p.heads + h) * D + 64 * g + lane] = acc[g] * inv;
 }
 
-// Workgroups wanted: three on a CU at once.
-uint32_t target_groups(int cus) { return 3u * (uint32_t)(cus > 0 ? cus : 256); }
+// Workgroups that a CU holds at once, by the kernel's registers.
+uint32_t resident_groups(uint32_t head_dim) { return head_dim == 64 ? 3 : 2; }
 
-// Records: parts of sequences of two splits and more. Each has at most twice
-// its units' share of the target.
-uint64_t max_records(int cus, const PagedAttentionArgs &a) {
-    return (2ull * target_groups(cus) + a.cache.kv_heads - 1) / a.cache.kv_heads * a.cache.kv_heads;
+// Stretches of a key/value head: as many workgroups as the device holds.
+uint32_t wanted_stretches(int cus, const PagedAttentionArgs &a) {
+    const uint32_t groups = resident_groups(a.cache.head_dim) * (uint32_t)(cus > 0 ? cus : 256);
+    return groups > a.cache.kv_heads ? groups / a.cache.kv_heads : 1;
 }
+
+// Stretches at most: the division's rounding, and a whole round of the dies.
+uint32_t most_stretches(int cus, const PagedAttentionArgs &a) { return (wanted_stretches(cus, a) + 2 + kDies - 1) / kDies * kDies; }
+
+// Two records (of kTileRows rows) a stretch and head.
+uint64_t record_rows(int cus, const PagedAttentionArgs &a) { return 2ull * most_stretches(cus, a) * a.cache.kv_heads * kTileRows; }
 
 template <int D>
 hipError_t launch_attention(hipStream_t s, int cus, const KernelArgs &k) {
     const qwh_paged_batch &b = k.p.batch;
-    // Row tiles at most: whole ones of all rows, and one more a sequence.
-    const uint64_t tiles = b.row_starts ? (uint64_t)b.rows * k.ratio / kTileRows + (b.batch < b.rows ? b.batch : b.rows)
-                                        : (uint64_t)b.batch * ((k.ratio + kTileRows - 1) / kTileRows);
-    const uint64_t blocks = (k.target / k.p.cache.kv_heads + tiles) * k.p.cache.kv_heads;
     const uint32_t rows = b.row_starts ? b.rows : b.batch;
     const uint64_t join = ((uint64_t)rows * k.p.heads + 3) / 4;
+    const uint64_t blocks = (uint64_t)most_stretches(cus, k.p) * k.p.cache.kv_heads;
     if (blocks > 0xffffffu || join > 0xffffffu) return hipErrorInvalidValue;
     paged_few_kernel<D><<<(uint32_t)blocks, 256, 0, s>>>(k);
-    // (One unit in all: nothing to join.)
+    // (Tiles of one unit: nothing to join.)
     if (k.held > kUnit) paged_join_kernel<D><<<(uint32_t)join, 256, 0, s>>>(k, rows);
     return hipGetLastError();
 }
@@ -582,20 +639,23 @@ hipError_t launch_attention(hipStream_t s, int cus, const KernelArgs &k) {
 }  // namespace
 
 size_t paged_attention_scratch_bytes(int cus, const PagedAttentionArgs &a) {
-    return max_records(cus, a) * kTileRows * (a.cache.head_dim + 2) * sizeof(float) + 256;
+    return a.batch.batch * sizeof(u4) + record_rows(cus, a) * (a.cache.head_dim + 2) * sizeof(float);
 }
 
 hipError_t launch_paged_attention(hipStream_t s, int cus, const PagedAttentionArgs &a, void *scratch, size_t scratch_bytes) {
     if (paged_attention_scratch_bytes(cus, a) > scratch_bytes) return hipErrorInvalidValue;
     KernelArgs k{};
     k.p = a;
-    const uint64_t held = (uint64_t)a.batch.table_pages * a.cache.page_size;
-    k.held = held < 0xfffffff0ull ? (uint32_t)held : 0xfffffff0u;
+    k.held = a.batch.table_pages * a.cache.page_size;  // (check_positions)
     k.ratio = a.heads / a.cache.kv_heads;
-    k.target = target_groups(cus);
+    k.ratio_magic = k.ratio == 1 ? 0 : (uint32_t)((1ull << 32) / k.ratio) + 1;
+    k.page_shift = (a.cache.page_size & (a.cache.page_size - 1)) ? 32 : (uint32_t)__builtin_ctz(a.cache.page_size);
+    k.stretches_most = most_stretches(cus, a);
+    k.inverse_stretches = 1.0f / (float)wanted_stretches(cus, a);
     k.scaling = kLog2e / sqrtf((float)a.cache.head_dim);
-    k.values = static_cast<float *>(scratch);
-    k.sums = k.values + max_records(cus, a) * kTileRows * a.cache.head_dim;
+    k.plan = static_cast<u4 *>(scratch);
+    k.values = reinterpret_cast<float *>(k.plan + a.batch.batch);
+    k.sums = k.values + record_rows(cus, a) * a.cache.head_dim;
     switch (a.cache.head_dim) {
     case 64: return launch_attention<64>(s, cus, k);
     case 128: return launch_attention<128>(s, cus, k);

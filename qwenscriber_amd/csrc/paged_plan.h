@@ -16,6 +16,8 @@ namespace paged {
 constexpr uint32_t kMaxBatch = 65535;
 constexpr uint32_t kMaxRows = 1u << 20;
 constexpr uint32_t kMaxHeads = 4096;
+constexpr uint64_t kMaxRowHeads = 1u << 23;
+constexpr uint32_t kMaxRatio = 512;
 
 // A refusal: a status and why, or QWH_OK.
 struct Refusal {
@@ -41,6 +43,8 @@ inline Refusal check_cache(const qwh_paged_cache *c) {
         return refuse(QWH_E_LIMIT_EXCEEDED, "pages * page_size of 2^32 - 1 or more");
     if ((unsigned __int128)c->pages * c->page_size * c->layers * c->kv_heads * c->head_dim >> 62)
         return refuse(QWH_E_LIMIT_EXCEEDED, "the pool's planes pass 2^62 bytes");
+    if ((uint64_t)c->pages * c->page_size * c->kv_heads * (c->head_dim / 16) >> 32)
+        return refuse(QWH_E_LIMIT_EXCEEDED, "a layer's code plane of 64 GiB or more");
     if (!c->k_scales || !c->k_codes || !c->v_scales || !c->v_codes)
         return refuse(QWH_E_INVALID_ARGUMENT, "a pool plane is null");
     if (!aligned(c->k_codes, 16) || !aligned(c->v_codes, 16))
@@ -67,12 +71,35 @@ inline Refusal check_batch(const qwh_paged_batch *b) {
     return {};
 }
 
+// Positions are 32-bit counts, with room to step past the last one.
+inline Refusal check_positions(const qwh_paged_cache &c, const qwh_paged_batch &b) {
+    if ((uint64_t)b.table_pages * c.page_size >= 0xffff0000ull)
+        return refuse(QWH_E_LIMIT_EXCEEDED, "page tables of 2^32 - 2^16 positions or more");
+    return {};
+}
+
 inline bool nothing_to_do(const qwh_paged_batch &b) { return b.batch == 0 || (b.row_starts && b.rows == 0); }
 
 inline Refusal check_heads(const qwh_paged_cache &c, uint32_t heads) {
     if (heads == 0 || heads % c.kv_heads != 0)
         return refuse(QWH_E_SHAPE_MISMATCH, "heads is not a multiple of kv_heads");
     if (heads > kMaxHeads) return refuse(QWH_E_LIMIT_EXCEEDED, "more than 4096 heads");
+    if (heads / c.kv_heads > kMaxRatio) return refuse(QWH_E_LIMIT_EXCEEDED, "more than 512 heads per kv head");
+    return {};
+}
+
+// (The grids' 32 bits.)
+inline Refusal check_row_heads(const qwh_paged_batch &b, uint32_t heads) {
+    if ((uint64_t)b.rows * heads > kMaxRowHeads) return refuse(QWH_E_LIMIT_EXCEEDED, "rows * heads of more than 2^23");
+    return {};
+}
+
+// The attention counts units of 8 query rows (of a kv head) by 128 positions
+// in 31 bits: rows in whole tiles, and one tile more a sequence.
+inline Refusal check_units(const qwh_paged_cache &c, const qwh_paged_batch &b, uint32_t heads) {
+    const uint64_t tiles = (uint64_t)b.rows * (heads / c.kv_heads) / 8 + (b.batch < b.rows ? b.batch : b.rows);
+    if (tiles * (((uint64_t)b.table_pages * c.page_size + 127) / 128) >= 0x7fffffffull)
+        return refuse(QWH_E_LIMIT_EXCEEDED, "rows times heads per kv head times positions past 2^41");
     return {};
 }
 

@@ -140,9 +140,11 @@ void check_refusals() {
     cache(QWH_E_UNSUPPORTED, "head_dim 320", [](auto &c) { c.head_dim = 320; });
     cache(QWH_E_LIMIT_EXCEEDED, "heads", [](auto &c) { c.kv_heads = 4097; });
     cache(QWH_E_LIMIT_EXCEEDED, "2^32 - 1 rows", [](auto &c) { c.pages = 0xffffffffu, c.page_size = 1; });
-    cache(QWH_OK, "2^32 - 2 rows", [](auto &c) { c.pages = 0xfffffffeu, c.page_size = 1, c.kv_heads = 1; });
+    cache(QWH_OK, "2^30 rows", [](auto &c) { c.pages = 1u << 30, c.page_size = 1, c.kv_heads = 1, c.head_dim = 64, c.pages -= 1; });
     cache(QWH_E_LIMIT_EXCEEDED, "2^33 rows", [](auto &c) { c.pages = 1u << 17, c.page_size = 1u << 16; });
     cache(QWH_E_LIMIT_EXCEEDED, "bytes", [](auto &c) { c.layers = 0xffffffffu, c.pages = 1u << 28, c.page_size = 8; });
+    cache(QWH_E_LIMIT_EXCEEDED, "64 GiB", [](auto &c) { c.pages = 1u << 22, c.page_size = 16; });
+    cache(QWH_OK, "below 64 GiB", [](auto &c) { c.pages = (1u << 22) - 1, c.page_size = 16; });
     cache(QWH_E_INVALID_ARGUMENT, "null scales", [](auto &c) { c.k_scales = nullptr; });
     cache(QWH_E_INVALID_ARGUMENT, "null codes", [](auto &c) { c.v_codes = nullptr; });
     cache(QWH_E_INVALID_ARGUMENT, "codes' alignment", [](auto &c) { c.k_codes += 8; });
@@ -169,11 +171,23 @@ void check_refusals() {
     batch(QWH_E_LIMIT_EXCEEDED, "sequences", [](auto &b) { b.batch = 65536; });
     batch(QWH_E_LIMIT_EXCEEDED, "rows", [](auto &b) { b.rows = (1u << 20) + 1; });
 
+    qwh_paged_batch tall = rows;
+    tall.table_pages = 0xfffefff;
+    expect(paged::check_positions(good, tall).status == QWH_OK, "positions below the limit");
+    ++tall.table_pages;
+    expect(paged::check_positions(good, tall).status == QWH_E_LIMIT_EXCEEDED, "positions");
+    expect(paged::check_row_heads(rows, 4096).status == QWH_OK, "rows times heads");
+    tall.rows = 1u << 20;
+    expect(paged::check_row_heads(tall, 8).status == QWH_OK, "2^23 rows times heads");
+    expect(paged::check_row_heads(tall, 9).status == QWH_E_LIMIT_EXCEEDED, "past 2^23 rows times heads");
     expect(paged::check_heads(good, 16).status == QWH_OK, "16 over 8");
     expect(paged::check_heads(good, 24).status == QWH_OK, "24 over 8");
     expect(paged::check_heads(good, 0).status == QWH_E_SHAPE_MISMATCH, "no query head");
     expect(paged::check_heads(good, 12).status == QWH_E_SHAPE_MISMATCH, "12 over 8");
     expect(paged::check_heads(good, 4104).status == QWH_E_LIMIT_EXCEEDED, "4104 heads");
+    const qwh_paged_cache narrow{1, 1, 1, 1, 64, plane, plane, plane, plane};
+    expect(paged::check_heads(narrow, 512).status == QWH_OK, "512 over 1");
+    expect(paged::check_heads(narrow, 513).status == QWH_E_LIMIT_EXCEEDED, "513 over 1");
     expect(paged::check_rows(plane, 2048, 2048, "", "").status == QWH_OK, "rows");
     expect(paged::check_rows(plane, 2050, 2048, "", "").status == QWH_E_INVALID_ARGUMENT, "an odd stride");
     expect(paged::check_rows(plane + 4, 2048, 2048, "", "").status == QWH_E_INVALID_ARGUMENT, "rows' alignment");
