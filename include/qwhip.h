@@ -356,7 +356,7 @@ typedef struct {
  * page tables[b][p / page_size]. `rows` is the number of rows the buffers
  * hold: rows behind the last sequence's are left as they are, and no row from
  * `rows` on is touched whatever row_starts holds. At most 65535 sequences,
- * 2^20 rows, 2^23 rows times query heads, 512 query heads per key/value head,
+ * 2^20 rows, 2^23 rows times query heads, 256 query heads per key/value head,
  * and page tables below 2^32 - 2^16 positions. */
 typedef struct {
     uint32_t batch, rows, table_pages;

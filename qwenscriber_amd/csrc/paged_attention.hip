@@ -18,6 +18,7 @@
 // ends inside a tile's positions leaves a record (maximum, sum, weighted
 // values) per query row, and a second launch joins the records in order.
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 #include "paged.h"
@@ -36,6 +37,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr uint32_t kUnit = 128;     // positions: one round of a workgroup
 constexpr uint32_t kTileRows = 8;   // query rows of a workgroup
 constexpr uint32_t kDies = 8;
+// Sequences of more query rows a key/value head take paged_many_kernel.
+constexpr uint32_t kFewRows = 32;
 
 struct KernelArgs {
     PagedAttentionArgs p;
@@ -47,7 +50,12 @@ struct KernelArgs {
     float inverse_stretches;
     float scaling;          // log2(e) / sqrt(head_dim)
     float *values, *sums;   // records: [record][row][D] and [record][row][2]
-    u4 *plan;               // per sequence: units of a stretch, its first unit, units of a tile
+    // Sequences of up to few_rows query rows a kv head take paged_few_kernel,
+    // the others paged_many_kernel.
+    uint32_t few_rows, stretches_most_many;
+    float inverse_stretches_many;
+    float *values_many, *sums_many;
+    u4 *plan;               // per sequence: units of a stretch, its first unit, units of a tile (many: whole_units), 1: many
 };
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -62,9 +70,14 @@ __device__ __forceinline__ uint32_t new_tokens(const qwh_paged_batch &batch, uin
     return end > begin ? end - begin : 0;
 }
 
-__device__ __forceinline__ uint32_t row_tiles(const KernelArgs &a, uint32_t n) { return (n * a.ratio + kTileRows - 1) / kTileRows; }
+__device__ __forceinline__ uint32_t row_tiles(const KernelArgs &a, uint32_t n, uint32_t rows = kTileRows) {
+    return (n * a.ratio + rows - 1) / rows;
+}
 
-// f / ratio for f up to 2^23 + kTileRows (ratio at most 512).
+__device__ __forceinline__ uint32_t whole_units(const KernelArgs &a, uint32_t first);
+__device__ __forceinline__ uint32_t tiles_units(const KernelArgs &a, uint32_t whole, uint32_t j);
+
+// f / ratio for f up to 2^23 + kTileRows (ratio at most 256).
 __device__ __forceinline__ uint32_t by_ratio(const KernelArgs &a, uint32_t f) {
     return a.ratio_magic ? __umulhi(f, a.ratio_magic) : f;
 }
@@ -95,35 +108,40 @@ struct WorkLine {
     uint32_t before = 0;          // units before them
     uint32_t n, first, units, upto;  // this lane's sequence: new tokens, its first position, units of a row tile, units up to its end
 
-    __device__ void load(const KernelArgs &a, int lane) {
+    // `rows`: of a tile, which also says whose sequences these are.
+    __device__ void load(const KernelArgs &a, int lane, uint32_t rows) {
         const qwh_paged_batch &batch = a.p.batch;
         const uint32_t b = base + lane;
         n = new_tokens(batch, b);
+        if ((n * a.ratio > a.few_rows) != (rows != kTileRows)) n = 0;
         first = b < batch.batch ? batch.first[b] : 0;
-        const uint64_t end = (uint64_t)first + n;
-        const uint32_t seen = n == 0 ? 0 : end < a.held ? (uint32_t)end : a.held;
-        units = (seen + kUnit - 1) / kUnit;
-        upto = wave_scan(row_tiles(a, n) * units);
-    }
-    // Units of the whole line (leaves the last 64 sequences loaded).
-    __device__ uint32_t length(const KernelArgs &a, int lane) {
-        load(a, lane);
-        uint32_t all = lane_of(upto, 63);
-        for (base = 64; base < a.p.batch.batch; base += 64) {
-            load(a, lane);
-            all = add_units(all, lane_of(upto, 63));
-        }
-        if (a.p.batch.batch > 64) {
-            base = 0;
-            load(a, lane);
+        const uint32_t tiles = row_tiles(a, n, rows);
+        if (rows == kTileRows) {
+            const uint64_t end = (uint64_t)first + n;
+            const uint32_t seen = n == 0 ? 0 : end < a.held ? (uint32_t)end : a.held;
+            units = (seen + kUnit - 1) / kUnit;
+            upto = wave_scan(tiles * units);
         } else {
+            upto = wave_scan(tiles_units(a, whole_units(a, first), tiles));
+        }
+    }
+    // Units of the whole line (leaves its first 64 sequences loaded).
+    __device__ uint32_t length(const KernelArgs &a, int lane, uint32_t rows = kTileRows) {
+        load(a, lane, rows);
+        uint32_t all = lane_of(upto, 63);
+        if (a.p.batch.batch > 64) {
+            for (base = 64; base < a.p.batch.batch; base += 64) {
+                load(a, lane, rows);
+                all = add_units(all, lane_of(upto, 63));
+            }
             base = 0;
+            load(a, lane, rows);
         }
         return all;
     }
     // The lane of the sequence that unit `at` lies in, moving on to its 64
     // (never back); false past the line.
-    __device__ bool find(const KernelArgs &a, uint32_t at, int lane, int &owner) {
+    __device__ bool find(const KernelArgs &a, uint32_t at, int lane, int &owner, uint32_t rows = kTileRows) {
         for (;;) {
             const uint64_t past = __ballot(add_units(before, upto) > at);
             if (past) {
@@ -133,7 +151,7 @@ struct WorkLine {
             before = add_units(before, lane_of(upto, 63));
             base += 64;
             if (base >= a.p.batch.batch) return false;
-            load(a, lane);
+            load(a, lane, rows);
         }
     }
 };
@@ -420,7 +438,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
                 for (int i = 0; i < 4; ++i) w[g][i] = s[i] == -INFINITY ? 0.0f : w[g][i];
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) largest = fmaxf(largest, w[g][i]);
+            for (int i = 0; i < 4; ++i) largest = fmaxf(largest, fabsf(w[g][i]));
         }
         largest = row_max(largest);
         const float e_now = fmaxf(fmaxf(e_w + ceilf(turn), (float)((int)(__float_as_uint(largest) >> 23) - 126)), -100.0f);
@@ -552,6 +570,456 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
     }
 }
 
+// ---- many query rows ----
+//
+// 128 query rows of a workgroup, 32 a wavefront, over 64 positions at a time
+// that the four wavefronts share: codes are turned into f16 once, on their way
+// to LDS (keys by position, values by dimension), and read from there as
+// operands of 32 x 32 x 16 products, each by both terms of the queries or
+// weights:
+//   scores  [position][row] = K Q^T, two blocks of 32 positions. Lane l holds
+//           row l % 32, positions 8 i + 4 (l / 32) + 0..3 of a block;
+//   values  [dimension][row] += V^T P^T, 16 positions at a time, counted in
+//           that order, so that weights stay in their lane.
+// Value scales: with vm the largest of a position's, the softmax runs over
+// score + log2(vm), so its weights P = p vm are at most 1 (2^3: the maximum
+// they are taken against moves only when it is passed by more) and so are
+// P vs / vm; the sum is of P / vm. Both terms of 2^12 P vs / vm then keep
+// 2^-22 of the row's largest.
+// Two LDS buffers and a barrier a tile: tile i + 1 is converted and tile i + 2
+// asked for at the start of tile i. Issue bound: of about 2600 cycles a
+// wavefront and tile (head_dim 128) the matrix cores work 2048.
+constexpr int kManyRows = 128;
+constexpr int kManyPositions = 64;
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+template <int D>
+struct ManyLayout {
+    static constexpr int G = D / 64;
+    static constexpr int kKeys = 0;                                  // [64][D] f16
+    static constexpr int kValues = kManyPositions * D * 2;           // [D][64] f16
+    static constexpr int kScales = kValues + D * kManyPositions * 2;  // [2 G + 2][64] f32: key scales, log2(vm), 1 / vm, 2^12 vs / vm
+    static constexpr int kBuffer = kScales + (2 * G + 2) * kManyPositions * 4;
+    static constexpr int kRows = 2 * kBuffer;                        // [4][64] pool rows in 16-byte pieces
+    static constexpr int kPoolRows = kRows + 4 * kManyPositions * 4;  // [4][64] pool rows
+    static constexpr int kThere = kPoolRows + 4 * kManyPositions * 4;  // [4] u64
+    static constexpr int kBytes = kThere + 4 * 8;
+    // A key row's 16-byte chunk c lies at c ^ key_turn(row), a value row's
+    // (dimension's) at c ^ value_turn(d): the 16 lanes that read at once then
+    // fall on all banks.
+    static __device__ __forceinline__ int key_turn(int row) { return D % 128 == 0 ? row & 15 : row >> 1 & 7; }
+    static __device__ __forceinline__ int value_turn(int d) { return (d >> 1 ^ d >> 4) & 7; }
+};
+
+// A value that the compiler must take to be new here: what is worked out from
+// it stays inside a loop, where it costs an instruction, instead of a register
+// all through it.
+__device__ __forceinline__ int anew(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+__device__ __forceinline__ f16v mma32(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// The units (kManyRows rows by kUnit positions) of a sequence's row tiles:
+// tile j ends by position first + (j / ratio + 1) * kUnit, so it has
+// whole + j / ratio units, whole = ceil(first / kUnit) + 1 (+ 1: a token's
+// heads over more than one tile). tiles_units(j): those of the tiles below j.
+__device__ __forceinline__ uint32_t whole_units(const KernelArgs &a, uint32_t first) {
+    return (min(first, a.held) + kUnit - 1) / kUnit + 1 + (a.ratio > (uint32_t)kManyRows ? 1 : 0);
+}
+
+__device__ __forceinline__ uint32_t tiles_units(const KernelArgs &a, uint32_t whole, uint32_t j) {
+    const uint32_t q = by_ratio(a, j);
+    return j * whole + a.ratio * (q * (q - 1) / 2) + q * (j - q * a.ratio);
+}
+
+template <int D>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const KernelArgs a) {
+    using Lay = ManyLayout<D>;
+    constexpr int G = D / 64;
+    constexpr uint32_t kPieces = D / 16;                   // 16-byte pieces of a head row's codes
+    constexpr int kValueItems = (2 * D + 255) / 256;       // (eight positions, four dimensions) a thread
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = (int)uniform(tid >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const qwh_paged_cache &c = a.p.cache;
+    const uint32_t kvh = blockIdx.x % c.kv_heads, stretch = blockIdx.x / c.kv_heads;
+    WorkLine line;
+    const uint32_t length = line.length(a, lane, kManyRows);
+    const float share = ceilf((float)length * a.inverse_stretches_many * 0.999999f);
+    const uint32_t per = uniform(share > 1.0f ? (uint32_t)share : 1);
+    if ((uint64_t)stretch * per >= length) return;
+    const uint32_t stretch_begin = stretch * per, stretch_end = min(stretch_begin + per, length);
+    const uint32_t kv_width = c.kv_heads * D, gpr = kv_width / 64;
+
+    for (uint32_t at = stretch_begin; at < stretch_end;) {
+        int owner;
+        if (!line.find(a, at, lane, owner, kManyRows)) return;
+        const uint32_t b = line.base + owner, tokens = lane_of(line.n, owner), first = lane_of(line.first, owner);
+        const uint32_t whole = whole_units(a, first), tiles = row_tiles(a, tokens, kManyRows);
+        const uint32_t seq_begin = add_units(line.before, lane_of(line.upto, owner)) - tiles_units(a, whole, tiles);
+        // The tile that unit `at` lies in: the last that begins at or below it.
+        uint32_t tile = 0, step = 1;
+        while (step * 64 < tiles) step *= 64;
+        for (; step >= 1; step /= 64) {
+            const uint32_t j = tile + lane * step;
+            const uint64_t below = __ballot(j < tiles && tiles_units(a, whole, j) <= at - seq_begin);
+            if (!below) return;  // (starts that fall)
+            tile += step * (63 - __builtin_clzll(below));
+            if (step == 1) break;
+        }
+        const uint32_t from = at - seq_begin - tiles_units(a, whole, tile), units = whole + by_ratio(a, tile);
+        if (from >= units) return;  // (starts that fall)
+        const uint32_t count = min(units - from, stretch_end - at);
+        const bool alone = count == units;
+        const uint32_t record = 2 * stretch + (at == stretch_begin ? 0 : 1);
+        if (at == seq_begin && kvh == 0 && tid == 0) a.plan[b] = u4{per, seq_begin, whole, 1};  // for the join
+        at += count;
+        const uint32_t start = a.p.batch.row_starts ? a.p.batch.row_starts[b] : b;
+        const uint32_t f = tile * kManyRows + 32 * wave + col;
+        const uint32_t t = by_ratio(a, f), r = f - t * a.ratio;
+        const bool active = t < tokens;
+        const auto place = [&](uint32_t token) {  // its position, at most the tables' last
+            const uint64_t p = (uint64_t)first + min(token, tokens - 1);
+            return p < a.held ? (uint32_t)p : a.held - 1;
+        };
+        // Positions up to limit for this lane's row, up to `common` for every
+        // row of the wavefront, up to `furthest` for some; `end` of the tile.
+        const uint32_t limit = place(t);
+        const uint32_t wave_first = tile * kManyRows + 32 * wave;
+        const bool busy = by_ratio(a, wave_first) < tokens;
+        const uint32_t common = uniform(place(by_ratio(a, wave_first)));
+        const uint32_t furthest = uniform(place(by_ratio(a, wave_first + 31)));
+        const uint32_t begin = from * kUnit;
+        uint32_t end = uniform(place(by_ratio(a, tile * kManyRows + kManyRows - 1))) + 1;
+        if (begin >= end) continue;  // (no row of the tile sees this part)
+        if (end - begin > count * kUnit) end = begin + count * kUnit;
+
+        const uint32_t *table = a.p.batch.tables + (size_t)b * a.p.batch.table_pages;
+        // Wavefront 0 looks the pool rows up, lane by position.
+        struct Place {
+            uint32_t page, within;
+        };
+        const auto lookup = [&](uint32_t base) {
+            const uint32_t p = min(base + lane, end - 1);
+            const uint32_t page = a.page_shift < 32 ? p >> a.page_shift : p / c.page_size;
+            return Place{table[page], p - page * c.page_size};
+        };
+        const auto put_rows = [&](const Place &p, uint32_t base, uint32_t slot) {
+            const bool has_row = (p.page < c.pages) & (base + lane < end);
+            const uint32_t safe = has_row ? p.page * c.page_size + p.within : 0;
+            const uint64_t there = __ballot(has_row);
+            reinterpret_cast<uint32_t *>(lds + Lay::kRows)[slot * kManyPositions + lane] = safe * (kv_width / 16);
+            reinterpret_cast<uint32_t *>(lds + Lay::kPoolRows)[slot * kManyPositions + lane] = safe;
+            if (lane == 0) reinterpret_cast<uint64_t *>(lds + Lay::kThere)[slot] = there;
+        };
+        // A tile on its way: raw codes and scales.
+        uint4 k_raw[G];
+        uint32_t v_raw[kValueItems][8];
+        uint16_t scale_raw[G];
+        const uint8_t *k_base = c.k_codes + kvh * D, *v_base = c.v_codes + kvh * D;
+        const uint16_t *scale_base = reinterpret_cast<const uint16_t *>(wave == 0 ? c.k_scales : c.v_scales) + kvh * G;
+        const auto load = [&](uint32_t slot) {
+            const int tid = anew(threadIdx.x);
+            const uint32_t *rows = reinterpret_cast<const uint32_t *>(lds + Lay::kRows) + slot * kManyPositions;
+            if (wave < 2) {
+                const size_t pool_row = reinterpret_cast<const uint32_t *>(lds + Lay::kPoolRows)[slot * kManyPositions + lane];
+#pragma unroll
+                for (int g = 0; g < G; ++g) scale_raw[g] = scale_base[pool_row * gpr + g];
+            }
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                const uint32_t piece = tid + 256 * j;
+                k_raw[j] = *reinterpret_cast<const uint4 *>(k_base + ((size_t)rows[piece / kPieces] << 4) + 16 * (piece % kPieces));
+            }
+#pragma unroll
+            for (int j = 0; j < kValueItems; ++j) {
+                const int item = tid + 256 * j, eight = item / (D / 4), quad = item % (D / 4);
+                if (2 * D % 256 != 0 && item >= 2 * D) break;
+                // Positions 16 s + 4 h + 0..3 and 16 s + 8 + 4 h + 0..3 of eight 2 s + h.
+                const u4 r0 = *reinterpret_cast<const u4 *>(rows + 16 * (eight / 2) + 4 * (eight & 1));
+                const u4 r1 = *reinterpret_cast<const u4 *>(rows + 16 * (eight / 2) + 8 + 4 * (eight & 1));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v_raw[j][i] = *reinterpret_cast<const uint32_t *>(v_base + ((size_t)r0[i] << 4) + 4 * quad);
+                    v_raw[j][4 + i] = *reinterpret_cast<const uint32_t *>(v_base + ((size_t)r1[i] << 4) + 4 * quad);
+                }
+            }
+        };
+        const auto convert = [&](uint32_t buffer) {
+            uint8_t *buf = lds + buffer * Lay::kBuffer;
+            const int tid = anew(threadIdx.x);
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                const int piece = tid + 256 * j, row = piece / (int)kPieces, chunk = 2 * (piece % (int)kPieces);
+                uint8_t *dst = buf + Lay::kKeys + row * (2 * D);
+                *reinterpret_cast<h8 *>(dst + 16 * (chunk ^ Lay::key_turn(row))) = codes8(k_raw[j].x, k_raw[j].y);
+                *reinterpret_cast<h8 *>(dst + 16 * ((chunk + 1) ^ Lay::key_turn(row))) = codes8(k_raw[j].z, k_raw[j].w);
+            }
+#pragma unroll
+            for (int j = 0; j < kValueItems; ++j) {
+                const int item = tid + 256 * j, eight = item / (D / 4), quad = item % (D / 4);
+                if (2 * D % 256 != 0 && item >= 2 * D) break;
+                uint8_t *dst = buf + Lay::kValues;
+                *reinterpret_cast<h8 *>(dst + (4 * quad) * 128 + 16 * (eight ^ Lay::value_turn(4 * quad))) = codes_across<0>(v_raw[j]);
+                *reinterpret_cast<h8 *>(dst + (4 * quad + 1) * 128 + 16 * (eight ^ Lay::value_turn(4 * quad + 1))) = codes_across<1>(v_raw[j]);
+                *reinterpret_cast<h8 *>(dst + (4 * quad + 2) * 128 + 16 * (eight ^ Lay::value_turn(4 * quad + 2))) = codes_across<2>(v_raw[j]);
+                *reinterpret_cast<h8 *>(dst + (4 * quad + 3) * 128 + 16 * (eight ^ Lay::value_turn(4 * quad + 3))) = codes_across<3>(v_raw[j]);
+            }
+            float *scales = reinterpret_cast<float *>(buf + Lay::kScales);
+            if (wave == 0) {
+#pragma unroll
+                for (int g = 0; g < G; ++g) scales[g * kManyPositions + lane] = dev::f16_bits_to_f32(scale_raw[g]);
+            } else if (wave == 1) {
+                // (A position of zero scales counts as one of f16's least:
+                // its weight still belongs to the sum.)
+                float vs[G], vm = 0x1p-24f;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    vs[g] = dev::f16_bits_to_f32(scale_raw[g]);
+                    vm = fmaxf(vm, fabsf(vs[g]));
+                }
+                const float inverse = 1.0f / vm;
+                scales[G * kManyPositions + lane] = __builtin_amdgcn_logf(vm);
+                scales[(G + 1) * kManyPositions + lane] = inverse;
+#pragma unroll
+                for (int g = 0; g < G; ++g) scales[(G + 2 + g) * kManyPositions + lane] = vs[g] * inverse * 4096.0f;
+            }
+        };
+
+        // The query rows' two terms, scaled by a power of two to below 2^8.
+        const size_t row = (size_t)start + t;
+        h8 qh[G][4], ql[G][4];
+        float qs;
+        {
+            f4 x[G][4][2];
+            float top = 0.0f;
+            const float *src = a.p.query + (active ? row * a.p.query_stride + (kvh * a.ratio + r) * D + 8 * half : 0);
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const f4 y = active ? *reinterpret_cast<const f4 *>(src + 64 * g + 16 * k + 4 * i) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+                        x[g][k][i] = y;
+                        top = fmaxf(top, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+                    }
+            top = fmaxf(top, dev::xor_lane<32>(top));
+            int e = 0;
+            if (top > 0.0f && top < INFINITY) (void)__builtin_frexpf(top, &e);
+            e = e < -100 ? -100 : e;
+            const float up = __builtin_ldexpf(1.0f, 8 - e);
+            qs = a.scaling * __builtin_ldexpf(kCodeScale, e - 8);
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const f4 y = x[g][k][i] * up;
+                        const float z[4] = {y.x, y.y, y.z, y.w};
+                        u2 hi, lo;
+                        two_terms(z, hi, lo);
+                        const h4 h = __builtin_bit_cast(h4, hi), l = __builtin_bit_cast(h4, lo);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            qh[g][k][4 * i + j] = h[j];
+                            ql[g][k][4 * i + j] = l[j];
+                        }
+                    }
+        }
+
+        float m = -INFINITY, l = 0.0f;
+        f16v acc[G][2];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) acc[g][i] = f16v{};
+
+        const auto use = [&](uint32_t buffer, uint32_t base, uint64_t there) {
+            const uint8_t *buf = lds + buffer * Lay::kBuffer;
+            const int col = anew(lane & 31), half = anew(lane >> 5);
+            const float *scales = reinterpret_cast<const float *>(buf + Lay::kScales);
+            const auto scale4 = [&](int which, int blk, int i) {  // of this lane's four positions 32 blk + 8 i + 4 half
+                return *reinterpret_cast<const f4 *>(scales + which * kManyPositions + 32 * blk + 8 * i + 4 * half);
+            };
+            f16v s[2];
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    f16v x = f16v{};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int chunk = 8 * g + 2 * k + half, at = 32 * blk + col;
+                        const h8 key = *reinterpret_cast<const h8 *>(buf + Lay::kKeys + at * (2 * D) + 16 * (chunk ^ Lay::key_turn(at)));
+                        x = mma32(key, ql[g][k], x);
+                        x = mma32(key, qh[g][k], x);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f4 ks = scale4(g, blk, i);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            s[blk][4 * i + j] = g == 0 ? ks[j] * x[4 * i + j] : fmaf(ks[j], x[4 * i + j], s[blk][4 * i + j]);
+                    }
+                    // (Held back, the next reads would cost registers, and spill.)
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            // (Two forms: a mask's comparisons cost as much as the softmax.)
+            const auto weigh = [&](auto every) __attribute__((always_inline)) {
+                constexpr bool EVERY = decltype(every)::value;
+                float mx = -INFINITY;
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f4 lv = scale4(G, blk, i);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            float x = fmaf(s[blk][4 * i + j], qs, lv[j]);
+                            if constexpr (!EVERY) {
+                                const uint32_t within = 32 * blk + 8 * i + 4 * half + j;
+                                if (!(there >> within & 1u) || base + within > limit) x = -INFINITY;
+                            }
+                            s[blk][4 * i + j] = x;
+                            mx = fmaxf(mx, x);
+                        }
+                    }
+                mx = fmaxf(mx, dev::xor_lane<32>(mx));
+                // The maximum moves when some row's is passed by 2^3, or it has
+                // none yet.
+                if (__ballot(mx > m + 3.0f)) {
+                    const float to = fmaxf(m, mx);
+                    const float less = exp2_fast(m - (to == -INFINITY ? 0.0f : to));
+                    l *= less;
+#pragma unroll
+                    for (int g = 0; g < G; ++g)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) acc[g][i][j] *= less;
+                    m = to;
+                }
+                const float low = m == -INFINITY ? 0.0f : m;
+                // 16 positions at a time: weights, then their products.
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                    for (int i = 0; i < 4; i += 2) {
+                        float p[8];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const f4 rv = scale4(G + 1, blk, i + k);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                p[4 * k + j] = exp2_fast(s[blk][4 * (i + k) + j] - low);
+                                // (As below: 1 / vm of a scale that is no number.)
+                                if constexpr (EVERY) l = fmaf(p[4 * k + j], rv[j], l);
+                                else l = s[blk][4 * (i + k) + j] == -INFINITY ? l : fmaf(p[4 * k + j], rv[j], l);
+                            }
+                        }
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            h8 hi, lo;
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const f4 vs = scale4(G + 2 + g, blk, i + k);
+                                float w[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    w[j] = p[4 * k + j] * vs[j];
+                                    if constexpr (!EVERY) w[j] = s[blk][4 * (i + k) + j] == -INFINITY ? 0.0f : w[j];
+                                }
+                                u2 h2v, l2v;
+                                two_terms(w, h2v, l2v);
+                                const h4 hw = __builtin_bit_cast(h4, h2v), lw = __builtin_bit_cast(h4, l2v);
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    hi[4 * k + j] = hw[j];
+                                    lo[4 * k + j] = lw[j];
+                                }
+                            }
+                            const int chunk = 4 * blk + i + half;  // 16 positions are chunks 2 s and 2 s + 1, s = 2 blk + i / 2
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const int d = 64 * g + 32 * k + col;
+                                const h8 value = *reinterpret_cast<const h8 *>(buf + Lay::kValues + d * 128 + 16 * (chunk ^ Lay::value_turn(d)));
+                                acc[g][k] = mma32(value, lo, acc[g][k]);
+                                acc[g][k] = mma32(value, hi, acc[g][k]);
+                            }
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            };
+            if (there == ~0ull && base + kManyPositions - 1 <= common) weigh(std::true_type{});
+            else weigh(std::false_type{});
+        };
+
+        // (The last part's reads of the buffers are done: its use() is behind
+        // a barrier for all but the last tile, and the rows' slots are not
+        // read in use().)
+        __syncthreads();
+        Place ahead{};
+        if (wave == 0) {
+            const Place p0 = lookup(begin), p1 = lookup(begin + kManyPositions), p2 = lookup(begin + 2 * kManyPositions);
+            ahead = lookup(begin + 3 * kManyPositions);
+            put_rows(p0, begin, 0);
+            put_rows(p1, begin + kManyPositions, 1);
+            put_rows(p2, begin + 2 * kManyPositions, 2);
+        }
+        __syncthreads();
+        load(0);
+        convert(0);
+        load(1);
+        uint32_t i = 0;
+        for (uint32_t base = begin; base < end; base += kManyPositions, ++i) {
+            __syncthreads();
+            if (wave == 0) {
+                put_rows(ahead, base + 3 * kManyPositions, (i + 3) & 3);
+                ahead = lookup(base + 4 * kManyPositions);
+            }
+            convert((i + 1) & 1);
+            load((i + 2) & 3);
+            const uint64_t there = reinterpret_cast<const uint64_t *>(lds + Lay::kThere)[i & 3];
+            if (busy && base <= furthest) use(i & 1, base, there);
+        }
+
+        if (!active) continue;
+        l += dev::xor_lane<32>(l);
+        // Lane: dimensions 64 g + 32 k + 8 i + 4 half + 0..3 of its row.
+        if (!alone) {
+            const size_t rec = ((size_t)record * c.kv_heads + kvh) * kManyRows + 32 * wave + col;
+            if (half == 0) {
+                a.sums_many[2 * rec] = m;
+                a.sums_many[2 * rec + 1] = l;
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<f4 *>(a.values_many + rec * D + 64 * g + 32 * k + 8 * q + 4 * half) =
+                            f4{acc[g][k][4 * q], acc[g][k][4 * q + 1], acc[g][k][4 * q + 2], acc[g][k][4 * q + 3]} * (kCodeScale / 4096.0f);
+            continue;
+        }
+        const float inv = l == 0.0f ? 0.0f : kCodeScale / 4096.0f / l;
+        float *out = a.p.out + (row * a.p.heads + kvh * a.ratio + r) * D + 4 * half;
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<f4 *>(out + 64 * g + 32 * k + 8 * q) =
+                        f4{acc[g][k][4 * q], acc[g][k][4 * q + 1], acc[g][k][4 * q + 2], acc[g][k][4 * q + 3]} * inv;
+    }
+}
+
 // Joins the records of a query row (one wavefront) in the order of its
 // positions. Rows whose tile one workgroup took whole were written by it.
 template <int D>
@@ -570,14 +1038,19 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const KernelArgs a, uin
     const uint32_t seen = seen64 < a.held ? (uint32_t)seen64 : a.held;
     // (Starts that fall can leave a sequence without a plan: whatever stands
     // there, only records are read.)
-    const uint32_t per = max(plan.x, 1u), units = plan.z;
+    const bool many = plan.w == 1;
+    const uint32_t per = max(plan.x, 1u), tile_rows = many ? kManyRows : kTileRows;
     const uint32_t kvh = h / a.ratio, f = t * a.ratio + (h - kvh * a.ratio);
-    const uint32_t tile = f / kTileRows, slot = f - tile * kTileRows;
-    const uint32_t begin = plan.y + tile * units;  // the tile's units
+    const uint32_t tile = f / tile_rows, slot = f - tile * tile_rows;
+    // The tile's units.
+    const uint32_t units = many ? plan.z + by_ratio(a, tile) : plan.z;
+    const uint32_t begin = plan.y + (many ? tiles_units(a, plan.z, tile) : tile * units);
     const uint32_t first = begin / per, last = (begin + units - 1) / per;
     if (first == last) return;
     // Stretches that hold positions this row sees.
-    const uint32_t used = min(min(last, (begin + (seen - 1) / kUnit) / per) - first + 1, a.stretches_most);
+    const uint32_t most = many ? a.stretches_most_many : a.stretches_most;
+    const uint32_t used = min(min(last, (begin + (seen - 1) / kUnit) / per) - first + 1, most);
+    const float *sums = many ? a.sums_many : a.sums, *values = many ? a.values_many : a.values;
     float M = -INFINITY, L = 0.0f, acc[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) acc[g] = 0.0f;
@@ -585,12 +1058,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const KernelArgs a, uin
         float m[4], l[4], v[4][G];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const uint32_t s = min(first + min(s0 + k, used - 1), a.stretches_most - 1);
-            const size_t rec = ((size_t)(2 * s + (s * per < begin ? 1 : 0)) * a.p.cache.kv_heads + kvh) * kTileRows + slot;
-            m[k] = a.sums[2 * rec];
-            l[k] = a.sums[2 * rec + 1];
+            const uint32_t s = min(first + min(s0 + k, used - 1), most - 1);
+            const size_t rec = ((size_t)(2 * s + (s * per < begin ? 1 : 0)) * a.p.cache.kv_heads + kvh) * tile_rows + slot;
+            m[k] = sums[2 * rec];
+            l[k] = sums[2 * rec + 1];
 #pragma unroll
-            for (int g = 0; g < G; ++g) v[k][g] = a.values[rec * D + 64 * g + lane];
+            for (int g = 0; g < G; ++g) v[k][g] = values[rec * D + 64 * g + lane];
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -608,54 +1081,92 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const KernelArgs a, uin
     for (int g = 0; g < G; ++g) a.p.out[((size_t)row * a.p.heads + h) * D + 64 * g + lane] = acc[g] * inv;
 }
 
-// Workgroups that a CU holds at once, by the kernel's registers.
-uint32_t resident_groups(uint32_t head_dim) { return head_dim == 64 ? 3 : 2; }
+// Workgroups that a CU holds at once, by the kernels' registers.
+uint32_t resident_few(uint32_t head_dim) { return head_dim == 64 ? 3 : 2; }
+uint32_t resident_many(uint32_t head_dim) { return head_dim <= 128 ? 2 : 1; }
 
 // Stretches of a key/value head: as many workgroups as the device holds.
-uint32_t wanted_stretches(int cus, const PagedAttentionArgs &a) {
-    const uint32_t groups = resident_groups(a.cache.head_dim) * (uint32_t)(cus > 0 ? cus : 256);
+uint32_t wanted_stretches(int cus, const PagedAttentionArgs &a, uint32_t resident) {
+    const uint32_t groups = resident * (uint32_t)(cus > 0 ? cus : 256);
     return groups > a.cache.kv_heads ? groups / a.cache.kv_heads : 1;
 }
 
 // Stretches at most: the division's rounding, and a whole round of the dies.
-uint32_t most_stretches(int cus, const PagedAttentionArgs &a) { return (wanted_stretches(cus, a) + 2 + kDies - 1) / kDies * kDies; }
+uint32_t most_stretches(int cus, const PagedAttentionArgs &a, uint32_t resident) {
+    return (wanted_stretches(cus, a, resident) + 2 + kDies - 1) / kDies * kDies;
+}
 
-// Two records (of kTileRows rows) a stretch and head.
-uint64_t record_rows(int cus, const PagedAttentionArgs &a) { return 2ull * most_stretches(cus, a) * a.cache.kv_heads * kTileRows; }
+// Which kernels a call needs: by the most query rows that a sequence may have
+// (one sequence: as if it had all rows of the buffer).
+struct Forms {
+    bool few, many;
+};
+
+Forms forms_of(const PagedAttentionArgs &a) {
+    const uint64_t ratio = a.heads / a.cache.kv_heads;
+    if (!a.batch.row_starts) return Forms{ratio <= kFewRows, ratio > kFewRows};
+    if (a.batch.rows * ratio <= kFewRows) return Forms{true, false};
+    return Forms{a.batch.batch > 1, true};
+}
+
+// Two records a stretch and head, each of a tile's rows.
+uint64_t record_rows_few(int cus, const PagedAttentionArgs &a) {
+    return forms_of(a).few ? 2ull * most_stretches(cus, a, resident_few(a.cache.head_dim)) * a.cache.kv_heads * kTileRows : 0;
+}
+uint64_t record_rows_many(int cus, const PagedAttentionArgs &a) {
+    return forms_of(a).many ? 2ull * most_stretches(cus, a, resident_many(a.cache.head_dim)) * a.cache.kv_heads * kManyRows : 0;
+}
 
 template <int D>
 hipError_t launch_attention(hipStream_t s, int cus, const KernelArgs &k) {
     const qwh_paged_batch &b = k.p.batch;
+    const Forms forms = forms_of(k.p);
     const uint32_t rows = b.row_starts ? b.rows : b.batch;
     const uint64_t join = ((uint64_t)rows * k.p.heads + 3) / 4;
-    const uint64_t blocks = (uint64_t)most_stretches(cus, k.p) * k.p.cache.kv_heads;
-    if (blocks > 0xffffffu || join > 0xffffffu) return hipErrorInvalidValue;
-    paged_few_kernel<D><<<(uint32_t)blocks, 256, 0, s>>>(k);
-    // (Tiles of one unit: nothing to join.)
-    if (k.held > kUnit) paged_join_kernel<D><<<(uint32_t)join, 256, 0, s>>>(k, rows);
+    const uint64_t few = (uint64_t)k.stretches_most * k.p.cache.kv_heads, many = (uint64_t)k.stretches_most_many * k.p.cache.kv_heads;
+    if (few > 0xffffffu || many > 0xffffffu || join > 0xffffffu) return hipErrorInvalidValue;
+    if (forms.many) {
+        constexpr int bytes = ManyLayout<D>::kBytes;
+        static_assert(bytes <= 160 * 1024, "a CU's LDS");
+        const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void *>(paged_many_kernel<D>),
+                                                   hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (err != hipSuccess) return err;
+        paged_many_kernel<D><<<(uint32_t)many, 256, bytes, s>>>(k);
+    }
+    if (forms.few) paged_few_kernel<D><<<(uint32_t)few, 256, 0, s>>>(k);
+    // (Few rows over tables of one unit: nothing to join.)
+    if (forms.many || k.held > kUnit) paged_join_kernel<D><<<(uint32_t)join, 256, 0, s>>>(k, rows);
     return hipGetLastError();
 }
 
 }  // namespace
 
 size_t paged_attention_scratch_bytes(int cus, const PagedAttentionArgs &a) {
-    return a.batch.batch * sizeof(u4) + record_rows(cus, a) * (a.cache.head_dim + 2) * sizeof(float);
+    return a.batch.batch * sizeof(u4) +
+           (record_rows_few(cus, a) + record_rows_many(cus, a)) * (a.cache.head_dim + 2) * sizeof(float);
 }
 
 hipError_t launch_paged_attention(hipStream_t s, int cus, const PagedAttentionArgs &a, void *scratch, size_t scratch_bytes) {
     if (paged_attention_scratch_bytes(cus, a) > scratch_bytes) return hipErrorInvalidValue;
     KernelArgs k{};
+    const uint32_t D = a.cache.head_dim;
     k.p = a;
     k.held = a.batch.table_pages * a.cache.page_size;  // (check_positions)
     k.ratio = a.heads / a.cache.kv_heads;
     k.ratio_magic = k.ratio == 1 ? 0 : (uint32_t)((1ull << 32) / k.ratio) + 1;
     k.page_shift = (a.cache.page_size & (a.cache.page_size - 1)) ? 32 : (uint32_t)__builtin_ctz(a.cache.page_size);
-    k.stretches_most = most_stretches(cus, a);
-    k.inverse_stretches = 1.0f / (float)wanted_stretches(cus, a);
-    k.scaling = kLog2e / sqrtf((float)a.cache.head_dim);
+    const Forms forms = forms_of(a);
+    k.few_rows = !forms.many ? 0xffffffffu : !forms.few ? 0 : kFewRows;
+    k.stretches_most = most_stretches(cus, a, resident_few(D));
+    k.inverse_stretches = 1.0f / (float)wanted_stretches(cus, a, resident_few(D));
+    k.stretches_most_many = most_stretches(cus, a, resident_many(D));
+    k.inverse_stretches_many = 1.0f / (float)wanted_stretches(cus, a, resident_many(D));
+    k.scaling = kLog2e / sqrtf((float)D);
     k.plan = static_cast<u4 *>(scratch);
     k.values = reinterpret_cast<float *>(k.plan + a.batch.batch);
-    k.sums = k.values + record_rows(cus, a) * a.cache.head_dim;
+    k.sums = k.values + record_rows_few(cus, a) * D;
+    k.values_many = k.sums + record_rows_few(cus, a) * 2;
+    k.sums_many = k.values_many + record_rows_many(cus, a) * D;
     switch (a.cache.head_dim) {
     case 64: return launch_attention<64>(s, cus, k);
     case 128: return launch_attention<128>(s, cus, k);

@@ -17,7 +17,7 @@ constexpr uint32_t kMaxBatch = 65535;
 constexpr uint32_t kMaxRows = 1u << 20;
 constexpr uint32_t kMaxHeads = 4096;
 constexpr uint64_t kMaxRowHeads = 1u << 23;
-constexpr uint32_t kMaxRatio = 512;
+constexpr uint32_t kMaxRatio = 256;
 
 // A refusal: a status and why, or QWH_OK.
 struct Refusal {
@@ -84,7 +84,7 @@ inline Refusal check_heads(const qwh_paged_cache &c, uint32_t heads) {
     if (heads == 0 || heads % c.kv_heads != 0)
         return refuse(QWH_E_SHAPE_MISMATCH, "heads is not a multiple of kv_heads");
     if (heads > kMaxHeads) return refuse(QWH_E_LIMIT_EXCEEDED, "more than 4096 heads");
-    if (heads / c.kv_heads > kMaxRatio) return refuse(QWH_E_LIMIT_EXCEEDED, "more than 512 heads per kv head");
+    if (heads / c.kv_heads > kMaxRatio) return refuse(QWH_E_LIMIT_EXCEEDED, "more than 256 heads per kv head");
     return {};
 }
 
@@ -95,10 +95,12 @@ inline Refusal check_row_heads(const qwh_paged_batch &b, uint32_t heads) {
 }
 
 // The attention counts units of 8 query rows (of a kv head) by 128 positions
-// in 31 bits: rows in whole tiles, and one tile more a sequence.
+// in 31 bits: rows in whole tiles, and one tile more a sequence; positions up
+// to the tables' last, rounded up, and a token's own tile.
 inline Refusal check_units(const qwh_paged_cache &c, const qwh_paged_batch &b, uint32_t heads) {
     const uint64_t tiles = (uint64_t)b.rows * (heads / c.kv_heads) / 8 + (b.batch < b.rows ? b.batch : b.rows);
-    if (tiles * (((uint64_t)b.table_pages * c.page_size + 127) / 128) >= 0x7fffffffull)
+    const uint64_t units = ((uint64_t)b.table_pages * c.page_size + 127) / 128 + b.rows / 128 + 3;
+    if (tiles * units >= 0x7fffffffull)
         return refuse(QWH_E_LIMIT_EXCEEDED, "rows times heads per kv head times positions past 2^41");
     return {};
 }
