@@ -18,7 +18,6 @@
 // ends inside a tile's positions leaves a record (maximum, sum, weighted
 // values) per query row, and a second launch joins the records in order.
 #include <cmath>
-#include <type_traits>
 
 #include "common.h"
 #include "paged.h"
@@ -600,7 +599,8 @@ struct ManyLayout {
     static constexpr int kKeys = 0;                                  // [64][D] f16
     static constexpr int kValues = kManyPositions * D * 2;           // [D][64] f16
     static constexpr int kScales = kValues + D * kManyPositions * 2;  // [2 G + 2][64] f32: key scales, log2(vm), 1 / vm, 2^12 vs / vm
-    static constexpr int kBuffer = kScales + (2 * G + 2) * kManyPositions * 4;
+    static constexpr int kBad = kScales + (2 * G + 2) * kManyPositions * 4;  // whether some value scale is no number
+    static constexpr int kBuffer = kBad + 16;
     static constexpr int kRows = 2 * kBuffer;                        // [4][64] pool rows in 16-byte pieces
     static constexpr int kPoolRows = kRows + 4 * kManyPositions * 4;  // [4][64] pool rows
     static constexpr int kThere = kPoolRows + 4 * kManyPositions * 4;  // [4] u64
@@ -757,6 +757,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
                 uint8_t *dst = buf + Lay::kKeys + row * (2 * D);
                 *reinterpret_cast<h8 *>(dst + 16 * (chunk ^ Lay::key_turn(row))) = codes8(k_raw[j].x, k_raw[j].y);
                 *reinterpret_cast<h8 *>(dst + 16 * ((chunk + 1) ^ Lay::key_turn(row))) = codes8(k_raw[j].z, k_raw[j].w);
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int j = 0; j < kValueItems; ++j) {
@@ -767,6 +768,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
                 *reinterpret_cast<h8 *>(dst + (4 * quad + 1) * 128 + 16 * (eight ^ Lay::value_turn(4 * quad + 1))) = codes_across<1>(v_raw[j]);
                 *reinterpret_cast<h8 *>(dst + (4 * quad + 2) * 128 + 16 * (eight ^ Lay::value_turn(4 * quad + 2))) = codes_across<2>(v_raw[j]);
                 *reinterpret_cast<h8 *>(dst + (4 * quad + 3) * 128 + 16 * (eight ^ Lay::value_turn(4 * quad + 3))) = codes_across<3>(v_raw[j]);
+                __builtin_amdgcn_sched_barrier(0);
             }
             float *scales = reinterpret_cast<float *>(buf + Lay::kScales);
             if (wave == 0) {
@@ -781,6 +783,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
                     vs[g] = dev::f16_bits_to_f32(scale_raw[g]);
                     vm = fmaxf(vm, fabsf(vs[g]));
                 }
+                bool bad = false;
+#pragma unroll
+                for (int g = 0; g < G; ++g) bad |= !(fabsf(vs[g]) < INFINITY);
+                const uint64_t some = __ballot(bad);
+                if (lane == 0) *reinterpret_cast<uint32_t *>(buf + Lay::kBad) = some != 0;
                 const float inverse = 1.0f / vm;
                 scales[G * kManyPositions + lane] = __builtin_amdgcn_logf(vm);
                 scales[(G + 1) * kManyPositions + lane] = inverse;
@@ -839,124 +846,115 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
 #pragma unroll
             for (int i = 0; i < 2; ++i) acc[g][i] = f16v{};
 
-        const auto use = [&](uint32_t buffer, uint32_t base, uint64_t there) {
+        // A block of 32 positions: base + 32 blk on.
+        const auto use = [&](uint32_t buffer, int blk, uint32_t base, uint32_t there) {
             const uint8_t *buf = lds + buffer * Lay::kBuffer;
             const int col = anew(lane & 31), half = anew(lane >> 5);
-            const float *scales = reinterpret_cast<const float *>(buf + Lay::kScales);
-            const auto scale4 = [&](int which, int blk, int i) {  // of this lane's four positions 32 blk + 8 i + 4 half
-                return *reinterpret_cast<const f4 *>(scales + which * kManyPositions + 32 * blk + 8 * i + 4 * half);
+            const float *scales = reinterpret_cast<const float *>(buf + Lay::kScales) + 32 * blk + 4 * half;
+            const auto scale4 = [&](int which, int i) {  // of this lane's four positions 8 i + 4 half
+                return *reinterpret_cast<const f4 *>(scales + which * kManyPositions + 8 * i);
             };
-            f16v s[2];
+            float s[16];
 #pragma unroll
-            for (int blk = 0; blk < 2; ++blk)
+            for (int g = 0; g < G; ++g) {
+                f16v x = f16v{};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int chunk = 8 * g + 2 * k + half, at = 32 * blk + col;
+                    const h8 key = *reinterpret_cast<const h8 *>(buf + Lay::kKeys + at * (2 * D) + 16 * (chunk ^ Lay::key_turn(at)));
+                    x = mma32(key, ql[g][k], x);
+                    x = mma32(key, qh[g][k], x);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f4 ks = scale4(g, i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[4 * i + j] = g == 0 ? ks[j] * x[4 * i + j] : fmaf(ks[j], x[4 * i + j], s[4 * i + j]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f4 lv = scale4(G, i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[4 * i + j] = fmaf(s[4 * i + j], qs, lv[j]);
+            }
+            // (Branches around scores and weights only: one around the sums
+            // would hold them twice, and spill.)
+            if (there != ~0u || base + 31 > common) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t within = 8 * i + 4 * half + j;
+                        if (!(there >> within & 1u) || base + within > limit) s[4 * i + j] = -INFINITY;
+                    }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
+            mx = fmaxf(mx, dev::xor_lane<32>(mx));
+            // The maximum moves when some row's is passed by 2^3, or it has
+            // none yet.
+            if (__ballot(mx > m + 3.0f)) {
+                const float to = fmaxf(m, mx);
+                const float less = exp2_fast(m - (to == -INFINITY ? 0.0f : to));
+                l *= less;
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) acc[g][i][j] *= less;
+                m = to;
+            }
+            const float low = m == -INFINITY ? 0.0f : m;
+            const bool numbers = uniform(*reinterpret_cast<const uint32_t *>(buf + Lay::kBad)) == 0;
+            // 16 positions at a time: weights, then their products.
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                float p[8];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const f4 rv = scale4(G + 1, i + k);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        p[4 * k + j] = exp2_fast(s[4 * (i + k) + j] - low);
+                        l = fmaf(p[4 * k + j], rv[j], l);
+                    }
+                }
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    f16v x = f16v{};
+                    float w[8];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int chunk = 8 * g + 2 * k + half, at = 32 * blk + col;
-                        const h8 key = *reinterpret_cast<const h8 *>(buf + Lay::kKeys + at * (2 * D) + 16 * (chunk ^ Lay::key_turn(at)));
-                        x = mma32(key, ql[g][k], x);
-                        x = mma32(key, qh[g][k], x);
+                    for (int k = 0; k < 2; ++k) {
+                        const f4 vs = scale4(G + 2 + g, i + k);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) w[4 * k + j] = p[4 * k + j] * vs[j];
                     }
+                    // (A scale that is no number must not reach rows that do not see it.)
+                    if (!numbers) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f4 ks = scale4(g, blk, i);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            s[blk][4 * i + j] = g == 0 ? ks[j] * x[4 * i + j] : fmaf(ks[j], x[4 * i + j], s[blk][4 * i + j]);
+                        for (int j = 0; j < 8; ++j) w[j] = s[4 * i + j] == -INFINITY ? 0.0f : w[j];
                     }
-                    // (Held back, the next reads would cost registers, and spill.)
+                    h8 hi, lo;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) hi[j] = (_Float16)w[j];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) lo[j] = (_Float16)(w[j] - (float)hi[j]);
+                    const int chunk = 4 * blk + i + half;  // 16 positions are chunks 2 s and 2 s + 1, s = 2 blk + i / 2
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int d = 64 * g + 32 * k + col;
+                        const h8 value = *reinterpret_cast<const h8 *>(buf + Lay::kValues + d * 128 + 16 * (chunk ^ Lay::value_turn(d)));
+                        acc[g][k] = mma32(value, lo, acc[g][k]);
+                        acc[g][k] = mma32(value, hi, acc[g][k]);
+                    }
+                    // (Reads moved up from the next round would cost
+                    // registers, and spill.)
                     __builtin_amdgcn_sched_barrier(0);
                 }
-            // (Two forms: a mask's comparisons cost as much as the softmax.)
-            const auto weigh = [&](auto every) __attribute__((always_inline)) {
-                constexpr bool EVERY = decltype(every)::value;
-                float mx = -INFINITY;
-#pragma unroll
-                for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f4 lv = scale4(G, blk, i);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            float x = fmaf(s[blk][4 * i + j], qs, lv[j]);
-                            if constexpr (!EVERY) {
-                                const uint32_t within = 32 * blk + 8 * i + 4 * half + j;
-                                if (!(there >> within & 1u) || base + within > limit) x = -INFINITY;
-                            }
-                            s[blk][4 * i + j] = x;
-                            mx = fmaxf(mx, x);
-                        }
-                    }
-                mx = fmaxf(mx, dev::xor_lane<32>(mx));
-                // The maximum moves when some row's is passed by 2^3, or it has
-                // none yet.
-                if (__ballot(mx > m + 3.0f)) {
-                    const float to = fmaxf(m, mx);
-                    const float less = exp2_fast(m - (to == -INFINITY ? 0.0f : to));
-                    l *= less;
-#pragma unroll
-                    for (int g = 0; g < G; ++g)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) acc[g][i][j] *= less;
-                    m = to;
-                }
-                const float low = m == -INFINITY ? 0.0f : m;
-                // 16 positions at a time: weights, then their products.
-#pragma unroll
-                for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-                    for (int i = 0; i < 4; i += 2) {
-                        float p[8];
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const f4 rv = scale4(G + 1, blk, i + k);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                p[4 * k + j] = exp2_fast(s[blk][4 * (i + k) + j] - low);
-                                // (As below: 1 / vm of a scale that is no number.)
-                                if constexpr (EVERY) l = fmaf(p[4 * k + j], rv[j], l);
-                                else l = s[blk][4 * (i + k) + j] == -INFINITY ? l : fmaf(p[4 * k + j], rv[j], l);
-                            }
-                        }
-#pragma unroll
-                        for (int g = 0; g < G; ++g) {
-                            h8 hi, lo;
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                const f4 vs = scale4(G + 2 + g, blk, i + k);
-                                float w[4];
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    w[j] = p[4 * k + j] * vs[j];
-                                    if constexpr (!EVERY) w[j] = s[blk][4 * (i + k) + j] == -INFINITY ? 0.0f : w[j];
-                                }
-                                u2 h2v, l2v;
-                                two_terms(w, h2v, l2v);
-                                const h4 hw = __builtin_bit_cast(h4, h2v), lw = __builtin_bit_cast(h4, l2v);
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    hi[4 * k + j] = hw[j];
-                                    lo[4 * k + j] = lw[j];
-                                }
-                            }
-                            const int chunk = 4 * blk + i + half;  // 16 positions are chunks 2 s and 2 s + 1, s = 2 blk + i / 2
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                const int d = 64 * g + 32 * k + col;
-                                const h8 value = *reinterpret_cast<const h8 *>(buf + Lay::kValues + d * 128 + 16 * (chunk ^ Lay::value_turn(d)));
-                                acc[g][k] = mma32(value, lo, acc[g][k]);
-                                acc[g][k] = mma32(value, hi, acc[g][k]);
-                            }
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-            };
-            if (there == ~0ull && base + kManyPositions - 1 <= common) weigh(std::true_type{});
-            else weigh(std::false_type{});
+            }
         };
 
         // (The last part's reads of the buffers are done: its use() is behind
@@ -983,9 +981,13 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
                 ahead = lookup(base + 4 * kManyPositions);
             }
             convert((i + 1) & 1);
+            __builtin_amdgcn_sched_barrier(0);
             load((i + 2) & 3);
+            __builtin_amdgcn_sched_barrier(0);
             const uint64_t there = reinterpret_cast<const uint64_t *>(lds + Lay::kThere)[i & 3];
-            if (busy && base <= furthest) use(i & 1, base, there);
+#pragma unroll 1
+            for (int blk = 0; blk < 2; ++blk)
+                if (busy && base + 32 * blk <= furthest) use(i & 1, blk, base + 32 * blk, (uint32_t)(there >> 32 * blk));
         }
 
         if (!active) continue;
