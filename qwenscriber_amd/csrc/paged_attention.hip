@@ -184,13 +184,16 @@ __device__ __forceinline__ h8 codes_across(const uint32_t (&w)[8]) {
     return h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
+// What a half leaves of x, as a half: one mixed multiply-add each.
+__device__ __forceinline__ _Float16 rest(float x, _Float16 hi) { return (_Float16)__builtin_fmaf((float)hi, -1.0f, x); }
+
 // x as hi + lo, both f16 (rounded to nearest, together 2^-22 of x).
 __device__ __forceinline__ void two_terms(const float (&x)[4], u2 &hi, u2 &lo) {
     h4 h, l;
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = (_Float16)x[i];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) l[i] = (_Float16)(x[i] - (float)h[i]);
+    for (int i = 0; i < 4; ++i) l[i] = rest(x[i], h[i]);
     hi = __builtin_bit_cast(u2, h);
     lo = __builtin_bit_cast(u2, l);
 }
@@ -583,8 +586,8 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
 // Value scales: with vm the largest of a position's, the softmax runs over
 // score + log2(vm), so its weights P = p vm are at most 1 (2^3: the maximum
 // they are taken against moves only when it is passed by more) and so are
-// P vs / vm; the sum is of P / vm. Both terms of 2^12 P vs / vm then keep
-// 2^-22 of the row's largest.
+// P vs / vm = p vs. Both terms of 2^12 p vs then keep 2^-22 of the row's
+// largest; the sum is of 2^12 p = 2^12 P / vm.
 // Two LDS buffers and a barrier a tile: tile i + 1 is converted and tile i + 2
 // asked for at the start of tile i. Issue bound: of about 2600 cycles a
 // wavefront and tile (head_dim 128) the matrix cores work 2048.
@@ -598,9 +601,10 @@ struct ManyLayout {
     static constexpr int G = D / 64;
     static constexpr int kKeys = 0;                                  // [64][D] f16
     static constexpr int kValues = kManyPositions * D * 2;           // [D][64] f16
-    static constexpr int kScales = kValues + D * kManyPositions * 2;  // [2 G + 2][64] f32: key scales, log2(vm), 1 / vm, 2^12 vs / vm
-    static constexpr int kBad = kScales + (2 * G + 2) * kManyPositions * 4;  // whether some value scale is no number
-    static constexpr int kBuffer = kBad + 16;
+    static constexpr int kScales = kValues + D * kManyPositions * 2;  // [2][64 / 4][G][4] f16: key scales, value scales
+    static constexpr int kWeights = kScales + 2 * G * kManyPositions * 2;  // [2][64] f32: log2(vm), 2^12 / vm
+    static constexpr int kBad = kWeights + 2 * kManyPositions * 4;   // whether some value scale is no number
+    static constexpr int kBuffer = (kBad + 4 + 511) / 512 * 512;  // (row addresses are put together bit by bit)
     static constexpr int kRows = 2 * kBuffer;                        // [4][64] pool rows in 16-byte pieces
     static constexpr int kPoolRows = kRows + 4 * kManyPositions * 4;  // [4][64] pool rows
     static constexpr int kThere = kPoolRows + 4 * kManyPositions * 4;  // [4] u64
@@ -770,36 +774,39 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
                 *reinterpret_cast<h8 *>(dst + (4 * quad + 3) * 128 + 16 * (eight ^ Lay::value_turn(4 * quad + 3))) = codes_across<3>(v_raw[j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            float *scales = reinterpret_cast<float *>(buf + Lay::kScales);
-            if (wave == 0) {
+            if (wave < 2) {
+                uint16_t *scales = reinterpret_cast<uint16_t *>(buf + Lay::kScales) + wave * G * kManyPositions + lane / 4 * (4 * G) + lane % 4;
 #pragma unroll
-                for (int g = 0; g < G; ++g) scales[g * kManyPositions + lane] = dev::f16_bits_to_f32(scale_raw[g]);
-            } else if (wave == 1) {
+                for (int g = 0; g < G; ++g) scales[4 * g] = scale_raw[g];
+            }
+            if (wave == 1) {
                 // (A position of zero scales counts as one of f16's least:
                 // its weight still belongs to the sum.)
-                float vs[G], vm = 0x1p-24f;
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    vs[g] = dev::f16_bits_to_f32(scale_raw[g]);
-                    vm = fmaxf(vm, fabsf(vs[g]));
-                }
+                float vm = 0x1p-24f;
                 bool bad = false;
 #pragma unroll
-                for (int g = 0; g < G; ++g) bad |= !(fabsf(vs[g]) < INFINITY);
+                for (int g = 0; g < G; ++g) {
+                    const float vs = fabsf(dev::f16_bits_to_f32(scale_raw[g]));
+                    vm = fmaxf(vm, vs);
+                    bad |= !(vs < INFINITY);
+                }
                 const uint64_t some = __ballot(bad);
                 if (lane == 0) *reinterpret_cast<uint32_t *>(buf + Lay::kBad) = some != 0;
-                const float inverse = 1.0f / vm;
-                scales[G * kManyPositions + lane] = __builtin_amdgcn_logf(vm);
-                scales[(G + 1) * kManyPositions + lane] = inverse;
-#pragma unroll
-                for (int g = 0; g < G; ++g) scales[(G + 2 + g) * kManyPositions + lane] = vs[g] * inverse * 4096.0f;
+                float *weights = reinterpret_cast<float *>(buf + Lay::kWeights);
+                weights[lane] = __builtin_amdgcn_logf(vm);
+                weights[kManyPositions + lane] = 4096.0f / vm;
             }
         };
 
-        // The query rows' two terms, scaled by a power of two to below 2^8.
+        // The query rows' two terms, times log2(e) / sqrt(D) and what brings
+        // products with the codes back. As they are where a wavefront's rows
+        // allow it (the largest value of each 2^-3 to 2^15, or zeros);
+        // otherwise scaled by a power of two a row to below 2^8, and the
+        // products by `fix` afterwards.
         const size_t row = (size_t)start + t;
         h8 qh[G][4], ql[G][4];
-        float qs;
+        float fix = 1.0f;
+        bool plain;
         {
             f4 x[G][4][2];
             float top = 0.0f;
@@ -815,11 +822,15 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
                         top = fmaxf(top, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
                     }
             top = fmaxf(top, dev::xor_lane<32>(top));
-            int e = 0;
-            if (top > 0.0f && top < INFINITY) (void)__builtin_frexpf(top, &e);
-            e = e < -100 ? -100 : e;
-            const float up = __builtin_ldexpf(1.0f, 8 - e);
-            qs = a.scaling * __builtin_ldexpf(kCodeScale, e - 8);
+            float up = a.scaling * kCodeScale;
+            plain = __ballot(!(top == 0.0f || (top * up >= 0x1p-3f && top * up < 0x1p15f))) == 0;
+            if (!plain) {
+                int e = 0;
+                if (top > 0.0f && top < INFINITY) (void)__builtin_frexpf(top, &e);
+                e = e < -100 ? -100 : e;
+                up = a.scaling * __builtin_ldexpf(1.0f, 8 - e);
+                fix = __builtin_ldexpf(kCodeScale, e - 8);
+            }
 #pragma unroll
             for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -850,34 +861,44 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
         const auto use = [&](uint32_t buffer, int blk, uint32_t base, uint32_t there) {
             const uint8_t *buf = lds + buffer * Lay::kBuffer;
             const int col = anew(lane & 31), half = anew(lane >> 5);
-            const float *scales = reinterpret_cast<const float *>(buf + Lay::kScales) + 32 * blk + 4 * half;
-            const auto scale4 = [&](int which, int i) {  // of this lane's four positions 8 i + 4 half
-                return *reinterpret_cast<const f4 *>(scales + which * kManyPositions + 8 * i);
+            // This lane's four positions 8 i + 4 half of the block: key or
+            // value scales, and log2(vm) or 2^12 / vm.
+            const uint8_t *scales = buf + Lay::kScales + (8 * blk + half) * (8 * G);
+            const auto scale4 = [&](int which, int g, int i) {
+                return *reinterpret_cast<const h4 *>(scales + which * (2 * G * kManyPositions) + i * (16 * G) + 8 * g);
             };
+            const uint8_t *weights = buf + Lay::kWeights + (32 * blk + 4 * half) * 4;
+            const auto weight4 = [&](int which, int i) { return *reinterpret_cast<const f4 *>(weights + which * (4 * kManyPositions) + 32 * i); };
+            // A chunk's place differs from the lane's first one in the bits
+            // of the chunk's number: one exclusive or, no sum. (Chunk 8 g + 2 k
+            // + half of key row 32 blk + col; chunk 4 blk + i + half of value
+            // row 64 g + 32 k + col, whose turn is the column's and 4 g + 2 k.)
+            const int key_at = (32 * blk + col) * (2 * D) + 16 * (half ^ Lay::key_turn(col));
+            const int value_at = col * 128 + 16 * ((half ^ Lay::value_turn(col) ^ 4 * blk) & 7);
             float s[16];
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 f16v x = f16v{};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int chunk = 8 * g + 2 * k + half, at = 32 * blk + col;
-                    const h8 key = *reinterpret_cast<const h8 *>(buf + Lay::kKeys + at * (2 * D) + 16 * (chunk ^ Lay::key_turn(at)));
+                    const int chunk = D % 128 == 0 ? key_at ^ 16 * (8 * g + 2 * k) : (key_at ^ 16 * (2 * k)) + 128 * g;
+                    const h8 key = *reinterpret_cast<const h8 *>(buf + Lay::kKeys + chunk);
                     x = mma32(key, ql[g][k], x);
                     x = mma32(key, qh[g][k], x);
                 }
+                if (!plain) {
+                    asm volatile("");  // (a branch: seldom taken)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] *= fix;
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const f4 ks = scale4(g, i);
+                    const h4 ks = scale4(0, g, i);
+                    const f4 lv = g == 0 ? weight4(0, i) : f4{};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) s[4 * i + j] = g == 0 ? ks[j] * x[4 * i + j] : fmaf(ks[j], x[4 * i + j], s[4 * i + j]);
+                    for (int j = 0; j < 4; ++j) s[4 * i + j] = fmaf((float)ks[j], x[4 * i + j], g == 0 ? lv[j] : s[4 * i + j]);
                 }
                 __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f4 lv = scale4(G, i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[4 * i + j] = fmaf(s[4 * i + j], qs, lv[j]);
             }
             // (Branches around scores and weights only: one around the sums
             // would hold them twice, and spill.)
@@ -916,37 +937,33 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
                 float p[8];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const f4 rv = scale4(G + 1, i + k);
+                    const f4 rv = weight4(1, i + k);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        p[4 * k + j] = exp2_fast(s[4 * (i + k) + j] - low);
-                        l = fmaf(p[4 * k + j], rv[j], l);
+                        p[4 * k + j] = exp2_fast(s[4 * (i + k) + j] - low) * rv[j];
+                        l += p[4 * k + j];
                     }
                 }
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    float w[8];
+                    float q[8];
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const f4 vs = scale4(G + 2 + g, i + k);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) w[4 * k + j] = p[4 * k + j] * vs[j];
-                    }
-                    // (A scale that is no number must not reach rows that do not see it.)
+                    for (int j = 0; j < 8; ++j) q[j] = p[j];
+                    h4 vs[2] = {scale4(1, g, i), scale4(1, g, i + 1)};
                     if (!numbers) {
+                        asm volatile("");
+                        // (A scale that is no number must not reach rows that do not see it.)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) w[j] = s[4 * i + j] == -INFINITY ? 0.0f : w[j];
+                        for (int j = 0; j < 8; ++j) vs[j / 4][j & 3] = s[4 * i + j] == -INFINITY ? (_Float16)0.0f : vs[j / 4][j & 3];
                     }
                     h8 hi, lo;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) hi[j] = (_Float16)w[j];
+                    for (int j = 0; j < 8; ++j) hi[j] = (_Float16)(q[j] * (float)vs[j / 4][j & 3]);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) lo[j] = (_Float16)(w[j] - (float)hi[j]);
-                    const int chunk = 4 * blk + i + half;  // 16 positions are chunks 2 s and 2 s + 1, s = 2 blk + i / 2
+                    for (int j = 0; j < 8; ++j) lo[j] = (_Float16)__builtin_fmaf(q[j], (float)vs[j / 4][j & 3], -(float)hi[j]);
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        const int d = 64 * g + 32 * k + col;
-                        const h8 value = *reinterpret_cast<const h8 *>(buf + Lay::kValues + d * 128 + 16 * (chunk ^ Lay::value_turn(d)));
+                        const h8 value = *reinterpret_cast<const h8 *>(buf + Lay::kValues + (64 * g + 32 * k) * 128 + (value_at ^ 16 * ((i ^ (4 * g + 2 * k)) & 7)));
                         acc[g][k] = mma32(value, lo, acc[g][k]);
                         acc[g][k] = mma32(value, hi, acc[g][k]);
                     }
@@ -1006,10 +1023,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
                         *reinterpret_cast<f4 *>(a.values_many + rec * D + 64 * g + 32 * k + 8 * q + 4 * half) =
-                            f4{acc[g][k][4 * q], acc[g][k][4 * q + 1], acc[g][k][4 * q + 2], acc[g][k][4 * q + 3]} * (kCodeScale / 4096.0f);
+                            f4{acc[g][k][4 * q], acc[g][k][4 * q + 1], acc[g][k][4 * q + 2], acc[g][k][4 * q + 3]} * kCodeScale;
             continue;
         }
-        const float inv = l == 0.0f ? 0.0f : kCodeScale / 4096.0f / l;
+        const float inv = l == 0.0f ? 0.0f : kCodeScale / l;
         float *out = a.p.out + (row * a.p.heads + kvh * a.ratio + r) * D + 4 * half;
 #pragma unroll
         for (int g = 0; g < G; ++g)
