@@ -5,18 +5,23 @@
 // logit first and the lower index first among equal ones: the sum of the
 // first k weights (top-k), where the running sum reaches top_p times that
 // (top-p), how many weights are at least min_p of the largest, and where the
-// running sum passes u times what is left. The row is never sorted: a
-// histogram over 2047 steps of the logit below the largest (count and sum of
-// weights a step) says in which step such a place lies, and only that step's
-// tokens are put in order.
+// running sum passes u times what is left. The row is never sorted. A first
+// launch goes over the logits once, 4096 of them a workgroup, and leaves for
+// each such part a histogram over steps of a quarter octave of the weight
+// (count and sum of weights) and its tokens of the best steps, up to 256 of
+// them. A second launch, a workgroup a row, adds the histograms and then needs
+// only the tokens of the steps in which a place lies: mostly those kept
+// beside the histograms, put in order in LDS.
 //
-// Weights are exp in 64 bits, rounded to whole multiples of 2^-s of the
-// largest (s = 62 less the bits of the row's length, so that a row's sum
-// fits 64 bits): integer sums are the same in any order, so histograms may be
-// filled with atomics and still every run draws the same token, and with 44
-// bits at a vocabulary of 151936 a draw differs from one in real numbers only
-// where u falls within about 1e-13 of a border.
-#include <cfloat>
+// Steps and weights: y = l * 4 / (T ln 2) in 64 bits, step floor(y), weight
+// 2^((y - a) / 4) with a the largest step of the part. A part's sums are of
+// weights in whole multiples of 2^-49: integers, so the order of the LDS
+// atomics does not matter. A token more than 49 octaves below the largest has
+// no weight and is not drawn. Parts are added in 64-bit floats in
+// a fixed order. Running sums so are good to about 1e-14, and a draw differs
+// from one in real numbers only where u falls that near to a border: with
+// 32-bit weights, about one draw in 1000 of an unfiltered row of 151936.
+#include <cmath>
 
 #include "common.h"
 #include "device.h"
@@ -24,9 +29,14 @@
 namespace qwh {
 namespace {
 
+constexpr uint32_t kPart = 4096;       // logits of a first-pass workgroup
+constexpr uint32_t kBins = 256;        // of the arrays
+constexpr uint32_t kDead = 197;        // the step of tokens without a weight: those before it weigh 2^-49 and more
+constexpr uint32_t kShort = 256;       // tokens kept beside a part's histogram
+constexpr uint32_t kList = 4096;       // tokens that the second pass puts in order
 constexpr int kThreads = 1024;
-constexpr uint32_t kBins = 2048;          // the last: tokens without a weight
-constexpr uint32_t kList = 4096;          // tokens of a step that are put in order in LDS
+constexpr double kUnit = 0x1p49;       // a weight of 1 in a part's integer sums
+constexpr uint32_t kPartsAtOnce = 32768;  // of a launch (160 MB of scratch)
 
 // Order-preserving bits of a logit (0: NaN, never drawn); -0 counts as 0.
 __device__ __forceinline__ uint32_t logit_key(float l) {
@@ -41,81 +51,175 @@ __device__ __forceinline__ float key_logit(uint32_t key) {
 
 constexpr uint32_t kKeyMinusInf = 0x007fffffu, kKeyPlusInf = 0xff800000u;
 
-// What turns a row's logits into weights.
-struct RowWeights {
-    double top, heat;    // the largest logit, the temperature
-    double bins_per_nat;
-    int shift;           // s
-    bool infinite;       // the largest is +infinity
+__device__ __forceinline__ bool is_greedy(const qwh_sampling &p) { return !(p.temperature > 0.0f) || p.top_k == 1; }
 
-    __device__ double below(uint32_t key) const { return (top - (double)key_logit(key)) / heat; }
-    // exp(-below), of the row's largest.
-    __device__ double weight(uint32_t key) const {
-        if (key <= kKeyMinusInf) return 0.0;
-        if (infinite) return key == kKeyPlusInf ? 1.0 : 0.0;
-        return exp(-below(key));
-    }
-    __device__ uint64_t fixed(double w) const { return (uint64_t)rint(ldexp(w, shift)); }
-    // The step of a key: never falls as the logit falls. Past 2^-(s + 1) of
-    // the largest there is no weight left.
+// 4 / (T ln 2).
+__device__ __forceinline__ double steps_per_logit(float temperature) { return 5.770780163555853 / (double)temperature; }
+
+// a * b, not fused into what it is added to.
+__device__ __forceinline__ double rounded_product(double a, double b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+
+// Weights against a reference step (infinite where the largest logit is: then
+// such logits weigh 1 and others nothing).
+struct Weights {
+    double c, reference;
+    bool infinite;
+
+    __device__ Weights(double c_, uint32_t top_key)
+        : c(c_), reference(floor(rounded_product((double)key_logit(top_key), c_))), infinite(top_key == kKeyPlusInf) {}
+    // A logit's step below the reference, at most kDead (no weight).
     __device__ uint32_t bin(uint32_t key) const {
-        if (key <= kKeyMinusInf) return kBins - 1;
-        if (infinite) return key == kKeyPlusInf ? 0u : kBins - 1;
-        return (uint32_t)fmin(below(key) * bins_per_nat, (double)(kBins - 1));
+        if (key <= kKeyMinusInf) return kDead;
+        if (infinite) return key == kKeyPlusInf ? 0 : kDead;
+        return (uint32_t)fmin(reference - floor(rounded_product((double)key_logit(key), c)), (double)kDead);
+    }
+    __device__ double weight(uint32_t key) const {
+        if (infinite) return key == kKeyPlusInf ? 1.0 : 0.0;
+        // (The product rounded first, as the reference's is: fused, the
+        // largest finite logits would leave its rounding error.)
+        return exp2((rounded_product((double)key_logit(key), c) - reference) * 0.25);
     }
 };
 
-__device__ __forceinline__ RowWeights row_weights(uint32_t top_key, float temperature, uint32_t count) {
-    RowWeights r;
-    r.top = (double)key_logit(top_key);
-    r.heat = (double)temperature;
-    r.infinite = top_key == kKeyPlusInf;
-    r.shift = 62 - (32 - __builtin_clz(count));
-    r.bins_per_nat = (double)(kBins - 1) / ((r.shift + 1) * 0.69314718055994530942);
-    return r;
+// What the first pass leaves of a part.
+struct Part {
+    uint64_t best;           // (key, ~index) of the largest
+    uint32_t kept, kept_bins;  // tokens in `tokens`: all of the steps below kept_bins
+    uint16_t count[kBins];
+    uint64_t mass[kBins];
+    uint64_t tokens[kShort];  // (~key, index)
+};
+
+__device__ __forceinline__ uint64_t wave_largest(uint64_t v) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+        const uint64_t o = __shfl_xor((unsigned long long)v, m, 64);
+        v = o > v ? o : v;
+    }
+    return v;
 }
 
-// Calls f(key, index) for the row's elements, some of them by each thread.
-template <typename F>
-__device__ __forceinline__ void each_logit(const float *row, uint32_t count, F f) {
-    if ((reinterpret_cast<uintptr_t>(row) & 15u) == 0) {
-        const uint32_t quads = count / 4;
-        for (uint32_t i = threadIdx.x; i < quads; i += kThreads) {
-            const float4 v = reinterpret_cast<const float4 *>(row)[i];
-            f(logit_key(v.x), 4 * i);
-            f(logit_key(v.y), 4 * i + 1);
-            f(logit_key(v.z), 4 * i + 2);
-            f(logit_key(v.w), 4 * i + 3);
+__global__ __launch_bounds__(256) void sample_parts_kernel(const float *logits, uint32_t count, const qwh_sampling *params,
+                                                           Part *parts) {
+    __shared__ uint32_t bins[kBins];
+    __shared__ unsigned long long masses[kBins];
+    __shared__ uint64_t wave_best[4];
+    __shared__ uint32_t wave_sum[4], kept, kept_bins;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float *row = logits + (size_t)blockIdx.y * count;
+    Part &part = parts[(size_t)blockIdx.y * gridDim.x + blockIdx.x];
+    const uint32_t first = blockIdx.x * kPart, n = min(kPart, count - first);
+    const qwh_sampling p = params[blockIdx.y];
+    bins[tid] = 0;
+    masses[tid] = 0;
+    if (tid == 0) kept = kept_bins = 0;
+    // Sixteen logits a thread, four in a row: 16-byte loads where the row
+    // allows them.
+    uint32_t key[16];
+    const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15u) == 0 && n == kPart;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t at = 1024 * k + 4 * tid;
+        if (aligned) {
+            const float4 v = *reinterpret_cast<const float4 *>(row + first + at);
+            key[4 * k] = logit_key(v.x);
+            key[4 * k + 1] = logit_key(v.y);
+            key[4 * k + 2] = logit_key(v.z);
+            key[4 * k + 3] = logit_key(v.w);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) key[4 * k + j] = at + j < n ? logit_key(row[first + at + j]) : 0u;
         }
-        const uint32_t i = 4 * quads + threadIdx.x;
-        if (i < count) f(logit_key(row[i]), i);
+    }
+    uint64_t best = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const uint64_t v = (uint64_t)key[i] << 32 | (uint32_t) ~(first + 1024 * (i / 4) + 4 * tid + i % 4);
+        best = v > best ? v : best;
+    }
+    best = wave_largest(best);
+    if (lane == 0) wave_best[wave] = best;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) best = wave_best[w] > best ? wave_best[w] : best;
+    const uint32_t top_key = (uint32_t)(best >> 32);
+    if (tid == 0) part.best = best;
+    if (is_greedy(p) || top_key <= kKeyMinusInf) {  // (no weight in this part: no token of it is asked for)
+        part.count[tid] = 0;
+        part.mass[tid] = 0;
+        if (tid == 0) {
+            part.kept = 0;
+            part.kept_bins = kBins;
+        }
         return;
     }
-    for (uint32_t i = threadIdx.x; i < count; i += kThreads) f(logit_key(row[i]), i);
+    const Weights w(steps_per_logit(p.temperature), top_key);
+    uint8_t bin[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t b = w.bin(key[i]);
+        bin[i] = (uint8_t)b;
+        if (b == kDead) continue;
+        atomicAdd(&bins[b], 1u);
+        atomicAdd(&masses[b], (unsigned long long)rint(w.weight(key[i]) * kUnit));
+    }
+    __syncthreads();
+    // The steps whose tokens fit the short list.
+    uint32_t sum = tid >= (int)kDead ? kShort + 1 : bins[tid];
+    part.count[tid] = (uint16_t)bins[tid];
+    part.mass[tid] = masses[tid];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(sum, d, 64);
+        if (lane >= d) sum += o;
+    }
+    if (lane == 63) wave_sum[wave] = sum;
+    __syncthreads();
+    for (int i = 0; i < wave; ++i) sum += wave_sum[i];
+    const uint64_t fits = __ballot(sum <= kShort);
+    if (lane == 0 && fits) atomicMax(&kept_bins, 64 * wave + (uint32_t)__popcll(fits));
+    __syncthreads();
+    const uint32_t below = kept_bins;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (bin[i] < below) {
+            const uint32_t at = atomicAdd(&kept, 1u);
+            part.tokens[at] = (uint64_t)~key[i] << 32 | (first + 1024 * (i / 4) + 4 * tid + i % 4);
+        }
+    __syncthreads();
+    if (tid == 0) {
+        part.kept = kept;
+        part.kept_bins = below;
+    }
 }
 
-struct SampleShared {
-    uint32_t count[kBins];   // per step; then before the step
-    uint64_t mass[kBins];
-    uint64_t list[kList];    // (~key, index): ascending is the row's order
-    uint64_t wave[16];
+struct RowShared {
+    double mass[kBins];      // before each step; at the last: all
+    uint32_t count[kBins];
+    uint32_t sums_n[4][kBins];
+    double sums_m[4][kBins];
+    uint64_t list[kList];
+    double run[kList];       // running sums of the ordered list
+    double wave_m[16];
     uint32_t wave_n[16];
-    uint64_t best;
-    uint32_t listed, at_least, found_bin, found_index, tie_index;
-    uint32_t found_count;
-    uint64_t found_mass, total;
-    uint32_t live;
+    uint64_t wave_best[16];
+    uint32_t listed, found, found_index;
+    double found_mass;
+    uint32_t found_count, counted, tie;
     uint32_t digits[256];
-    uint64_t digit_mass[256];
+    unsigned long long digit_mass[256];
 };
 
 // Inclusive sums over the workgroup, in thread order.
-__device__ __forceinline__ void block_scan(SampleShared &sh, uint32_t &n, uint64_t &m) {
+__device__ __forceinline__ void block_scan(RowShared &sh, uint32_t &n, double &m) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const uint32_t n2 = __shfl_up(n, d, 64);
-        const uint64_t m2 = __shfl_up((unsigned long long)m, d, 64);
+        const double m2 = __shfl_up(m, d, 64);
         if (lane >= d) {
             n += n2;
             m += m2;
@@ -124,249 +228,406 @@ __device__ __forceinline__ void block_scan(SampleShared &sh, uint32_t &n, uint64
     __syncthreads();
     if (lane == 63) {
         sh.wave_n[wave] = n;
-        sh.wave[wave] = m;
+        sh.wave_m[wave] = m;
     }
     __syncthreads();
+    uint32_t n0 = 0;
+    double m0 = 0.0;
     for (int w = 0; w < wave; ++w) {
-        n += sh.wave_n[w];
-        m += sh.wave[w];
+        n0 += sh.wave_n[w];
+        m0 += sh.wave_m[w];
     }
+    n += n0;
+    m += m0;
 }
 
-// Where a place is asked for: the first token of the order at which the
-// running count, or the running sum, reaches `at` (at least 1).
-struct Place {
-    bool by_mass;
-    uint64_t at;
-    __device__ bool reached(uint32_t n, uint64_t m) const { return (by_mass ? m : n) >= at; }
+struct Row {
+    const float *logits;
+    uint32_t count, n_parts;
+    const Part *parts;
+    Weights w;
+
+    // Calls f(key, index) for the row's tokens of steps lo .. hi, each once,
+    // a wavefront a part: from the part's short list where that has them, or
+    // from the logits where some lie behind it.
+    template <typename F>
+    __device__ void each(uint32_t lo, uint32_t hi, F f) const {
+        const int lane = threadIdx.x & 63;
+        for (uint32_t i = threadIdx.x >> 6; i < n_parts; i += kThreads / 64) {
+            const Part &part = parts[i];
+            const uint32_t top = (uint32_t)(part.best >> 32);
+            if (top <= kKeyMinusInf) continue;
+            // The part's steps below the row's.
+            const Weights own(w.c, top);
+            const double shift = own.infinite == w.infinite ? (w.infinite ? 0.0 : w.reference - own.reference) : (double)kBins;
+            if (shift > (double)hi) continue;
+            const uint32_t s = (uint32_t)shift, last = hi - s;  // the part's last step asked for
+            bool beyond = false;
+            for (uint32_t b = max(part.kept_bins, lo > s ? lo - s : 0); b <= last; b += 64)
+                beyond |= __ballot(b + lane <= last && b + lane < kDead && part.count[b + lane]) != 0;
+            if (!beyond) {
+                for (uint32_t k = lane; k < part.kept; k += 64) {
+                    const uint64_t t = part.tokens[k];
+                    const uint32_t b = w.bin((uint32_t)(~t >> 32));
+                    if (b >= lo && b <= hi) f((uint32_t)(~t >> 32), (uint32_t)t);
+                }
+                continue;
+            }
+            const uint32_t begin = i * kPart, end = min(begin + kPart, count);
+            for (uint32_t k = begin + lane; k < end; k += 64) {
+                const uint32_t key = logit_key(logits[k]);
+                const uint32_t b = w.bin(key);
+                if (b >= lo && b <= hi && b < kDead) f(key, k);
+            }
+        }
+    }
 };
 
-// The place in the row: found_index the token there, found_count and
-// found_mass the running count and sum with it. It lies in some step (the
-// caller asks for no place behind the last token with a weight).
-__device__ void find_place(SampleShared &sh, const float *row, uint32_t count, const RowWeights &rw, const Place &p) {
+// Tokens of steps lo .. hi (n of them, at most kList) in order in sh.list,
+// sh.run their running sums on top of `before`.
+__device__ void order_steps(RowShared &sh, const Row &row, uint32_t lo, uint32_t hi, uint32_t n, double before) {
     const int tid = threadIdx.x;
     __syncthreads();
-    // sh.count / sh.mass hold what lies before each step (and at [kBins - 1]
-    // the totals).
-    for (uint32_t b = tid; b + 1 < kBins; b += kThreads)
-        if (!p.reached(sh.count[b], sh.mass[b]) && p.reached(sh.count[b + 1], sh.mass[b + 1])) sh.found_bin = b;
     if (tid == 0) sh.listed = 0;
     __syncthreads();
-    const uint32_t bin = sh.found_bin;
-    const uint32_t n0 = sh.count[bin], n = sh.count[bin + 1] - n0;
-    const uint64_t m0 = sh.mass[bin];
-    if (n <= kList) {
-        each_logit(row, count, [&](uint32_t key, uint32_t i) {
-            if (rw.bin(key) == bin) sh.list[atomicAdd(&sh.listed, 1u)] = (uint64_t)~key << 32 | i;
-        });
-        uint32_t padded = 2;
-        while (padded < n) padded *= 2;
-        for (uint32_t i = n + tid; i < padded; i += kThreads) sh.list[i] = ~0ull;
-        for (uint32_t size = 2; size <= padded; size *= 2) {
-            for (uint32_t step = size / 2; step >= 1; step /= 2) {
-                __syncthreads();
-                for (uint32_t k = tid; k < padded / 2; k += kThreads) {
-                    const uint32_t i = 2 * k - (k & (step - 1)), j = i + step;
-                    const uint64_t x = sh.list[i], y = sh.list[j];
-                    if ((x > y) == ((i & size) == 0)) {
-                        sh.list[i] = y;
-                        sh.list[j] = x;
-                    }
+    row.each(lo, hi, [&](uint32_t key, uint32_t i) {
+        const uint32_t at = atomicAdd(&sh.listed, 1u);
+        if (at < kList) sh.list[at] = (uint64_t)~key << 32 | i;
+    });
+    uint32_t padded = 64;
+    while (padded < n) padded *= 2;
+    __syncthreads();
+    for (uint32_t i = min(sh.listed, n) + tid; i < padded; i += kThreads) sh.list[i] = ~0ull;
+    for (uint32_t size = 2; size <= padded; size *= 2) {
+        for (uint32_t step = size / 2; step >= 1; step /= 2) {
+            // (Pairs within 64 entries are one wavefront's, from the second
+            // step of them on.)
+            __syncthreads();
+            for (uint32_t k = tid; k < padded / 2; k += kThreads) {
+                const uint32_t i = 2 * k - (k & (step - 1)), j = i + step;
+                const uint64_t x = sh.list[i], y = sh.list[j];
+                if ((x > y) == ((i & size) == 0)) {
+                    sh.list[i] = y;
+                    sh.list[j] = x;
                 }
             }
         }
+    }
+    __syncthreads();
+    double w[4], sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t i = 4 * tid + k;
+        w[k] = i < n && sh.list[i] != ~0ull ? row.w.weight((uint32_t)(~sh.list[i] >> 32)) : 0.0;
+        sum += w[k];
+    }
+    uint32_t none = 0;
+    double run = sum;
+    block_scan(sh, none, run);
+    run = before + (run - sum);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t i = 4 * tid + k;
+        run += w[k];
+        if (i < n) sh.run[i] = run;
+    }
+    __syncthreads();
+}
+
+// The first entry of the ordered list (of n) whose running sum reaches
+// (`past`: exceeds) `at`; the last if none does.
+__device__ uint32_t reach(RowShared &sh, uint32_t n, double at, bool past) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.found = n - 1;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+        const bool here = past ? sh.run[i] > at : sh.run[i] >= at;
+        const bool before = i > 0 && (past ? sh.run[i - 1] > at : sh.run[i - 1] >= at);
+        if (here && !before) atomicMin(&sh.found, i);
+    }
+    __syncthreads();
+    return sh.found;
+}
+
+// The step in which the count (`by_mass`: the sum) reaches `at` (past:
+// exceeds it): the last step with tokens if none does.
+__device__ uint32_t step_of(RowShared &sh, bool by_mass, double at, bool past) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.found = kBins;
+    __syncthreads();
+    const uint32_t b = threadIdx.x;
+    if (b < kDead && sh.count[b + 1] > sh.count[b]) {
+        const double v = by_mass ? sh.mass[b + 1] : (double)sh.count[b + 1];
+        if (past ? v > at : v >= at) atomicMin(&sh.found, b);
+    }
+    __syncthreads();
+    if (sh.found == kBins) {  // (uniform; the sums' last bits)
         __syncthreads();
-        // Running sums over the ordered list, four tokens a thread.
-        uint32_t mine = 0;
-        uint64_t w[4], sum = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint32_t i = 4 * tid + k;
-            w[k] = 0;
-            if (i < n) {
-                w[k] = rw.fixed(rw.weight((uint32_t)(~sh.list[i] >> 32)));
-                ++mine;
-                sum += w[k];
-            }
-        }
-        uint32_t run_n = mine;
-        uint64_t run_m = sum;
-        block_scan(sh, run_n, run_m);
-        run_n += n0 - mine;
-        run_m += m0 - sum;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint32_t i = 4 * tid + k;
-            if (i >= n) break;
-            const bool before = p.reached(run_n, run_m);
-            ++run_n;
-            run_m += w[k];
-            if (!before && p.reached(run_n, run_m)) {
-                sh.found_index = (uint32_t)sh.list[i];
-                sh.found_count = run_n;
-                sh.found_mass = run_m;
-            }
+        if (threadIdx.x == 0) sh.found = 0;
+        __syncthreads();
+        if (b < kDead && sh.count[b + 1] > sh.count[b]) atomicMax(&sh.found, b);
+        __syncthreads();
+    }
+    return sh.found;
+}
+
+// A place in step `bin`: the entry where the count (by_mass: sum) reaches
+// `at` (past: exceeds it). found_index, and count and sum up to it.
+__device__ void place_in(RowShared &sh, const Row &row, uint32_t bin, bool by_mass, double at, bool past) {
+    const int tid = threadIdx.x;
+    const uint32_t n0 = sh.count[bin], n = sh.count[bin + 1] - n0;
+    const double m0 = sh.mass[bin];
+    if (n <= kList) {
+        order_steps(sh, row, bin, bin, n, m0);
+        const uint32_t k = by_mass ? reach(sh, n, at, past) : (uint32_t)fmin(fmax(at - n0, 1.0), (double)n) - 1;
+        __syncthreads();
+        if (tid == 0) {
+            sh.found_index = (uint32_t)sh.list[k];
+            sh.found_count = n0 + k + 1;
+            sh.found_mass = sh.run[k];
         }
         __syncthreads();
         return;
     }
     // More tokens than the list holds: the key at the place digit by digit,
-    // each pass a histogram of the step's tokens that share the digits so far.
-    uint32_t prefix = 0, nb = n0;
-    uint64_t mb = m0;
+    // each pass a histogram of the step's tokens that share the digits so far
+    // (sums in integers again: 4096 and more of them, in multiples of 2^-36).
+    uint32_t prefix = 0;
+    double nb = n0, mb = m0;
     for (int digit = 3; digit >= 0; --digit) {
-        for (int i = tid; i < 256; i += kThreads) {
-            sh.digits[i] = 0;
-            sh.digit_mass[i] = 0;
+        __syncthreads();
+        if (tid < 256) {
+            sh.digits[tid] = 0;
+            sh.digit_mass[tid] = 0;
         }
         __syncthreads();
-        each_logit(row, count, [&](uint32_t key, uint32_t) {
-            if (rw.bin(key) != bin || (digit < 3 && (key >> (8 * digit + 8)) != prefix)) return;
+        row.each(bin, bin, [&](uint32_t key, uint32_t) {
+            if (digit < 3 && (key >> (8 * digit + 8)) != prefix) return;
             const uint32_t d = 255u - ((key >> (8 * digit)) & 255u);
             atomicAdd(&sh.digits[d], 1u);
-            atomicAdd(reinterpret_cast<unsigned long long *>(&sh.digit_mass[d]), (unsigned long long)rw.fixed(rw.weight(key)));
+            // (Within a step weights differ by 2^(1/4) at most: against the
+            // step's own, so that small ones keep their bits.)
+            atomicAdd(&sh.digit_mass[d], (unsigned long long)rint(row.w.weight(key) * exp2(0.25 * bin) * 0x1p36));
         });
         __syncthreads();
+        const double unit = exp2(-0.25 * bin) * 0x1p-36;
         const uint32_t mine = tid < 256 ? sh.digits[tid] : 0;
-        const uint64_t mass = tid < 256 ? sh.digit_mass[tid] : 0;
+        const double mass = tid < 256 ? (double)sh.digit_mass[tid] * unit : 0.0;
         uint32_t run_n = mine;
-        uint64_t run_m = mass;
+        double run_m = mass;
         block_scan(sh, run_n, run_m);
-        if (!p.reached(nb + run_n - mine, mb + run_m - mass) && p.reached(nb + run_n, mb + run_m)) {
-            sh.found_bin = 255u - tid;
-            sh.found_count = nb + run_n - mine;
-            sh.found_mass = mb + run_m - mass;
+        if (tid == 0) sh.found = 256;
+        __syncthreads();
+        const double v = by_mass ? mb + run_m : nb + run_n;
+        if (mine && (past ? v > at : v >= at)) atomicMin(&sh.found, (uint32_t)tid);
+        __syncthreads();
+        if (sh.found == 256) {
+            __syncthreads();
+            if (tid == 0) sh.found = 0;
+            __syncthreads();
+            if (mine) atomicMax(&sh.found, (uint32_t)tid);
+            __syncthreads();
+        }
+        const uint32_t d = sh.found;
+        if (tid == (int)d) {
+            sh.found_count = run_n - mine;
+            sh.found_mass = run_m - mass;
         }
         __syncthreads();
-        prefix = prefix << 8 | sh.found_bin;
-        nb = sh.found_count;
-        mb = sh.found_mass;
+        prefix = prefix << 8 | (255u - d);
+        nb += sh.found_count;
+        mb += sh.found_mass;
         __syncthreads();
     }
     // Tokens of one logit, in index order, all of one weight: which of them.
-    const uint64_t w = rw.fixed(rw.weight(prefix));
-    uint32_t low = 1, high = count;  // the place's number among them
-    while (low < high) {
-        const uint32_t mid = low + (high - low) / 2;
-        if (p.reached(nb + mid, mb + mid * w)) high = mid;
-        else low = mid + 1;
-    }
+    const double w = row.w.weight(prefix);
+    const uint32_t ties = sh.digits[255u - (prefix & 255u)];
+    double nth = by_mass ? (past ? floor((at - mb) / w) + 1.0 : ceil((at - mb) / w)) : at - nb;
+    nth = fmin(fmax(nth, 1.0), (double)ties);
+    const uint32_t low = (uint32_t)nth;
     uint32_t seen = 0;  // of them before this stretch
-    for (uint32_t base = 0; base < count; base += kThreads) {
+    for (uint32_t base = 0; base < row.count; base += kThreads) {
         const uint32_t i = base + tid;
-        uint32_t run = i < count && logit_key(row[i]) == prefix ? 1u : 0u;
+        uint32_t run = i < row.count && logit_key(row.logits[i]) == prefix ? 1u : 0u;
         const uint32_t own = run;
-        uint64_t none = 0;
+        double none = 0.0;
         block_scan(sh, run, none);
         if (own && seen + run == low) sh.found_index = i;
-        if (tid == kThreads - 1) sh.tie_index = run;
+        if (tid == kThreads - 1) sh.tie = run;
         __syncthreads();
-        seen += sh.tie_index;
+        seen += sh.tie;
         __syncthreads();
         if (seen >= low) break;
     }
     if (tid == 0) {
-        sh.found_count = nb + low;
+        sh.found_count = (uint32_t)(nb + low);
         sh.found_mass = mb + low * w;
     }
     __syncthreads();
 }
 
-__global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logits, uint32_t count, const qwh_sampling *params,
-                                                               const float *uniform, uint32_t *ids) {
-    __shared__ SampleShared sh;
+__global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logits, uint32_t count, uint32_t n_parts,
+                                                               const qwh_sampling *params, const float *uniform,
+                                                               const Part *all_parts, uint32_t *ids) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_row[];
+    RowShared &sh = *reinterpret_cast<RowShared *>(lds_row);
     const int tid = threadIdx.x;
-    const float *row = logits + (size_t)blockIdx.x * count;
     const qwh_sampling p = params[blockIdx.x];
+    const Part *parts = all_parts + (size_t)blockIdx.x * n_parts;
     // The largest logit, the lowest index among equal ones.
     uint64_t best = 0;
-    each_logit(row, count, [&](uint32_t key, uint32_t i) {
-        const uint64_t v = (uint64_t)key << 32 | (uint32_t)~i;
-        best = v > best ? v : best;
-    });
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-        const uint64_t o = __shfl_xor((unsigned long long)best, m, 64);
-        best = o > best ? o : best;
-    }
-    if ((tid & 63) == 0) sh.wave[tid >> 6] = best;
+    for (uint32_t i = tid; i < n_parts; i += kThreads) best = parts[i].best > best ? parts[i].best : best;
+    best = wave_largest(best);
+    if ((tid & 63) == 0) sh.wave_best[tid >> 6] = best;
     __syncthreads();
-    for (int w = 0; w < kThreads / 64; ++w) best = sh.wave[w] > best ? sh.wave[w] : best;
-    __syncthreads();
+    for (int w = 0; w < kThreads / 64; ++w) best = sh.wave_best[w] > best ? sh.wave_best[w] : best;
     const uint32_t top_key = (uint32_t)(best >> 32);
-    if (!(p.temperature > 0.0f) || top_key <= kKeyMinusInf || p.top_k == 1) {
+    if (is_greedy(p) || top_key <= kKeyMinusInf) {
         if (tid == 0) ids[blockIdx.x] = top_key <= kKeyMinusInf ? 0u : ~(uint32_t)best;
         return;
     }
-    const RowWeights rw = row_weights(top_key, p.temperature, count);
-    const double least = p.min_p > 0.0f ? (double)fminf(p.min_p, 1.0f) : 0.0;
-    for (uint32_t b = tid; b < kBins; b += kThreads) {
-        sh.count[b] = 0;
-        sh.mass[b] = 0;
-    }
-    if (tid == 0) sh.at_least = 0;
-    __syncthreads();
-    uint32_t mine = 0;
-    each_logit(row, count, [&](uint32_t key, uint32_t) {
-        const uint32_t b = rw.bin(key);
-        if (b == kBins - 1) return;
-        const double w = rw.weight(key);
-        atomicAdd(&sh.count[b], 1u);
-        atomicAdd(reinterpret_cast<unsigned long long *>(&sh.mass[b]), (unsigned long long)rw.fixed(w));
-        mine += w >= least;
-    });
-    if (mine) atomicAdd(&sh.at_least, mine);
-    __syncthreads();
+    const Row row{logits + (size_t)blockIdx.x * count, count, n_parts, parts, Weights(steps_per_logit(p.temperature), top_key)};
+    // The parts' histograms, each shifted by its own largest step: four
+    // threads a step, every fourth part each.
     {
-        // Sums before each step.
-        const uint32_t n0 = sh.count[2 * tid], n1 = sh.count[2 * tid + 1];
-        const uint64_t m0 = sh.mass[2 * tid], m1 = sh.mass[2 * tid + 1];
-        uint32_t n = n0 + n1;
-        uint64_t m = m0 + m1;
-        block_scan(sh, n, m);
-        sh.count[2 * tid] = n - n0 - n1;
-        sh.mass[2 * tid] = m - m0 - m1;
-        sh.count[2 * tid + 1] = n - n1;
-        sh.mass[2 * tid + 1] = m - m1;
+        const uint32_t b = tid & (kBins - 1), group = tid / kBins;
+        uint32_t n = 0;
+        double m = 0.0;
+        for (uint32_t i = group; i < n_parts; i += kThreads / kBins) {
+            const uint32_t top = (uint32_t)(parts[i].best >> 32);
+            const Weights own(row.w.c, top);
+            const double shift = own.infinite == row.w.infinite ? (own.infinite ? 0.0 : row.w.reference - own.reference) : (double)kBins;
+            if (top <= kKeyMinusInf || shift > (double)b || b >= kDead) continue;
+            const uint32_t at = b - (uint32_t)shift;
+            n += parts[i].count[at];
+            m += (double)parts[i].mass[at] * exp2(-0.25 * shift);
+        }
+        sh.sums_n[group][b] = n;
+        sh.sums_m[group][b] = m;
+        __syncthreads();
+        uint32_t run_n = 0;
+        double run_m = 0.0;
+        if (group == 0) {
+            run_n = n = (sh.sums_n[0][b] + sh.sums_n[1][b]) + (sh.sums_n[2][b] + sh.sums_n[3][b]);
+            run_m = m = ((sh.sums_m[0][b] + sh.sums_m[1][b]) + (sh.sums_m[2][b] + sh.sums_m[3][b])) * (1.0 / kUnit);
+        }
+        block_scan(sh, run_n, run_m);
+        if (group == 0) {
+            // Before the step; the next step's is this one's end, exactly.
+            if (b + 1 < kBins) {
+                sh.count[b + 1] = run_n;
+                sh.mass[b + 1] = run_m;
+            }
+            if (b == 0) {
+                sh.count[0] = 0;
+                sh.mass[0] = 0.0;
+            }
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    const uint32_t live = sh.count[kBins - 1];
-    uint64_t kept = sh.mass[kBins - 1];  // the sum of the first `tokens`
-    uint32_t tokens = live;
-    if (p.top_k > 0 && p.top_k < live) {
-        find_place(sh, row, count, rw, Place{false, p.top_k});
-        tokens = sh.found_count;
-        kept = sh.found_mass;
-    }
-    if (p.top_p < 1.0f) {
-        // A token is kept while the sum before it is below top_p * kept: the
-        // last one is where the sum reaches it.
-        const double reach = fmax((double)p.top_p * (double)kept, 1.0);
-        find_place(sh, row, count, rw, Place{true, (uint64_t)ceil(reach)});
-        tokens = sh.found_count;
-        kept = sh.found_mass;
-    }
-    const uint32_t least_tokens = least > 0.0 ? (sh.at_least > 1 ? sh.at_least : 1u) : tokens;
-    if (least_tokens < tokens) {
-        find_place(sh, row, count, rw, Place{false, least_tokens});
-        kept = sh.found_mass;
-    }
+    const uint32_t live = sh.count[kDead];
+    const bool by_k = p.top_k > 0 && p.top_k < live, by_p = p.top_p < 1.0f;
+    const double least = p.min_p > 0.0f ? (double)fminf(p.min_p, 1.0f) : 0.0;
+    const double top = (double)key_logit(top_key), heat = (double)p.temperature;
+    const auto enough = [&](uint32_t key) {
+        return row.w.infinite || exp(((double)key_logit(key) - top) / heat) >= least;
+    };
     const float u = uniform[blockIdx.x];
-    // The first token past u * kept; from u = 1 on the last one with a weight.
-    const double target = (u > 0.0f ? fmin((double)u, 1.0) : 0.0) * (double)kept;
-    const uint64_t past = (uint64_t)target;
-    find_place(sh, row, count, rw, Place{true, past < kept ? past + 1 : kept});
+    const double draw = u > 0.0f ? fmin((double)u, 1.0) : 0.0;
+    // The last step that any rule can keep a token of.
+    uint32_t last = step_of(sh, false, (double)live, false);
+    if (by_k) last = min(last, step_of(sh, false, (double)p.top_k, false));
+    else if (by_p) last = min(last, step_of(sh, true, (double)p.top_p * sh.mass[kDead], false));
+    else if (least > 0.0 && !row.w.infinite) last = min(last, (uint32_t)fmin(row.w.reference - floor(top * row.w.c + 4.0 * log2(least)) + 1.0, (double)(kDead - 1)));
+    const uint32_t n = sh.count[last + 1];
+    if ((by_k || by_p || least > 0.0) && n <= kList) {
+        // All that may be kept fits the list: the rules one after another on
+        // its running sums.
+        order_steps(sh, row, 0, last, n, 0.0);
+        uint32_t tokens = by_k ? min(p.top_k, n) : n;
+        if (by_p) {
+            const double whole = by_k ? sh.run[tokens - 1] : sh.mass[kDead];
+            tokens = min(tokens, reach(sh, tokens, (double)p.top_p * whole, false) + 1);
+        }
+        if (least > 0.0) {
+            __syncthreads();
+            if (tid == 0) sh.counted = 0;
+            __syncthreads();
+            uint32_t mine = 0;
+            for (uint32_t i = tid; i < tokens; i += kThreads) mine += enough((uint32_t)(~sh.list[i] >> 32));
+            if (mine) atomicAdd(&sh.counted, mine);
+            __syncthreads();
+            tokens = max(sh.counted, 1u);
+        }
+        const double kept = sh.run[tokens - 1];
+        const uint32_t k = draw >= 1.0 ? tokens - 1 : reach(sh, tokens, draw * kept, true);
+        __syncthreads();
+        if (tid == 0) ids[blockIdx.x] = (uint32_t)sh.list[min(k, tokens - 1)];
+        return;
+    }
+    // Otherwise each place by itself.
+    double kept = sh.mass[kDead];
+    uint32_t tokens = live;
+    if (by_k) {
+        place_in(sh, row, step_of(sh, false, (double)p.top_k, false), false, (double)p.top_k, false);
+        tokens = sh.found_count;
+        kept = sh.found_mass;
+    }
+    if (by_p) {
+        const double at = (double)p.top_p * kept;
+        place_in(sh, row, step_of(sh, true, at, false), true, at, false);
+        tokens = sh.found_count;
+        kept = sh.found_mass;
+    }
+    if (least > 0.0 && !row.w.infinite) {
+        // Tokens of at least min_p: all of the steps above its own and the
+        // one before that, and those of the next three that are.
+        const double at = row.w.reference - floor(top * row.w.c + 4.0 * log2(least)) - 1.0;
+        const uint32_t lo = (uint32_t)fmin(fmax(at, 0.0), (double)(kDead - 1)), hi = min(lo + 2, kDead - 1);
+        __syncthreads();
+        if (tid == 0) sh.counted = 0;
+        __syncthreads();
+        row.each(lo, hi, [&](uint32_t key, uint32_t) {
+            if (enough(key)) atomicAdd(&sh.counted, 1u);
+        });
+        __syncthreads();
+        const uint32_t reaching = max(sh.count[lo] + sh.counted, 1u);
+        if (reaching < tokens) {
+            tokens = reaching;
+            place_in(sh, row, step_of(sh, false, (double)tokens, false), false, (double)tokens, false);
+            kept = sh.found_mass;
+        }
+    }
+    if (draw >= 1.0) place_in(sh, row, step_of(sh, false, (double)tokens, false), false, (double)tokens, false);
+    else place_in(sh, row, step_of(sh, true, draw * kept, true), true, draw * kept, true);
     if (tid == 0) ids[blockIdx.x] = sh.found_index;
+}
+
+uint32_t parts_of(uint32_t count) { return (count + kPart - 1) / kPart; }
+uint32_t rows_at_once(uint32_t rows, uint32_t count) {
+    const uint32_t most = kPartsAtOnce / parts_of(count);
+    return most < 1 ? 1 : rows < most ? rows : most;
 }
 
 }  // namespace
 
-size_t sample_scratch_bytes(uint32_t, uint32_t) { return 256; }
+size_t sample_scratch_bytes(uint32_t rows, uint32_t count) {
+    return (size_t)rows_at_once(rows, count) * parts_of(count) * sizeof(Part);
+}
 
 hipError_t launch_sample_rows(hipStream_t s, const float *logits, uint32_t rows, uint32_t count, const qwh_sampling *params,
-                              const float *uniform, void *, uint32_t *ids) {
-    sample_rows_kernel<<<rows, kThreads, 0, s>>>(logits, count, params, uniform, ids);
+                              const float *uniform, void *scratch, uint32_t *ids) {
+    const uint32_t n_parts = parts_of(count), at_once = rows_at_once(rows, count);
+    Part *parts = static_cast<Part *>(scratch);
+    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void *>(sample_rows_kernel),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(RowShared));
+    if (err != hipSuccess) return err;
+    for (uint32_t r = 0; r < rows; r += at_once) {
+        const uint32_t n = rows - r < at_once ? rows - r : at_once;
+        const float *from = logits + (size_t)r * count;
+        sample_parts_kernel<<<dim3(n_parts, n), 256, 0, s>>>(from, count, params + r, parts);
+        sample_rows_kernel<<<n, kThreads, sizeof(RowShared), s>>>(from, count, n_parts, params + r, uniform + r, parts, ids + r);
+    }
     return hipGetLastError();
 }
 
