@@ -321,7 +321,7 @@ typedef struct {
  * drawn, nor one of -infinity beside a larger one; where the largest is
  * +infinity, only those are drawn, evenly. A row with nothing but NaN and
  * -infinity gives 0. params_dev: one record per row. Weights and sums are held
- * in 64 bits and added in a fixed order; a token whose weight is below 2^-49 of
+ * in 64 bits and added in a fixed order; a token whose weight is below 2^-63 of
  * the largest is not drawn. At most 65535 rows and 2^26 logits a row. */
 int32_t qwh_sample_rows(qwh_ctx *ctx, const float *logits_dev, uint32_t rows, uint32_t count,
                         const qwh_sampling *params_dev, const float *uniform_dev, uint32_t *ids_dev);

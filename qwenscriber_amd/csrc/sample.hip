@@ -9,18 +9,19 @@
 // launch goes over the logits once, 4096 of them a workgroup, and leaves for
 // each such part a histogram over steps of a quarter octave of the weight
 // (count and sum of weights) and its tokens of the best steps, up to 256 of
-// them. A second launch, a workgroup a row, adds the histograms and then needs
-// only the tokens of the steps in which a place lies: mostly those kept
-// beside the histograms, put in order in LDS.
+// them, by step. A second launch, a workgroup a row, adds the histograms and
+// then needs only the tokens of the steps in which a place lies: mostly those
+// kept beside the histograms, put in order in LDS.
 //
-// Steps and weights: y = l * 4 / (T ln 2) in 64 bits, step floor(y), weight
-// 2^((y - a) / 4) with a the largest step of the part. A part's sums are of
-// weights in whole multiples of 2^-49: integers, so the order of the LDS
-// atomics does not matter. A token more than 49 octaves below the largest has
-// no weight and is not drawn. Parts are added in 64-bit floats in
-// a fixed order. Running sums so are good to about 1e-14, and a draw differs
-// from one in real numbers only where u falls that near to a border: with
-// 32-bit weights, about one draw in 1000 of an unfiltered row of 151936.
+// Steps and weights: y = l * 4 / (T ln 2) in 64 bits; step floor(y), the same
+// grid in every part; within a step a token weighs 2^((y - floor(y)) / 4), 1
+// to 2^(1/4), and the step itself is a power of 2^(1/4) that comes in when
+// steps are added. Within a step the sums are of weights in whole multiples
+// of 2^-37: integers, so the order of the LDS atomics does not matter, and
+// count and sum share one 64-bit word and one atomic. Running sums over steps
+// and tokens are 64-bit floats in a fixed order. A draw so differs from one
+// in real numbers only where u falls within about 1e-12 of a border; with
+// 32-bit weights, about one draw in 1000 of an unfiltered row of 151936 would.
 #include <cmath>
 
 #include "common.h"
@@ -30,12 +31,14 @@ namespace qwh {
 namespace {
 
 constexpr uint32_t kPart = 4096;       // logits of a first-pass workgroup
-constexpr uint32_t kBins = 256;        // of the arrays
-constexpr uint32_t kDead = 197;        // the step of tokens without a weight: those before it weigh 2^-49 and more
+constexpr uint32_t kBins = 256;
+constexpr uint32_t kDead = kBins - 1;  // the step of tokens that are not drawn, 63 octaves and more below the largest
 constexpr uint32_t kShort = 256;       // tokens kept beside a part's histogram
 constexpr uint32_t kList = 4096;       // tokens that the second pass puts in order
+constexpr uint32_t kRanked = 1024;     // (up to these by counting smaller ones)
 constexpr int kThreads = 1024;
-constexpr double kUnit = 0x1p49;       // a weight of 1 in a part's integer sums
+constexpr int kUnitBits = 37;          // of a weight of 1 in a step's sum
+constexpr int kCountShift = 50;        // 4096 * 2^(1/4) * 2^37 < 2^50: the count stands above the sum
 constexpr uint32_t kPartsAtOnce = 32768;  // of a launch (160 MB of scratch)
 
 // Order-preserving bits of a logit (0: NaN, never drawn); -0 counts as 0.
@@ -62,6 +65,24 @@ __device__ __forceinline__ double rounded_product(double a, double b) {
     return a * b;
 }
 
+// 2^(f / 4) for f in [0, 1): e^t about the middle of the range, t = (f - 1/2)
+// ln(2) / 4 below 0.087 in magnitude, by its series to t^9 / 9! (the next term
+// is below 1e-17).
+__device__ __forceinline__ double quarter_power(double f) {
+    const double t = (f - 0.5) * 0.17328679513998633;
+    double e = 1.0 / 362880;
+    e = fma(e, t, 1.0 / 40320);
+    e = fma(e, t, 1.0 / 5040);
+    e = fma(e, t, 1.0 / 720);
+    e = fma(e, t, 1.0 / 120);
+    e = fma(e, t, 1.0 / 24);
+    e = fma(e, t, 1.0 / 6);
+    e = fma(e, t, 0.5);
+    e = fma(e, t, 1.0);
+    e = fma(e, t, 1.0);
+    return e * 1.0905077326652577;  // 2^(1/8)
+}
+
 // Weights against a reference step (infinite where the largest logit is: then
 // such logits weigh 1 and others nothing).
 struct Weights {
@@ -70,27 +91,49 @@ struct Weights {
 
     __device__ Weights(double c_, uint32_t top_key)
         : c(c_), reference(floor(rounded_product((double)key_logit(top_key), c_))), infinite(top_key == kKeyPlusInf) {}
-    // A logit's step below the reference, at most kDead (no weight).
+    // A logit's step below the reference, at most kDead, and its weight
+    // within the step.
+    __device__ uint32_t bin(uint32_t key, double &within) const {
+        within = 1.0;
+        if (key <= kKeyMinusInf) return kDead;
+        if (infinite) return key == kKeyPlusInf ? 0 : kDead;
+        // (The product rounded first, as the reference's is: fused, the
+        // largest finite logits would leave its rounding error.)
+        const double y = rounded_product((double)key_logit(key), c), step = floor(y);
+        within = quarter_power(y - step);
+        return (uint32_t)fmin(reference - step, (double)kDead);
+    }
     __device__ uint32_t bin(uint32_t key) const {
         if (key <= kKeyMinusInf) return kDead;
         if (infinite) return key == kKeyPlusInf ? 0 : kDead;
         return (uint32_t)fmin(reference - floor(rounded_product((double)key_logit(key), c)), (double)kDead);
     }
-    __device__ double weight(uint32_t key) const {
-        if (infinite) return key == kKeyPlusInf ? 1.0 : 0.0;
-        // (The product rounded first, as the reference's is: fused, the
-        // largest finite logits would leave its rounding error.)
-        return exp2((rounded_product((double)key_logit(key), c) - reference) * 0.25);
+    // The steps between a part's largest and this one's (kDead: none of the
+    // part's tokens counts).
+    __device__ uint32_t shift(uint32_t part_top) const {
+        if (part_top <= kKeyMinusInf) return kDead;
+        if (infinite) return part_top == kKeyPlusInf ? 0 : kDead;
+        return bin(part_top);
     }
 };
 
+// A step's weight.
+__device__ __forceinline__ double step_weight(uint32_t bin) { return exp2(-0.25 * bin); }
+
+// A weight within a step as a whole number of units: the sum with 2^52 rounds
+// to one and holds it in its low bits.
+__device__ __forceinline__ uint64_t units_of(double within) {
+    const double v = within * (double)(1ull << kUnitBits) + 0x1p52;
+    return __builtin_bit_cast(uint64_t, v) & 0xfffffffffffffull;
+}
+
 // What the first pass leaves of a part.
 struct Part {
-    uint64_t best;           // (key, ~index) of the largest
-    uint32_t kept, kept_bins;  // tokens in `tokens`: all of the steps below kept_bins
-    uint16_t count[kBins];
-    uint64_t mass[kBins];
-    uint64_t tokens[kShort];  // (~key, index)
+    uint64_t best;            // (key, ~index) of the largest
+    uint32_t kept_bins, pad;  // `tokens` has all of the steps below kept_bins
+    uint64_t sum[kBins];      // a step's count << kCountShift, and its sum in units
+    uint16_t upto[kBins];     // tokens up to and with the step
+    uint64_t tokens[kShort];  // (~key, index), by step
 };
 
 __device__ __forceinline__ uint64_t wave_largest(uint64_t v) {
@@ -104,18 +147,17 @@ __device__ __forceinline__ uint64_t wave_largest(uint64_t v) {
 
 __global__ __launch_bounds__(256) void sample_parts_kernel(const float *logits, uint32_t count, const qwh_sampling *params,
                                                            Part *parts) {
-    __shared__ uint32_t bins[kBins];
-    __shared__ unsigned long long masses[kBins];
+    __shared__ unsigned long long sums[kBins];
+    __shared__ uint32_t place[kBins];
     __shared__ uint64_t wave_best[4];
-    __shared__ uint32_t wave_sum[4], kept, kept_bins;
+    __shared__ uint32_t wave_sum[4], kept_bins;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float *row = logits + (size_t)blockIdx.y * count;
     Part &part = parts[(size_t)blockIdx.y * gridDim.x + blockIdx.x];
     const uint32_t first = blockIdx.x * kPart, n = min(kPart, count - first);
     const qwh_sampling p = params[blockIdx.y];
-    bins[tid] = 0;
-    masses[tid] = 0;
-    if (tid == 0) kept = kept_bins = 0;
+    sums[tid] = 0;
+    if (tid == 0) kept_bins = 0;
     // Sixteen logits a thread, four in a row: 16-byte loads where the row
     // allows them.
     uint32_t key[16];
@@ -134,81 +176,75 @@ __global__ __launch_bounds__(256) void sample_parts_kernel(const float *logits, 
             for (int j = 0; j < 4; ++j) key[4 * k + j] = at + j < n ? logit_key(row[first + at + j]) : 0u;
         }
     }
-    uint64_t best = 0;
+    // The largest key, then the lowest index that has it.
+    uint32_t top_key = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const uint64_t v = (uint64_t)key[i] << 32 | (uint32_t) ~(first + 1024 * (i / 4) + 4 * tid + i % 4);
-        best = v > best ? v : best;
-    }
+    for (int i = 0; i < 16; ++i) top_key = max(top_key, key[i]);
+    uint32_t at_top = 15;
+#pragma unroll
+    for (int i = 15; i >= 0; --i)
+        if (key[i] == top_key) at_top = i;
+    uint64_t best = (uint64_t)top_key << 32 | (uint32_t) ~(first + 1024 * (at_top / 4) + 4 * tid + at_top % 4);
     best = wave_largest(best);
     if (lane == 0) wave_best[wave] = best;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 4; ++w) best = wave_best[w] > best ? wave_best[w] : best;
-    const uint32_t top_key = (uint32_t)(best >> 32);
+    top_key = (uint32_t)(best >> 32);
     if (tid == 0) part.best = best;
-    if (is_greedy(p) || top_key <= kKeyMinusInf) {  // (no weight in this part: no token of it is asked for)
-        part.count[tid] = 0;
-        part.mass[tid] = 0;
-        if (tid == 0) {
-            part.kept = 0;
-            part.kept_bins = kBins;
-        }
-        return;
-    }
+    if (is_greedy(p) || top_key <= kKeyMinusInf) return;  // (nothing else of it is read)
     const Weights w(steps_per_logit(p.temperature), top_key);
     uint8_t bin[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const uint32_t b = w.bin(key[i]);
+        double within;
+        const uint32_t b = w.bin(key[i], within);
         bin[i] = (uint8_t)b;
-        if (b == kDead) continue;
-        atomicAdd(&bins[b], 1u);
-        atomicAdd(&masses[b], (unsigned long long)rint(w.weight(key[i]) * kUnit));
+        if (b < kDead) atomicAdd(&sums[b], (unsigned long long)(1ull << kCountShift | units_of(within)));
     }
     __syncthreads();
     // The steps whose tokens fit the short list.
-    uint32_t sum = tid >= (int)kDead ? kShort + 1 : bins[tid];
-    part.count[tid] = (uint16_t)bins[tid];
-    part.mass[tid] = masses[tid];
+    const uint64_t sum = sums[tid];
+    uint32_t upto = (uint32_t)(sum >> kCountShift);
+    const uint32_t own = upto;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(sum, d, 64);
-        if (lane >= d) sum += o;
+        const uint32_t o = __shfl_up(upto, d, 64);
+        if (lane >= d) upto += o;
     }
-    if (lane == 63) wave_sum[wave] = sum;
+    if (lane == 63) wave_sum[wave] = upto;
     __syncthreads();
-    for (int i = 0; i < wave; ++i) sum += wave_sum[i];
-    const uint64_t fits = __ballot(sum <= kShort);
+    for (int i = 0; i < wave; ++i) upto += wave_sum[i];
+    part.sum[tid] = sum;
+    part.upto[tid] = (uint16_t)upto;
+    place[tid] = upto - own;
+    const uint64_t fits = __ballot(upto <= kShort && tid < (int)kDead);
     if (lane == 0 && fits) atomicMax(&kept_bins, 64 * wave + (uint32_t)__popcll(fits));
     __syncthreads();
     const uint32_t below = kept_bins;
 #pragma unroll
     for (int i = 0; i < 16; ++i)
         if (bin[i] < below) {
-            const uint32_t at = atomicAdd(&kept, 1u);
+            const uint32_t at = atomicAdd(&place[bin[i]], 1u);
             part.tokens[at] = (uint64_t)~key[i] << 32 | (first + 1024 * (i / 4) + 4 * tid + i % 4);
         }
-    __syncthreads();
-    if (tid == 0) {
-        part.kept = kept;
-        part.kept_bins = below;
-    }
+    if (tid == 0) part.kept_bins = below;
 }
 
 struct RowShared {
-    double mass[kBins];      // before each step; at the last: all
+    double mass[kBins];      // before each step; at kDead: all
     uint32_t count[kBins];
     uint32_t sums_n[4][kBins];
-    double sums_m[4][kBins];
-    uint64_t list[kList];
+    uint64_t sums_m[4][kBins];
+    uint64_t list[kList], ordered[kList];
     double run[kList];       // running sums of the ordered list
     double wave_m[16];
     uint32_t wave_n[16];
     uint64_t wave_best[16];
-    uint32_t listed, found, found_index;
+    uint32_t listed, raw_parts, found, found_index;
+    uint32_t raw[kThreads];
     double found_mass;
-    uint32_t found_count, counted, tie;
+    uint32_t found_count, counted, tie, edge[2];
     uint32_t digits[256];
     unsigned long long digit_mass[256];
 };
@@ -243,82 +279,133 @@ __device__ __forceinline__ void block_scan(RowShared &sh, uint32_t &n, double &m
 
 struct Row {
     const float *logits;
-    uint32_t count, n_parts;
+    uint32_t count, n_parts, top_key;
     const Part *parts;
     Weights w;
+};
 
-    // Calls f(key, index) for the row's tokens of steps lo .. hi, each once,
-    // a wavefront a part: from the part's short list where that has them, or
-    // from the logits where some lie behind it.
-    template <typename F>
-    __device__ void each(uint32_t lo, uint32_t hi, F f) const {
-        const int lane = threadIdx.x & 63;
-        for (uint32_t i = threadIdx.x >> 6; i < n_parts; i += kThreads / 64) {
-            const Part &part = parts[i];
-            const uint32_t top = (uint32_t)(part.best >> 32);
-            if (top <= kKeyMinusInf) continue;
-            // The part's steps below the row's.
-            const Weights own(w.c, top);
-            const double shift = own.infinite == w.infinite ? (w.infinite ? 0.0 : w.reference - own.reference) : (double)kBins;
-            if (shift > (double)hi) continue;
-            const uint32_t s = (uint32_t)shift, last = hi - s;  // the part's last step asked for
-            bool beyond = false;
-            for (uint32_t b = max(part.kept_bins, lo > s ? lo - s : 0); b <= last; b += 64)
-                beyond |= __ballot(b + lane <= last && b + lane < kDead && part.count[b + lane]) != 0;
-            if (!beyond) {
-                for (uint32_t k = lane; k < part.kept; k += 64) {
-                    const uint64_t t = part.tokens[k];
-                    const uint32_t b = w.bin((uint32_t)(~t >> 32));
-                    if (b >= lo && b <= hi) f((uint32_t)(~t >> 32), (uint32_t)t);
+// The smallest key whose step is at most `bin`, by a whole wavefront: up to
+// the row's largest, whose step is 0, steps never rise with the key, so 64
+// keys at a time bracket it.
+__device__ uint32_t first_key(const Weights &w, uint32_t top_key, uint32_t bin) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint64_t low = 0, high = top_key;  // below low: not; from high on: yes
+    while (high - low > 0) {
+        const uint64_t step = (high - low + 63) / 64;
+        const uint64_t key = low + lane * step;
+        const bool yes = key >= high || w.bin((uint32_t)key) <= bin;
+        const uint64_t all = __ballot(yes);
+        const int at = all ? __builtin_ctzll(all) : 64;
+        const uint64_t found = low + at * step;
+        if (step == 1) return (uint32_t)(found < high ? found : high);
+        high = found < high ? found : high;
+        low = at ? low + (at - 1) * step + 1 : low;
+    }
+    return (uint32_t)low;
+}
+
+// Calls f(key, index) for the row's tokens of steps lo .. hi (below kDead),
+// each once: eight lanes a part on its short list, where that has all of
+// them, and then a wavefront a part on the logits of the others.
+template <typename F>
+__device__ __forceinline__ void each_token(RowShared &sh, const Row &row, uint32_t lo, uint32_t hi, F f) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (uint32_t base = 0; base < row.n_parts; base += kThreads) {
+        const uint32_t held = min((uint32_t)kThreads, row.n_parts - base);
+        __syncthreads();
+        if (tid == 0) sh.raw_parts = 0;
+        __syncthreads();
+        for (uint32_t i = tid / 8; i < held; i += kThreads / 8) {
+            const Part &part = row.parts[base + i];
+            const uint32_t s = row.w.shift((uint32_t)(part.best >> 32));
+            if (s > hi) continue;
+            const uint32_t begin = lo > s ? part.upto[lo - s - 1] : 0, end = part.upto[hi - s];
+            if (begin >= end) continue;
+            if (hi - s < part.kept_bins) {
+                for (uint32_t k = begin + tid % 8; k < end; k += 8) {
+                    const uint64_t token = part.tokens[k];
+                    f((uint32_t)(~token >> 32), (uint32_t)token);
                 }
-                continue;
+            } else if (tid % 8 == 0) {
+                sh.raw[atomicAdd(&sh.raw_parts, 1u)] = base + i;
             }
-            const uint32_t begin = i * kPart, end = min(begin + kPart, count);
-            for (uint32_t k = begin + lane; k < end; k += 64) {
-                const uint32_t key = logit_key(logits[k]);
-                const uint32_t b = w.bin(key);
-                if (b >= lo && b <= hi && b < kDead) f(key, k);
+        }
+        __syncthreads();
+        if (sh.raw_parts == 0) continue;
+        // Steps as ranges of keys: an integer comparison a logit.
+        if (wave < 2) {
+            const uint32_t edge = wave == 0 ? first_key(row.w, row.top_key, hi)
+                                            : lo == 0 ? row.top_key : first_key(row.w, row.top_key, lo - 1) - 1;
+            if (lane == 0) sh.edge[wave] = edge;
+        }
+        __syncthreads();
+        const uint32_t low = sh.edge[0], high = sh.edge[1];
+        for (uint32_t r = wave; r < sh.raw_parts; r += kThreads / 64) {
+            const uint32_t begin = sh.raw[r] * kPart, end = min(begin + kPart, row.count);
+            for (uint32_t k = begin + lane; k < end; k += 256) {
+                float l[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) l[j] = row.logits[min(k + 64 * j, end - 1)];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t key = logit_key(l[j]);
+                    if (k + 64 * j < end && key >= low && key <= high) f(key, k + 64 * j);
+                }
             }
         }
     }
-};
+    __syncthreads();
+}
 
-// Tokens of steps lo .. hi (n of them, at most kList) in order in sh.list,
+// Tokens of steps lo .. hi (n of them, at most kList) in order in sh.ordered,
 // sh.run their running sums on top of `before`.
-__device__ void order_steps(RowShared &sh, const Row &row, uint32_t lo, uint32_t hi, uint32_t n, double before) {
+__device__ __noinline__ void order_steps(RowShared &sh, const Row &row, uint32_t lo, uint32_t hi, uint32_t n, double before) {
     const int tid = threadIdx.x;
     __syncthreads();
     if (tid == 0) sh.listed = 0;
-    __syncthreads();
-    row.each(lo, hi, [&](uint32_t key, uint32_t i) {
+    each_token(sh, row, lo, hi, [&](uint32_t key, uint32_t i) {
         const uint32_t at = atomicAdd(&sh.listed, 1u);
         if (at < kList) sh.list[at] = (uint64_t)~key << 32 | i;
     });
-    uint32_t padded = 64;
-    while (padded < n) padded *= 2;
-    __syncthreads();
-    for (uint32_t i = min(sh.listed, n) + tid; i < padded; i += kThreads) sh.list[i] = ~0ull;
-    for (uint32_t size = 2; size <= padded; size *= 2) {
-        for (uint32_t step = size / 2; step >= 1; step /= 2) {
-            // (Pairs within 64 entries are one wavefront's, from the second
-            // step of them on.)
-            __syncthreads();
-            for (uint32_t k = tid; k < padded / 2; k += kThreads) {
-                const uint32_t i = 2 * k - (k & (step - 1)), j = i + step;
-                const uint64_t x = sh.list[i], y = sh.list[j];
-                if ((x > y) == ((i & size) == 0)) {
-                    sh.list[i] = y;
-                    sh.list[j] = x;
+    if (n <= kRanked) {
+        // A token's place is the number of smaller ones (all differ).
+        if (tid < (int)n) {
+            const uint64_t own = sh.list[tid];
+            uint32_t rank = 0;
+#pragma unroll 4
+            for (uint32_t k = 0; k < n; ++k) rank += sh.list[k] < own;
+            sh.ordered[rank] = own;
+        }
+    } else {
+        uint32_t padded = 2 * kRanked;
+        while (padded < n) padded *= 2;
+        for (uint32_t i = tid; i < padded; i += kThreads) sh.ordered[i] = i < n ? sh.list[i] : ~0ull;
+        for (uint32_t size = 2; size <= padded; size *= 2) {
+            for (uint32_t step = size / 2; step >= 1; step /= 2) {
+                __syncthreads();
+                for (uint32_t k = tid; k < padded / 2; k += kThreads) {
+                    const uint32_t i = 2 * k - (k & (step - 1)), j = i + step;
+                    const uint64_t x = sh.ordered[i], y = sh.ordered[j];
+                    if ((x > y) == ((i & size) == 0)) {
+                        sh.ordered[i] = y;
+                        sh.ordered[j] = x;
+                    }
                 }
             }
         }
     }
     __syncthreads();
+    const uint32_t per = n <= kThreads ? 1 : 4;  // entries a thread
     double w[4], sum = 0.0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const uint32_t i = 4 * tid + k;
-        w[k] = i < n && sh.list[i] != ~0ull ? row.w.weight((uint32_t)(~sh.list[i] >> 32)) : 0.0;
+    for (uint32_t k = 0; k < 4; ++k) {
+        const uint32_t i = per * tid + k;
+        w[k] = 0.0;
+        if (k < per && i < n) {
+            double within;
+            const uint32_t bin = row.w.bin((uint32_t)(~sh.ordered[i] >> 32), within);
+            w[k] = step_weight(bin) * within;
+        }
         sum += w[k];
     }
     uint32_t none = 0;
@@ -326,10 +413,10 @@ __device__ void order_steps(RowShared &sh, const Row &row, uint32_t lo, uint32_t
     block_scan(sh, none, run);
     run = before + (run - sum);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const uint32_t i = 4 * tid + k;
+    for (uint32_t k = 0; k < 4; ++k) {
+        const uint32_t i = per * tid + k;
         run += w[k];
-        if (i < n) sh.run[i] = run;
+        if (k < per && i < n) sh.run[i] = run;
     }
     __syncthreads();
 }
@@ -373,7 +460,7 @@ __device__ uint32_t step_of(RowShared &sh, bool by_mass, double at, bool past) {
 
 // A place in step `bin`: the entry where the count (by_mass: sum) reaches
 // `at` (past: exceeds it). found_index, and count and sum up to it.
-__device__ void place_in(RowShared &sh, const Row &row, uint32_t bin, bool by_mass, double at, bool past) {
+__device__ __noinline__ void place_in(RowShared &sh, const Row &row, uint32_t bin, bool by_mass, double at, bool past) {
     const int tid = threadIdx.x;
     const uint32_t n0 = sh.count[bin], n = sh.count[bin + 1] - n0;
     const double m0 = sh.mass[bin];
@@ -382,7 +469,7 @@ __device__ void place_in(RowShared &sh, const Row &row, uint32_t bin, bool by_ma
         const uint32_t k = by_mass ? reach(sh, n, at, past) : (uint32_t)fmin(fmax(at - n0, 1.0), (double)n) - 1;
         __syncthreads();
         if (tid == 0) {
-            sh.found_index = (uint32_t)sh.list[k];
+            sh.found_index = (uint32_t)sh.ordered[k];
             sh.found_count = n0 + k + 1;
             sh.found_mass = sh.run[k];
         }
@@ -391,26 +478,24 @@ __device__ void place_in(RowShared &sh, const Row &row, uint32_t bin, bool by_ma
     }
     // More tokens than the list holds: the key at the place digit by digit,
     // each pass a histogram of the step's tokens that share the digits so far
-    // (sums in integers again: 4096 and more of them, in multiples of 2^-36).
+    // (sums in units of 2^-36: 2^26 of them fit 64 bits).
     uint32_t prefix = 0;
     double nb = n0, mb = m0;
+    const double unit = step_weight(bin) * 0x1p-36;
     for (int digit = 3; digit >= 0; --digit) {
         __syncthreads();
         if (tid < 256) {
             sh.digits[tid] = 0;
             sh.digit_mass[tid] = 0;
         }
-        __syncthreads();
-        row.each(bin, bin, [&](uint32_t key, uint32_t) {
+        each_token(sh, row, bin, bin, [&](uint32_t key, uint32_t) {
             if (digit < 3 && (key >> (8 * digit + 8)) != prefix) return;
             const uint32_t d = 255u - ((key >> (8 * digit)) & 255u);
+            double within;
+            (void)row.w.bin(key, within);
             atomicAdd(&sh.digits[d], 1u);
-            // (Within a step weights differ by 2^(1/4) at most: against the
-            // step's own, so that small ones keep their bits.)
-            atomicAdd(&sh.digit_mass[d], (unsigned long long)rint(row.w.weight(key) * exp2(0.25 * bin) * 0x1p36));
+            atomicAdd(&sh.digit_mass[d], (unsigned long long)rint(within * 0x1p36));
         });
-        __syncthreads();
-        const double unit = exp2(-0.25 * bin) * 0x1p-36;
         const uint32_t mine = tid < 256 ? sh.digits[tid] : 0;
         const double mass = tid < 256 ? (double)sh.digit_mass[tid] * unit : 0.0;
         uint32_t run_n = mine;
@@ -440,7 +525,9 @@ __device__ void place_in(RowShared &sh, const Row &row, uint32_t bin, bool by_ma
         __syncthreads();
     }
     // Tokens of one logit, in index order, all of one weight: which of them.
-    const double w = row.w.weight(prefix);
+    double w;
+    (void)row.w.bin(prefix, w);
+    w *= step_weight(bin);
     const uint32_t ties = sh.digits[255u - (prefix & 255u)];
     double nth = by_mass ? (past ? floor((at - mb) / w) + 1.0 : ceil((at - mb) / w)) : at - nb;
     nth = fmin(fmax(nth, 1.0), (double)ties);
@@ -486,21 +573,28 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
         if (tid == 0) ids[blockIdx.x] = top_key <= kKeyMinusInf ? 0u : ~(uint32_t)best;
         return;
     }
-    const Row row{logits + (size_t)blockIdx.x * count, count, n_parts, parts, Weights(steps_per_logit(p.temperature), top_key)};
+    const Row row{logits + (size_t)blockIdx.x * count, count, n_parts, top_key, parts,
+                  Weights(steps_per_logit(p.temperature), top_key)};
     // The parts' histograms, each shifted by its own largest step: four
-    // threads a step, every fourth part each.
+    // threads a step, every fourth part each. Parts' sums share the grid of
+    // steps, so they are added as integers.
     {
         const uint32_t b = tid & (kBins - 1), group = tid / kBins;
         uint32_t n = 0;
-        double m = 0.0;
-        for (uint32_t i = group; i < n_parts; i += kThreads / kBins) {
-            const uint32_t top = (uint32_t)(parts[i].best >> 32);
-            const Weights own(row.w.c, top);
-            const double shift = own.infinite == row.w.infinite ? (own.infinite ? 0.0 : row.w.reference - own.reference) : (double)kBins;
-            if (top <= kKeyMinusInf || shift > (double)b || b >= kDead) continue;
-            const uint32_t at = b - (uint32_t)shift;
-            n += parts[i].count[at];
-            m += (double)parts[i].mass[at] * exp2(-0.25 * shift);
+        uint64_t m = 0;
+        for (uint32_t base = 0; base < n_parts; base += kThreads) {
+            __syncthreads();
+            if (base + tid < n_parts) sh.raw[tid] = row.w.shift((uint32_t)(parts[base + tid].best >> 32));
+            __syncthreads();
+            const uint32_t held = min((uint32_t)kThreads, n_parts - base);
+#pragma unroll 4
+            for (uint32_t i = group; i < held; i += kThreads / kBins) {
+                const uint32_t s = sh.raw[i];
+                if (s > b || b >= kDead) continue;
+                const uint64_t sum = parts[base + i].sum[b - s];
+                n += (uint32_t)(sum >> kCountShift);
+                m += sum & ((1ull << kCountShift) - 1);
+            }
         }
         sh.sums_n[group][b] = n;
         sh.sums_m[group][b] = m;
@@ -508,8 +602,9 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
         uint32_t run_n = 0;
         double run_m = 0.0;
         if (group == 0) {
-            run_n = n = (sh.sums_n[0][b] + sh.sums_n[1][b]) + (sh.sums_n[2][b] + sh.sums_n[3][b]);
-            run_m = m = ((sh.sums_m[0][b] + sh.sums_m[1][b]) + (sh.sums_m[2][b] + sh.sums_m[3][b])) * (1.0 / kUnit);
+            run_n = (sh.sums_n[0][b] + sh.sums_n[1][b]) + (sh.sums_n[2][b] + sh.sums_n[3][b]);
+            m = (sh.sums_m[0][b] + sh.sums_m[1][b]) + (sh.sums_m[2][b] + sh.sums_m[3][b]);
+            run_m = (double)m * (step_weight(b) / (double)(1ull << kUnitBits));
         }
         block_scan(sh, run_n, run_m);
         if (group == 0) {
@@ -554,7 +649,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
             if (tid == 0) sh.counted = 0;
             __syncthreads();
             uint32_t mine = 0;
-            for (uint32_t i = tid; i < tokens; i += kThreads) mine += enough((uint32_t)(~sh.list[i] >> 32));
+            for (uint32_t i = tid; i < tokens; i += kThreads) mine += enough((uint32_t)(~sh.ordered[i] >> 32));
             if (mine) atomicAdd(&sh.counted, mine);
             __syncthreads();
             tokens = max(sh.counted, 1u);
@@ -562,7 +657,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
         const double kept = sh.run[tokens - 1];
         const uint32_t k = draw >= 1.0 ? tokens - 1 : reach(sh, tokens, draw * kept, true);
         __syncthreads();
-        if (tid == 0) ids[blockIdx.x] = (uint32_t)sh.list[min(k, tokens - 1)];
+        if (tid == 0) ids[blockIdx.x] = (uint32_t)sh.ordered[min(k, tokens - 1)];
         return;
     }
     // Otherwise each place by itself.
@@ -587,10 +682,9 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
         __syncthreads();
         if (tid == 0) sh.counted = 0;
         __syncthreads();
-        row.each(lo, hi, [&](uint32_t key, uint32_t) {
+        each_token(sh, row, lo, hi, [&](uint32_t key, uint32_t) {
             if (enough(key)) atomicAdd(&sh.counted, 1u);
         });
-        __syncthreads();
         const uint32_t reaching = max(sh.count[lo] + sh.counted, 1u);
         if (reaching < tokens) {
             tokens = reaching;
