@@ -34,8 +34,8 @@ constexpr uint32_t kPart = 4096;       // logits of a first-pass workgroup
 constexpr uint32_t kBins = 256;
 constexpr uint32_t kDead = kBins - 1;  // the step of tokens that are not drawn, 63 octaves and more below the largest
 constexpr uint32_t kShort = 256;       // tokens kept beside a part's histogram
-constexpr uint32_t kList = 4096;       // tokens that the second pass puts in order
-constexpr uint32_t kRanked = 1024;     // (up to these by counting smaller ones)
+constexpr uint32_t kList = 12288;      // tokens that the second pass takes into LDS
+constexpr uint32_t kOrder = 256;       // and of these, puts in order
 constexpr int kThreads = 1024;
 constexpr int kUnitBits = 37;          // of a weight of 1 in a step's sum
 constexpr int kCountShift = 50;        // 4096 * 2^(1/4) * 2^37 < 2^50: the count stands above the sum
@@ -234,19 +234,18 @@ __global__ __launch_bounds__(256) void sample_parts_kernel(const float *logits, 
 struct RowShared {
     double mass[kBins];      // before each step; at kDead: all
     uint32_t count[kBins];
-    uint32_t sums_n[4][kBins];
-    uint64_t sums_m[4][kBins];
-    uint64_t list[kList], ordered[kList];
-    double run[kList];       // running sums of the ordered list
+    uint64_t list[kList];
+    uint64_t picked[kOrder], ordered[kOrder];
+    double run[kOrder];      // running sums of the ordered tokens
+    uint32_t split_n[kThreads];            // (of histograms: counts,
+    unsigned long long split_m[kThreads];  // and sums)
+    uint32_t raw[kThreads];
     double wave_m[16];
     uint32_t wave_n[16];
     uint64_t wave_best[16];
-    uint32_t listed, raw_parts, found, found_index;
-    uint32_t raw[kThreads];
+    uint32_t listed, raw_parts, found, found_index, edge[2];
+    uint32_t found_count, counted, tie;
     double found_mass;
-    uint32_t found_count, counted, tie, edge[2];
-    uint32_t digits[256];
-    unsigned long long digit_mass[256];
 };
 
 // Inclusive sums over the workgroup, in thread order.
@@ -304,12 +303,29 @@ __device__ uint32_t first_key(const Weights &w, uint32_t top_key, uint32_t bin) 
     return (uint32_t)low;
 }
 
-// Calls f(key, index) for the row's tokens of steps lo .. hi (below kDead),
-// each once: eight lanes a part on its short list, where that has all of
-// them, and then a wavefront a part on the logits of the others.
+// The keys of steps lo .. hi: between edge[0] and edge[1], both included.
+__device__ __forceinline__ void find_edges(RowShared &sh, const Row &row, uint32_t lo, uint32_t hi) {
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+    if (wave < 2) {
+        const uint32_t edge = wave == 0  ? first_key(row.w, row.top_key, hi)
+                              : lo == 0 ? row.top_key
+                                        : first_key(row.w, row.top_key, lo - 1) - 1;
+        if ((threadIdx.x & 63) == 0) sh.edge[wave] = edge;
+    }
+    __syncthreads();
+}
+
+// Calls f(key, index) for the row's tokens of steps lo .. hi (below kDead)
+// with keys from low to high, each once: eight lanes a part on its short
+// list, where that has all of them, then a wavefront on each half of the
+// others' logits.
 template <typename F>
-__device__ __forceinline__ void each_token(RowShared &sh, const Row &row, uint32_t lo, uint32_t hi, F f) {
+__device__ __forceinline__ void each_token(RowShared &sh, const Row &row, uint32_t lo, uint32_t hi, uint32_t low, uint32_t high,
+                                           F f) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr uint32_t kHalf = kPart / 2;
+    const bool aligned = (reinterpret_cast<uintptr_t>(row.logits) & 15u) == 0;
     for (uint32_t base = 0; base < row.n_parts; base += kThreads) {
         const uint32_t held = min((uint32_t)kThreads, row.n_parts - base);
         __syncthreads();
@@ -324,32 +340,43 @@ __device__ __forceinline__ void each_token(RowShared &sh, const Row &row, uint32
             if (hi - s < part.kept_bins) {
                 for (uint32_t k = begin + tid % 8; k < end; k += 8) {
                     const uint64_t token = part.tokens[k];
-                    f((uint32_t)(~token >> 32), (uint32_t)token);
+                    const uint32_t key = (uint32_t)(~token >> 32);
+                    if (key >= low && key <= high) f(key, (uint32_t)token);
                 }
             } else if (tid % 8 == 0) {
                 sh.raw[atomicAdd(&sh.raw_parts, 1u)] = base + i;
             }
         }
         __syncthreads();
-        if (sh.raw_parts == 0) continue;
-        // Steps as ranges of keys: an integer comparison a logit.
-        if (wave < 2) {
-            const uint32_t edge = wave == 0 ? first_key(row.w, row.top_key, hi)
-                                            : lo == 0 ? row.top_key : first_key(row.w, row.top_key, lo - 1) - 1;
-            if (lane == 0) sh.edge[wave] = edge;
-        }
-        __syncthreads();
-        const uint32_t low = sh.edge[0], high = sh.edge[1];
-        for (uint32_t r = wave; r < sh.raw_parts; r += kThreads / 64) {
-            const uint32_t begin = sh.raw[r] * kPart, end = min(begin + kPart, row.count);
-            for (uint32_t k = begin + lane; k < end; k += 256) {
-                float l[4];
+        const uint32_t halves = 2 * sh.raw_parts;
+        for (uint32_t r = wave; r < halves; r += kThreads / 64) {
+            const uint32_t begin = sh.raw[r / 2] * kPart + r % 2 * kHalf;
+            if (begin >= row.count) continue;
+            const uint32_t n = min(kHalf, row.count - begin);
+            const float *from = row.logits + begin;
+            if (aligned && n == kHalf) {
+                float4 l[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) l[j] = row.logits[min(k + 64 * j, end - 1)];
+                for (int j = 0; j < 8; ++j) l[j] = *reinterpret_cast<const float4 *>(from + 256 * j + 4 * lane);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t key = logit_key(l[j]);
-                    if (k + 64 * j < end && key >= low && key <= high) f(key, k + 64 * j);
+                for (int j = 0; j < 8; ++j) {
+                    const float four[4] = {l[j].x, l[j].y, l[j].z, l[j].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t key = logit_key(four[i]);
+                        if (key >= low && key <= high) f(key, begin + 256 * j + 4 * lane + i);
+                    }
+                }
+            } else {
+                for (uint32_t k = lane; k < n; k += 256) {
+                    float l[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) l[j] = from[min(k + 64 * j, n - 1)];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t key = logit_key(l[j]);
+                        if (k + 64 * j < n && key >= low && key <= high) f(key, begin + k + 64 * j);
+                    }
                 }
             }
         }
@@ -357,67 +384,51 @@ __device__ __forceinline__ void each_token(RowShared &sh, const Row &row, uint32
     __syncthreads();
 }
 
-// Tokens of steps lo .. hi (n of them, at most kList) in order in sh.ordered,
-// sh.run their running sums on top of `before`.
-__device__ __noinline__ void order_steps(RowShared &sh, const Row &row, uint32_t lo, uint32_t hi, uint32_t n, double before) {
-    const int tid = threadIdx.x;
+// Takes the tokens of steps lo .. hi with keys from low to high into the list.
+__device__ __noinline__ void collect(RowShared &sh, const Row &row, uint32_t lo, uint32_t hi, uint32_t low, uint32_t high) {
     __syncthreads();
-    if (tid == 0) sh.listed = 0;
-    each_token(sh, row, lo, hi, [&](uint32_t key, uint32_t i) {
+    if (threadIdx.x == 0) sh.listed = 0;
+    each_token(sh, row, lo, hi, low, high, [&](uint32_t key, uint32_t i) {
         const uint32_t at = atomicAdd(&sh.listed, 1u);
         if (at < kList) sh.list[at] = (uint64_t)~key << 32 | i;
     });
-    if (n <= kRanked) {
-        // A token's place is the number of smaller ones (all differ).
-        if (tid < (int)n) {
-            const uint64_t own = sh.list[tid];
-            uint32_t rank = 0;
-#pragma unroll 4
-            for (uint32_t k = 0; k < n; ++k) rank += sh.list[k] < own;
-            sh.ordered[rank] = own;
-        }
-    } else {
-        uint32_t padded = 2 * kRanked;
-        while (padded < n) padded *= 2;
-        for (uint32_t i = tid; i < padded; i += kThreads) sh.ordered[i] = i < n ? sh.list[i] : ~0ull;
-        for (uint32_t size = 2; size <= padded; size *= 2) {
-            for (uint32_t step = size / 2; step >= 1; step /= 2) {
-                __syncthreads();
-                for (uint32_t k = tid; k < padded / 2; k += kThreads) {
-                    const uint32_t i = 2 * k - (k & (step - 1)), j = i + step;
-                    const uint64_t x = sh.ordered[i], y = sh.ordered[j];
-                    if ((x > y) == ((i & size) == 0)) {
-                        sh.ordered[i] = y;
-                        sh.ordered[j] = x;
-                    }
-                }
-            }
+}
+
+// The list's n tokens (at most kOrder) with keys from low to high in order in
+// sh.ordered, sh.run their running sums on top of `before`.
+__device__ __noinline__ void order_listed(RowShared &sh, const Row &row, uint32_t low, uint32_t high, uint32_t n, double before) {
+    const uint32_t tid = threadIdx.x;
+    __syncthreads();
+    if (tid == 0) sh.counted = 0;
+    if (tid < kOrder) sh.picked[tid] = ~0ull;
+    __syncthreads();
+    const uint32_t all = min(sh.listed, kList);
+    for (uint32_t i = tid; i < all; i += kThreads) {
+        const uint64_t token = sh.list[i];
+        const uint32_t key = (uint32_t)(~token >> 32);
+        if (key >= low && key <= high) {
+            const uint32_t at = atomicAdd(&sh.counted, 1u);
+            if (at < kOrder) sh.picked[at] = token;
         }
     }
     __syncthreads();
-    const uint32_t per = n <= kThreads ? 1 : 4;  // entries a thread
-    double w[4], sum = 0.0;
-#pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) {
-        const uint32_t i = per * tid + k;
-        w[k] = 0.0;
-        if (k < per && i < n) {
-            double within;
-            const uint32_t bin = row.w.bin((uint32_t)(~sh.ordered[i] >> 32), within);
-            w[k] = step_weight(bin) * within;
-        }
-        sum += w[k];
+    // A token's place is the number of smaller ones (all differ).
+    if (tid < n) {
+        const uint64_t own = sh.picked[tid];
+        uint32_t rank = 0;
+#pragma unroll 8
+        for (uint32_t k = 0; k < n; ++k) rank += sh.picked[k] < own;
+        sh.ordered[rank] = own;
+    }
+    __syncthreads();
+    double run = 0.0, within;
+    if (tid < n) {
+        const uint32_t bin = row.w.bin((uint32_t)(~sh.ordered[tid] >> 32), within);
+        run = step_weight(bin) * within;
     }
     uint32_t none = 0;
-    double run = sum;
     block_scan(sh, none, run);
-    run = before + (run - sum);
-#pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) {
-        const uint32_t i = per * tid + k;
-        run += w[k];
-        if (k < per && i < n) sh.run[i] = run;
-    }
+    if (tid < n) sh.run[tid] = before + run;
     __syncthreads();
 }
 
@@ -459,96 +470,113 @@ __device__ uint32_t step_of(RowShared &sh, bool by_mass, double at, bool past) {
 }
 
 // A place in step `bin`: the entry where the count (by_mass: sum) reaches
-// `at` (past: exceeds it). found_index, and count and sum up to it.
-__device__ __noinline__ void place_in(RowShared &sh, const Row &row, uint32_t bin, bool by_mass, double at, bool past) {
-    const int tid = threadIdx.x;
-    const uint32_t n0 = sh.count[bin], n = sh.count[bin + 1] - n0;
-    const double m0 = sh.mass[bin];
-    if (n <= kList) {
-        order_steps(sh, row, bin, bin, n, m0);
-        const uint32_t k = by_mass ? reach(sh, n, at, past) : (uint32_t)fmin(fmax(at - n0, 1.0), (double)n) - 1;
+// `at` (past: exceeds it). found_index, and count and sum up to it. `listed`:
+// the list has the step's tokens (and perhaps others).
+__device__ __noinline__ void place_in(RowShared &sh, const Row &row, uint32_t bin, bool by_mass, double at, bool past,
+                                      bool listed) {
+    const uint32_t tid = threadIdx.x;
+    uint32_t nb = sh.count[bin], n = sh.count[bin + 1] - nb;
+    double mb = sh.mass[bin];
+    find_edges(sh, row, bin, bin);
+    uint32_t low = sh.edge[0], high = sh.edge[1];
+    // The range of keys split into up to 1024 equal ones, and the one that
+    // has the place again, until it has few tokens or one key. (Sums in units
+    // of 2^-36: 2^26 weights fit 64 bits.)
+    const double unit = step_weight(bin) * 0x1p-36;
+    while (true) {
+        if (!listed && n <= kList) {
+            collect(sh, row, bin, bin, low, high);
+            listed = true;
+        }
+        if (n <= kOrder || low >= high) break;
+        const uint32_t width = 32 - __builtin_clz(high - low), shift = width > 10 ? width - 10 : 0;
+        __syncthreads();
+        sh.split_n[tid] = 0;
+        sh.split_m[tid] = 0;
+        __syncthreads();
+        const auto add = [&](uint32_t key, uint32_t) {
+            const uint32_t d = (high - key) >> shift;
+            double within;
+            (void)row.w.bin(key, within);
+            atomicAdd(&sh.split_n[d], 1u);
+            atomicAdd(&sh.split_m[d], (unsigned long long)rint(within * 0x1p36));
+        };
+        if (listed) {
+            const uint32_t all = min(sh.listed, kList);
+            for (uint32_t i = tid; i < all; i += kThreads) {
+                const uint64_t token = sh.list[i];
+                const uint32_t key = (uint32_t)(~token >> 32);
+                if (key >= low && key <= high) add(key, (uint32_t)token);
+            }
+            __syncthreads();
+        } else {
+            each_token(sh, row, bin, bin, low, high, add);
+        }
+        const uint32_t mine = sh.split_n[tid];
+        const double mass = (double)sh.split_m[tid] * unit;
+        uint32_t run_n = mine;
+        double run_m = mass;
+        block_scan(sh, run_n, run_m);
+        if (tid == 0) sh.found = kThreads;
+        __syncthreads();
+        const double v = by_mass ? mb + run_m : (double)nb + run_n;
+        if (mine && (past ? v > at : v >= at)) atomicMin(&sh.found, tid);
+        __syncthreads();
+        if (sh.found == kThreads) {  // (uniform; the sums' last bits)
+            __syncthreads();
+            if (tid == 0) sh.found = 0;
+            __syncthreads();
+            if (mine) atomicMax(&sh.found, tid);
+            __syncthreads();
+        }
+        const uint32_t d = sh.found;
+        if (tid == d) {
+            sh.found_count = run_n - mine;
+            sh.found_mass = run_m - mass;
+        }
+        __syncthreads();
+        high -= d << shift;
+        low = max(low, high - min(high, (1u << shift) - 1));
+        n = sh.split_n[d];
+        nb += sh.found_count;
+        mb += sh.found_mass;
+    }
+    if (n <= kOrder) {
+        order_listed(sh, row, low, high, n, mb);
+        const uint32_t k = by_mass ? reach(sh, n, at, past) : (uint32_t)fmin(fmax(at - nb, 1.0), (double)n) - 1;
         __syncthreads();
         if (tid == 0) {
             sh.found_index = (uint32_t)sh.ordered[k];
-            sh.found_count = n0 + k + 1;
+            sh.found_count = nb + k + 1;
             sh.found_mass = sh.run[k];
         }
         __syncthreads();
         return;
     }
-    // More tokens than the list holds: the key at the place digit by digit,
-    // each pass a histogram of the step's tokens that share the digits so far
-    // (sums in units of 2^-36: 2^26 of them fit 64 bits).
-    uint32_t prefix = 0;
-    double nb = n0, mb = m0;
-    const double unit = step_weight(bin) * 0x1p-36;
-    for (int digit = 3; digit >= 0; --digit) {
-        __syncthreads();
-        if (tid < 256) {
-            sh.digits[tid] = 0;
-            sh.digit_mass[tid] = 0;
-        }
-        each_token(sh, row, bin, bin, [&](uint32_t key, uint32_t) {
-            if (digit < 3 && (key >> (8 * digit + 8)) != prefix) return;
-            const uint32_t d = 255u - ((key >> (8 * digit)) & 255u);
-            double within;
-            (void)row.w.bin(key, within);
-            atomicAdd(&sh.digits[d], 1u);
-            atomicAdd(&sh.digit_mass[d], (unsigned long long)rint(within * 0x1p36));
-        });
-        const uint32_t mine = tid < 256 ? sh.digits[tid] : 0;
-        const double mass = tid < 256 ? (double)sh.digit_mass[tid] * unit : 0.0;
-        uint32_t run_n = mine;
-        double run_m = mass;
-        block_scan(sh, run_n, run_m);
-        if (tid == 0) sh.found = 256;
-        __syncthreads();
-        const double v = by_mass ? mb + run_m : nb + run_n;
-        if (mine && (past ? v > at : v >= at)) atomicMin(&sh.found, (uint32_t)tid);
-        __syncthreads();
-        if (sh.found == 256) {
-            __syncthreads();
-            if (tid == 0) sh.found = 0;
-            __syncthreads();
-            if (mine) atomicMax(&sh.found, (uint32_t)tid);
-            __syncthreads();
-        }
-        const uint32_t d = sh.found;
-        if (tid == (int)d) {
-            sh.found_count = run_n - mine;
-            sh.found_mass = run_m - mass;
-        }
-        __syncthreads();
-        prefix = prefix << 8 | (255u - d);
-        nb += sh.found_count;
-        mb += sh.found_mass;
-        __syncthreads();
-    }
     // Tokens of one logit, in index order, all of one weight: which of them.
     double w;
-    (void)row.w.bin(prefix, w);
+    (void)row.w.bin(low, w);
     w *= step_weight(bin);
-    const uint32_t ties = sh.digits[255u - (prefix & 255u)];
     double nth = by_mass ? (past ? floor((at - mb) / w) + 1.0 : ceil((at - mb) / w)) : at - nb;
-    nth = fmin(fmax(nth, 1.0), (double)ties);
-    const uint32_t low = (uint32_t)nth;
+    nth = fmin(fmax(nth, 1.0), (double)n);
+    const uint32_t which = (uint32_t)nth;
     uint32_t seen = 0;  // of them before this stretch
     for (uint32_t base = 0; base < row.count; base += kThreads) {
         const uint32_t i = base + tid;
-        uint32_t run = i < row.count && logit_key(row.logits[i]) == prefix ? 1u : 0u;
+        uint32_t run = i < row.count && logit_key(row.logits[i]) == low ? 1u : 0u;
         const uint32_t own = run;
         double none = 0.0;
         block_scan(sh, run, none);
-        if (own && seen + run == low) sh.found_index = i;
-        if (tid == kThreads - 1) sh.tie = run;
+        if (own && seen + run == which) sh.found_index = i;
+        if (tid == kThreads - 1u) sh.tie = run;
         __syncthreads();
         seen += sh.tie;
         __syncthreads();
-        if (seen >= low) break;
+        if (seen >= which) break;
     }
     if (tid == 0) {
-        sh.found_count = (uint32_t)(nb + low);
-        sh.found_mass = mb + low * w;
+        sh.found_count = (uint32_t)(nb + which);
+        sh.found_mass = mb + which * w;
     }
     __syncthreads();
 }
@@ -596,14 +624,17 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
                 m += sum & ((1ull << kCountShift) - 1);
             }
         }
-        sh.sums_n[group][b] = n;
-        sh.sums_m[group][b] = m;
+        sh.split_n[tid] = n;
+        sh.split_m[tid] = m;
         __syncthreads();
         uint32_t run_n = 0;
         double run_m = 0.0;
         if (group == 0) {
-            run_n = (sh.sums_n[0][b] + sh.sums_n[1][b]) + (sh.sums_n[2][b] + sh.sums_n[3][b]);
-            m = (sh.sums_m[0][b] + sh.sums_m[1][b]) + (sh.sums_m[2][b] + sh.sums_m[3][b]);
+            for (uint32_t g = 1; g < kThreads / kBins; ++g) {
+                n += sh.split_n[g * kBins + b];
+                m += sh.split_m[g * kBins + b];
+            }
+            run_n = n;
             run_m = (double)m * (step_weight(b) / (double)(1ull << kUnitBits));
         }
         block_scan(sh, run_n, run_m);
@@ -634,11 +665,16 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
     if (by_k) last = min(last, step_of(sh, false, (double)p.top_k, false));
     else if (by_p) last = min(last, step_of(sh, true, (double)p.top_p * sh.mass[kDead], false));
     else if (least > 0.0 && !row.w.infinite) last = min(last, (uint32_t)fmin(row.w.reference - floor(top * row.w.c + 4.0 * log2(least)) + 1.0, (double)(kDead - 1)));
+    // All that may be kept, if it fits the list.
     const uint32_t n = sh.count[last + 1];
-    if ((by_k || by_p || least > 0.0) && n <= kList) {
-        // All that may be kept fits the list: the rules one after another on
-        // its running sums.
-        order_steps(sh, row, 0, last, n, 0.0);
+    const bool listed = (by_k || by_p || least > 0.0) && n <= kList;
+    if (listed) {
+        find_edges(sh, row, 0, last);
+        collect(sh, row, 0, last, sh.edge[0], sh.edge[1]);
+    }
+    if (listed && n <= kOrder) {
+        // The rules one after another on its running sums.
+        order_listed(sh, row, 0, row.top_key, n, 0.0);
         uint32_t tokens = by_k ? min(p.top_k, n) : n;
         if (by_p) {
             const double whole = by_k ? sh.run[tokens - 1] : sh.mass[kDead];
@@ -664,13 +700,13 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
     double kept = sh.mass[kDead];
     uint32_t tokens = live;
     if (by_k) {
-        place_in(sh, row, step_of(sh, false, (double)p.top_k, false), false, (double)p.top_k, false);
+        place_in(sh, row, step_of(sh, false, (double)p.top_k, false), false, (double)p.top_k, false, listed);
         tokens = sh.found_count;
         kept = sh.found_mass;
     }
     if (by_p) {
         const double at = (double)p.top_p * kept;
-        place_in(sh, row, step_of(sh, true, at, false), true, at, false);
+        place_in(sh, row, step_of(sh, true, at, false), true, at, false, listed);
         tokens = sh.found_count;
         kept = sh.found_mass;
     }
@@ -682,18 +718,19 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
         __syncthreads();
         if (tid == 0) sh.counted = 0;
         __syncthreads();
-        each_token(sh, row, lo, hi, [&](uint32_t key, uint32_t) {
+        find_edges(sh, row, lo, hi);
+        each_token(sh, row, lo, hi, sh.edge[0], sh.edge[1], [&](uint32_t key, uint32_t) {
             if (enough(key)) atomicAdd(&sh.counted, 1u);
         });
         const uint32_t reaching = max(sh.count[lo] + sh.counted, 1u);
         if (reaching < tokens) {
             tokens = reaching;
-            place_in(sh, row, step_of(sh, false, (double)tokens, false), false, (double)tokens, false);
+            place_in(sh, row, step_of(sh, false, (double)tokens, false), false, (double)tokens, false, listed);
             kept = sh.found_mass;
         }
     }
-    if (draw >= 1.0) place_in(sh, row, step_of(sh, false, (double)tokens, false), false, (double)tokens, false);
-    else place_in(sh, row, step_of(sh, true, draw * kept, true), true, draw * kept, true);
+    if (draw >= 1.0) place_in(sh, row, step_of(sh, false, (double)tokens, false), false, (double)tokens, false, listed);
+    else place_in(sh, row, step_of(sh, true, draw * kept, true), true, draw * kept, true, listed);
     if (tid == 0) ids[blockIdx.x] = sh.found_index;
 }
 
