@@ -240,10 +240,11 @@ struct RowShared {
     uint32_t split_n[kThreads];            // (of histograms: counts,
     unsigned long long split_m[kThreads];  // and sums)
     uint32_t raw[kThreads];
+    uint16_t shift[kThreads], kept[kThreads];  // of the first parts
     double wave_m[16];
     uint32_t wave_n[16];
     uint64_t wave_best[16];
-    uint32_t listed, raw_parts, found, found_index, edge[2];
+    uint32_t listed, raw_parts, found, found_index, edge[2], last_live;
     uint32_t found_count, counted, tie;
     double found_mass;
 };
@@ -268,9 +269,12 @@ __device__ __forceinline__ void block_scan(RowShared &sh, uint32_t &n, double &m
     __syncthreads();
     uint32_t n0 = 0;
     double m0 = 0.0;
-    for (int w = 0; w < wave; ++w) {
-        n0 += sh.wave_n[w];
-        m0 += sh.wave_m[w];
+#pragma unroll
+    for (int w = 0; w < kThreads / 64 - 1; ++w) {
+        const uint32_t n2 = sh.wave_n[w];
+        const double m2 = sh.wave_m[w];
+        n0 += w < wave ? n2 : 0;
+        m0 += w < wave ? m2 : 0.0;
     }
     n += n0;
     m += m0;
@@ -317,12 +321,13 @@ __device__ __forceinline__ void find_edges(RowShared &sh, const Row &row, uint32
 }
 
 // Calls f(key, index) for the row's tokens of steps lo .. hi (below kDead)
-// with keys from low to high, each once: eight lanes a part on its short
+// with keys from low to high, each once (`whole`: whole steps; the keys are
+// then found here where they are needed): eight lanes a part on its short
 // list, where that has all of them, then a wavefront on each half of the
 // others' logits.
 template <typename F>
-__device__ __forceinline__ void each_token(RowShared &sh, const Row &row, uint32_t lo, uint32_t hi, uint32_t low, uint32_t high,
-                                           F f) {
+__device__ __forceinline__ void each_token(RowShared &sh, const Row &row, uint32_t lo, uint32_t hi, bool whole, uint32_t low,
+                                           uint32_t high, F f) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     constexpr uint32_t kHalf = kPart / 2;
     const bool aligned = (reinterpret_cast<uintptr_t>(row.logits) & 15u) == 0;
@@ -333,15 +338,16 @@ __device__ __forceinline__ void each_token(RowShared &sh, const Row &row, uint32
         __syncthreads();
         for (uint32_t i = tid / 8; i < held; i += kThreads / 8) {
             const Part &part = row.parts[base + i];
-            const uint32_t s = row.w.shift((uint32_t)(part.best >> 32));
+            const uint32_t s = base ? row.w.shift((uint32_t)(part.best >> 32)) : sh.shift[i];
             if (s > hi) continue;
+            const uint32_t kept = base ? part.kept_bins : sh.kept[i];
             const uint32_t begin = lo > s ? part.upto[lo - s - 1] : 0, end = part.upto[hi - s];
             if (begin >= end) continue;
-            if (hi - s < part.kept_bins) {
+            if (hi - s < kept) {
                 for (uint32_t k = begin + tid % 8; k < end; k += 8) {
                     const uint64_t token = part.tokens[k];
                     const uint32_t key = (uint32_t)(~token >> 32);
-                    if (key >= low && key <= high) f(key, (uint32_t)token);
+                    if (whole || (key >= low && key <= high)) f(key, (uint32_t)token);
                 }
             } else if (tid % 8 == 0) {
                 sh.raw[atomicAdd(&sh.raw_parts, 1u)] = base + i;
@@ -349,6 +355,12 @@ __device__ __forceinline__ void each_token(RowShared &sh, const Row &row, uint32
         }
         __syncthreads();
         const uint32_t halves = 2 * sh.raw_parts;
+        if (whole && halves) {
+            find_edges(sh, row, lo, hi);
+            whole = false;
+            low = sh.edge[0];
+            high = sh.edge[1];
+        }
         for (uint32_t r = wave; r < halves; r += kThreads / 64) {
             const uint32_t begin = sh.raw[r / 2] * kPart + r % 2 * kHalf;
             if (begin >= row.count) continue;
@@ -384,11 +396,13 @@ __device__ __forceinline__ void each_token(RowShared &sh, const Row &row, uint32
     __syncthreads();
 }
 
-// Takes the tokens of steps lo .. hi with keys from low to high into the list.
-__device__ __noinline__ void collect(RowShared &sh, const Row &row, uint32_t lo, uint32_t hi, uint32_t low, uint32_t high) {
+// Takes the tokens of steps lo .. hi (not `whole`: of them, with keys from low
+// to high) into the list.
+__device__ __noinline__ void collect(RowShared &sh, const Row &row, uint32_t lo, uint32_t hi, bool whole, uint32_t low,
+                                     uint32_t high) {
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = 0;
-    each_token(sh, row, lo, hi, low, high, [&](uint32_t key, uint32_t i) {
+    each_token(sh, row, lo, hi, whole, low, high, [&](uint32_t key, uint32_t i) {
         const uint32_t at = atomicAdd(&sh.listed, 1u);
         if (at < kList) sh.list[at] = (uint64_t)~key << 32 | i;
     });
@@ -399,25 +413,28 @@ __device__ __noinline__ void collect(RowShared &sh, const Row &row, uint32_t lo,
 __device__ __noinline__ void order_listed(RowShared &sh, const Row &row, uint32_t low, uint32_t high, uint32_t n, double before) {
     const uint32_t tid = threadIdx.x;
     __syncthreads();
-    if (tid == 0) sh.counted = 0;
-    if (tid < kOrder) sh.picked[tid] = ~0ull;
-    __syncthreads();
     const uint32_t all = min(sh.listed, kList);
-    for (uint32_t i = tid; i < all; i += kThreads) {
-        const uint64_t token = sh.list[i];
-        const uint32_t key = (uint32_t)(~token >> 32);
-        if (key >= low && key <= high) {
-            const uint32_t at = atomicAdd(&sh.counted, 1u);
-            if (at < kOrder) sh.picked[at] = token;
+    const uint64_t *tokens = sh.list;
+    if (all > n) {
+        tokens = sh.picked;
+        if (tid == 0) sh.counted = 0;
+        __syncthreads();
+        for (uint32_t i = tid; i < all; i += kThreads) {
+            const uint64_t token = sh.list[i];
+            const uint32_t key = (uint32_t)(~token >> 32);
+            if (key >= low && key <= high) {
+                const uint32_t at = atomicAdd(&sh.counted, 1u);
+                if (at < kOrder) sh.picked[at] = token;
+            }
         }
+        __syncthreads();
     }
-    __syncthreads();
     // A token's place is the number of smaller ones (all differ).
     if (tid < n) {
-        const uint64_t own = sh.picked[tid];
+        const uint64_t own = tokens[tid];
         uint32_t rank = 0;
 #pragma unroll 8
-        for (uint32_t k = 0; k < n; ++k) rank += sh.picked[k] < own;
+        for (uint32_t k = 0; k < n; ++k) rank += tokens[k] < own;
         sh.ordered[rank] = own;
     }
     __syncthreads();
@@ -450,22 +467,18 @@ __device__ uint32_t reach(RowShared &sh, uint32_t n, double at, bool past) {
 // The step in which the count (`by_mass`: the sum) reaches `at` (past:
 // exceeds it): the last step with tokens if none does.
 __device__ uint32_t step_of(RowShared &sh, bool by_mass, double at, bool past) {
+    // (The sums never fall, and step 0 has the largest: where they pass `at`
+    // is a step with tokens. That none does is left to the sums' last bits.)
+    const auto passes = [&](uint32_t b) {
+        const double v = by_mass ? sh.mass[b + 1] : (double)sh.count[b + 1];
+        return past ? v > at : v >= at;
+    };
     __syncthreads();
-    if (threadIdx.x == 0) sh.found = kBins;
+    if (threadIdx.x == 0) sh.found = sh.last_live;
     __syncthreads();
     const uint32_t b = threadIdx.x;
-    if (b < kDead && sh.count[b + 1] > sh.count[b]) {
-        const double v = by_mass ? sh.mass[b + 1] : (double)sh.count[b + 1];
-        if (past ? v > at : v >= at) atomicMin(&sh.found, b);
-    }
+    if (b < kDead && passes(b) && (b == 0 || !passes(b - 1))) sh.found = b;
     __syncthreads();
-    if (sh.found == kBins) {  // (uniform; the sums' last bits)
-        __syncthreads();
-        if (threadIdx.x == 0) sh.found = 0;
-        __syncthreads();
-        if (b < kDead && sh.count[b + 1] > sh.count[b]) atomicMax(&sh.found, b);
-        __syncthreads();
-    }
     return sh.found;
 }
 
@@ -477,15 +490,21 @@ __device__ __noinline__ void place_in(RowShared &sh, const Row &row, uint32_t bi
     const uint32_t tid = threadIdx.x;
     uint32_t nb = sh.count[bin], n = sh.count[bin + 1] - nb;
     double mb = sh.mass[bin];
-    find_edges(sh, row, bin, bin);
-    uint32_t low = sh.edge[0], high = sh.edge[1];
+    // (Few tokens that the list does not have are all that it then has.)
+    uint32_t low = 0, high = row.top_key;
+    const bool whole = !listed && n <= kOrder;
+    if (!whole) {
+        find_edges(sh, row, bin, bin);
+        low = sh.edge[0];
+        high = sh.edge[1];
+    }
     // The range of keys split into up to 1024 equal ones, and the one that
     // has the place again, until it has few tokens or one key. (Sums in units
     // of 2^-36: 2^26 weights fit 64 bits.)
     const double unit = step_weight(bin) * 0x1p-36;
     while (true) {
         if (!listed && n <= kList) {
-            collect(sh, row, bin, bin, low, high);
+            collect(sh, row, bin, bin, whole, low, high);
             listed = true;
         }
         if (n <= kOrder || low >= high) break;
@@ -510,7 +529,7 @@ __device__ __noinline__ void place_in(RowShared &sh, const Row &row, uint32_t bi
             }
             __syncthreads();
         } else {
-            each_token(sh, row, bin, bin, low, high, add);
+            each_token(sh, row, bin, bin, false, low, high, add);
         }
         const uint32_t mine = sh.split_n[tid];
         const double mass = (double)sh.split_m[tid] * unit;
@@ -612,14 +631,23 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
         uint64_t m = 0;
         for (uint32_t base = 0; base < n_parts; base += kThreads) {
             __syncthreads();
-            if (base + tid < n_parts) sh.raw[tid] = row.w.shift((uint32_t)(parts[base + tid].best >> 32));
+            if (base + tid < n_parts) {
+                const Part &part = parts[base + tid];
+                const uint32_t kept = part.kept_bins, s = row.w.shift((uint32_t)(part.best >> 32));
+                sh.raw[tid] = s;
+                if (base == 0) {
+                    sh.shift[tid] = (uint16_t)s;
+                    sh.kept[tid] = (uint16_t)kept;
+                }
+            }
             __syncthreads();
             const uint32_t held = min((uint32_t)kThreads, n_parts - base);
-#pragma unroll 4
+#pragma unroll 10
             for (uint32_t i = group; i < held; i += kThreads / kBins) {
+                // (A part all of whose tokens are dead has written no sums.)
                 const uint32_t s = sh.raw[i];
-                if (s > b || b >= kDead) continue;
-                const uint64_t sum = parts[base + i].sum[b - s];
+                const uint64_t read = parts[base + i].sum[b >= s ? b - s : 0];
+                const uint64_t sum = s > b || b >= kDead ? 0 : read;
                 n += (uint32_t)(sum >> kCountShift);
                 m += sum & ((1ull << kCountShift) - 1);
             }
@@ -650,6 +678,8 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
             }
         }
         __syncthreads();
+        if (tid < (int)kDead && sh.count[tid + 1] == sh.count[kDead] && sh.count[tid] != sh.count[kDead]) sh.last_live = tid;
+        __syncthreads();
     }
     const uint32_t live = sh.count[kDead];
     const bool by_k = p.top_k > 0 && p.top_k < live, by_p = p.top_p < 1.0f;
@@ -661,7 +691,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
     const float u = uniform[blockIdx.x];
     const double draw = u > 0.0f ? fmin((double)u, 1.0) : 0.0;
     // The last step that any rule can keep a token of.
-    uint32_t last = step_of(sh, false, (double)live, false);
+    uint32_t last = sh.last_live;
     if (by_k) last = min(last, step_of(sh, false, (double)p.top_k, false));
     else if (by_p) last = min(last, step_of(sh, true, (double)p.top_p * sh.mass[kDead], false));
     else if (least > 0.0 && !row.w.infinite) last = min(last, (uint32_t)fmin(row.w.reference - floor(top * row.w.c + 4.0 * log2(least)) + 1.0, (double)(kDead - 1)));
@@ -669,8 +699,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
     const uint32_t n = sh.count[last + 1];
     const bool listed = (by_k || by_p || least > 0.0) && n <= kList;
     if (listed) {
-        find_edges(sh, row, 0, last);
-        collect(sh, row, 0, last, sh.edge[0], sh.edge[1]);
+        collect(sh, row, 0, last, true, 0, 0);
     }
     if (listed && n <= kOrder) {
         // The rules one after another on its running sums.
@@ -718,8 +747,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
         __syncthreads();
         if (tid == 0) sh.counted = 0;
         __syncthreads();
-        find_edges(sh, row, lo, hi);
-        each_token(sh, row, lo, hi, sh.edge[0], sh.edge[1], [&](uint32_t key, uint32_t) {
+        each_token(sh, row, lo, hi, true, 0, 0, [&](uint32_t key, uint32_t) {
             if (enough(key)) atomicAdd(&sh.counted, 1u);
         });
         const uint32_t reaching = max(sh.count[lo] + sh.counted, 1u);
