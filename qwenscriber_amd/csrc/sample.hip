@@ -117,8 +117,11 @@ struct Weights {
     }
 };
 
-// A step's weight.
-__device__ __forceinline__ double step_weight(uint32_t bin) { return exp2(-0.25 * bin); }
+// A step's weight, 2^(-bin / 4).
+__device__ __forceinline__ double step_weight(uint32_t bin) {
+    const double odd = bin & 1 ? 0.8408964152537145 : 1.0, half = bin & 2 ? 0.7071067811865476 : 1.0;
+    return ldexp(odd * half, -(int)(bin >> 2));
+}
 
 // A weight within a step as a whole number of units: the sum with 2^52 rounds
 // to one and holds it in its low bits.
@@ -642,14 +645,22 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
             }
             __syncthreads();
             const uint32_t held = min((uint32_t)kThreads, n_parts - base);
-#pragma unroll 10
-            for (uint32_t i = group; i < held; i += kThreads / kBins) {
-                // (A part all of whose tokens are dead has written no sums.)
-                const uint32_t s = sh.raw[i];
-                const uint64_t read = parts[base + i].sum[b >= s ? b - s : 0];
-                const uint64_t sum = s > b || b >= kDead ? 0 : read;
-                n += (uint32_t)(sum >> kCountShift);
-                m += sum & ((1ull << kCountShift) - 1);
+            for (uint32_t i0 = group; i0 < held; i0 += 8 * (kThreads / kBins)) {
+                uint64_t read[8];
+                uint32_t s[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t i = i0 + k * (kThreads / kBins);
+                    s[k] = i < held ? sh.raw[i] : kDead;
+                    read[k] = parts[base + min(i, held - 1)].sum[b >= s[k] ? b - s[k] : 0];
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    // (A part all of whose tokens are dead has written no sums.)
+                    const uint64_t sum = s[k] > b || b >= kDead ? 0 : read[k];
+                    n += (uint32_t)(sum >> kCountShift);
+                    m += sum & ((1ull << kCountShift) - 1);
+                }
             }
         }
         sh.split_n[tid] = n;
