@@ -36,8 +36,7 @@ struct PagedAttentionArgs {
 struct PagedCopyArgs {
     qwh_paged_cache cache;
     uint64_t code_page, scale_page;  // bytes of a page's rows
-    uint32_t code_blocks, scale_blocks;
-    uint32_t scale_unit;             // 16 or 2 bytes
+    uint32_t code_pieces, scale_pieces;  // of a page's keys or values in a layer
 };
 
 hipError_t launch_paged_append(hipStream_t s, const PagedAppendArgs &args);

@@ -101,62 +101,74 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs
 
 // ---- copies of pages ----
 //
-// A thread holds kPieces 16-byte pieces of a page (of narrower ones where a
-// scale page is no multiple of 16 bytes) in one layer through a whole chain
-// of steps (paged_plan.h): what one step reads, an earlier or later step of
-// the same thread writes, so chains need no barrier, and a source that goes
-// to several pages is read once.
+// A page is, in every layer, key codes, value codes, key scales and value
+// scales; all layers' 16-byte pieces of these (2-byte ones of scales whose
+// page is no multiple of 16 bytes) stand in one line, and a workgroup takes an
+// equal stretch of it: no workgroup has a small plane to itself. A thread
+// holds its kPieces pieces through a whole chain of steps (paged_plan.h): what
+// one step reads, an earlier or later step of the same thread writes, so
+// chains need no barrier, and a source that goes to several pages is read
+// once.
 constexpr int kPieces = 4;
 
-template <typename T>
-__device__ __forceinline__ void copy_pieces(uint8_t *base, uint64_t page_bytes, uint32_t first, uint32_t pieces,
-                                            const paged::CopySteps &steps, uint32_t begin, uint32_t end) {
-    T v[kPieces], saved[kPieces];
+template <bool kNarrowScales>
+__global__ __launch_bounds__(256) void paged_copy_kernel(const PagedCopyArgs a, const paged::CopySteps steps) {
+    const uint32_t begin = steps.chain[blockIdx.y], end = steps.chain[blockIdx.y + 1];
+    const uint32_t per_layer = 2 * (a.code_pieces + a.scale_pieces);
+    const uint64_t start = (uint64_t)blockIdx.x * (256 * kPieces);
+    const uint32_t first_layer = (uint32_t)(start / per_layer), offset = (uint32_t)(start - (uint64_t)first_layer * per_layer);
+    uint8_t *at[kPieces];  // the piece in page 0
+    bool in_codes[kPieces], there[kPieces];
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+        uint32_t i = offset + 256 * k + threadIdx.x;
+        const uint32_t more = i / per_layer;
+        uint32_t layer = first_layer + more;
+        i -= more * per_layer;
+        there[k] = layer < a.cache.layers;
+        layer = min(layer, a.cache.layers - 1);  // (read, not written)
+        const bool codes = i < 2 * a.code_pieces;
+        if (!codes) i -= 2 * a.code_pieces;
+        const uint32_t plane = codes ? a.code_pieces : a.scale_pieces;
+        const bool values = i >= plane;
+        if (values) i -= plane;
+        const uint32_t bytes = kNarrowScales && !codes ? 2 : 16;
+        uint8_t *base = codes ? (values ? a.cache.v_codes : a.cache.k_codes) : (values ? a.cache.v_scales : a.cache.k_scales);
+        in_codes[k] = codes;
+        at[k] = base + (uint64_t)layer * a.cache.pages * (codes ? a.code_page : a.scale_page) + (uint64_t)i * bytes;
+    }
+    typedef uint32_t Piece __attribute__((ext_vector_type(4)));
+    const auto load = [&](Piece(&v)[kPieces], uint32_t src) {
+        const uint64_t in_code = src * a.code_page, in_scale = src * a.scale_page;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+            const uint8_t *from = at[k] + (in_codes[k] ? in_code : in_scale);
+            if (!kNarrowScales || in_codes[k]) v[k] = *reinterpret_cast<const Piece *>(from);
+            else v[k].x = *reinterpret_cast<const uint16_t *>(from);
+        }
+    };
+    const auto store = [&](const Piece(&v)[kPieces], uint32_t dst) {
+        const uint64_t in_code = dst * a.code_page, in_scale = dst * a.scale_page;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+            if (!there[k]) continue;
+            uint8_t *to = at[k] + (in_codes[k] ? in_code : in_scale);
+            if (!kNarrowScales || in_codes[k]) *reinterpret_cast<Piece *>(to) = v[k];
+            else *reinterpret_cast<uint16_t *>(to) = (uint16_t)v[k].x;
+        }
+    };
+    Piece v[kPieces] = {}, saved[kPieces] = {};
     uint32_t held = paged::kSaved;  // the page in v
     for (uint32_t i = begin; i < end; ++i) {
         const uint32_t src = steps.src[i], dst = steps.dst[i];
-        if (src == paged::kSaved) {
-#pragma unroll
-            for (int k = 0; k < kPieces; ++k) v[k] = saved[k];
-        } else if (src != held) {
-            const T *from = reinterpret_cast<const T *>(base + src * page_bytes);
-#pragma unroll
-            for (int k = 0; k < kPieces; ++k)
-                if (first + 256 * k < pieces) v[k] = from[first + 256 * k];
+        if (dst == paged::kSaved) load(saved, src);
+        else if (src == paged::kSaved) store(saved, dst);
+        else {
+            if (src != held) load(v, src);
+            held = src;
+            store(v, dst);
         }
-        held = src;
-        if (dst == paged::kSaved) {
-#pragma unroll
-            for (int k = 0; k < kPieces; ++k) saved[k] = v[k];
-            held = paged::kSaved;
-            continue;
-        }
-        T *to = reinterpret_cast<T *>(base + dst * page_bytes);
-#pragma unroll
-        for (int k = 0; k < kPieces; ++k)
-            if (first + 256 * k < pieces) to[first + 256 * k] = v[k];
     }
-}
-
-__global__ __launch_bounds__(256) void paged_copy_kernel(const PagedCopyArgs a, const paged::CopySteps steps) {
-    const uint32_t layer = blockIdx.y, chain = blockIdx.z;
-    const uint32_t begin = steps.chain[chain], end = steps.chain[chain + 1];
-    const uint64_t code_page = a.code_page, scale_page = a.scale_page;
-    uint32_t block = blockIdx.x;
-    const bool codes = block < 2 * a.code_blocks;
-    if (!codes) block -= 2 * a.code_blocks;
-    const uint32_t per = codes ? a.code_blocks : a.scale_blocks;
-    const bool values = block >= per;
-    if (values) block -= per;
-    const uint32_t first = block * 256 * kPieces + threadIdx.x;
-    if (codes) {
-        uint8_t *base = (values ? a.cache.v_codes : a.cache.k_codes) + (uint64_t)layer * a.cache.pages * code_page;
-        copy_pieces<uint4>(base, code_page, first, (uint32_t)(code_page / 16), steps, begin, end);
-        return;
-    }
-    uint8_t *base = (values ? a.cache.v_scales : a.cache.k_scales) + (uint64_t)layer * a.cache.pages * scale_page;
-    if (a.scale_unit == 16) copy_pieces<uint4>(base, scale_page, first, (uint32_t)(scale_page / 16), steps, begin, end);
-    else copy_pieces<uint16_t>(base, scale_page, first, (uint32_t)(scale_page / 2), steps, begin, end);
 }
 
 }  // namespace
@@ -184,15 +196,15 @@ hipError_t launch_paged_copy(hipStream_t s, const qwh_paged_cache &cache, const 
     a.code_page = cache.page_size * width;
     a.scale_page = cache.page_size * (width / 64) * 2;
     // 16-byte pieces of the scales where every page starts and ends on them.
-    a.scale_unit = a.scale_page % 16 == 0 && paged::aligned(cache.k_scales, 16) && paged::aligned(cache.v_scales, 16) ? 16 : 2;
-    const uint64_t per_block = 256 * kPieces;
-    const uint64_t code_blocks = (a.code_page / 16 + per_block - 1) / per_block;
-    const uint64_t scale_blocks = (a.scale_page / a.scale_unit + per_block - 1) / per_block;
-    if (2 * (code_blocks + scale_blocks) > 0xffffffu || cache.layers > 65535) return hipErrorInvalidValue;
-    a.code_blocks = (uint32_t)code_blocks;
-    a.scale_blocks = (uint32_t)scale_blocks;
-    const dim3 grid((uint32_t)(2 * (code_blocks + scale_blocks)), cache.layers, steps.chains);
-    paged_copy_kernel<<<grid, 256, 0, s>>>(a, steps);
+    const bool narrow = a.scale_page % 16 != 0 || !paged::aligned(cache.k_scales, 16) || !paged::aligned(cache.v_scales, 16);
+    a.code_pieces = (uint32_t)(a.code_page / 16);
+    a.scale_pieces = (uint32_t)(a.scale_page / (narrow ? 2 : 16));
+    const uint64_t pieces = 2 * ((uint64_t)a.code_pieces + a.scale_pieces) * cache.layers;
+    const uint64_t blocks = (pieces + 256 * kPieces - 1) / (256 * kPieces);
+    if (blocks > 0xffffffu) return hipErrorInvalidValue;
+    const dim3 grid((uint32_t)blocks, steps.chains);
+    if (narrow) paged_copy_kernel<true><<<grid, 256, 0, s>>>(a, steps);
+    else paged_copy_kernel<false><<<grid, 256, 0, s>>>(a, steps);
     return hipGetLastError();
 }
 
