@@ -143,14 +143,16 @@ __device__ __forceinline__ float f16_bits_to_f32(uint16_t bits) {
 
 // quant.zig:280-288 `quantizeOne`: round half away from zero against the
 // stored scale, clamp to [min_code, max_code].
-__device__ __forceinline__ int quantize_one(float value, float stored_scale, int min_code,
-                                            int max_code) {
-    if (stored_scale == 0.0f) return 0;
-    float scaled = __fdiv_rn(value, stored_scale);
+__device__ __forceinline__ int round_code(float scaled, int min_code, int max_code) {
     float rounded = scaled >= 0.0f ? floorf(__fadd_rn(scaled, 0.5f)) : ceilf(__fsub_rn(scaled, 0.5f));
     if (rounded <= (float)min_code) return min_code;
     if (rounded >= (float)max_code) return max_code;
     return (int)rounded;
+}
+__device__ __forceinline__ int quantize_one(float value, float stored_scale, int min_code,
+                                            int max_code) {
+    if (stored_scale == 0.0f) return 0;
+    return round_code(__fdiv_rn(value, stored_scale), min_code, max_code);
 }
 
 // ---------------------------------------------------------------------------

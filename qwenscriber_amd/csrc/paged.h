@@ -96,22 +96,46 @@ __device__ __forceinline__ uint32_t paged_pool_row(const qwh_paged_cache &c, con
     return page < c.pages ? page * c.page_size + (pos - at * c.page_size) : kNoRow;
 }
 
-// Four values of a 64-value group held by 16 consecutive lanes (lane % 16 the
-// place in the group) as q8 (quant.zig:209-288): codes to codes[4 * lane], the
-// group's scale to scales[lane / 16].
-__device__ __forceinline__ void store_q8x4(const float (&v)[4], int lane, uint8_t *codes, uint16_t *scales) {
-    float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+__device__ __forceinline__ float quad_max(const float (&v)[4]) {
+    return fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+}
+
+// The largest of 8 or 16 aligned lanes.
+template <int LANES>
+__device__ __forceinline__ float group_max(float m) {
     m = fmaxf(m, dev::xor_lane<1>(m));
     m = fmaxf(m, dev::xor_lane<2>(m));
     m = fmaxf(m, dev::xor_lane<4>(m));
-    m = fmaxf(m, dev::xor_lane<8>(m));
-    const uint16_t bits = dev::f32_to_f16_bits(__fdiv_rn(m, 128.0f));
+    if constexpr (LANES == 16) m = fmaxf(m, dev::xor_lane<8>(m));
+    return m;
+}
+
+// Four values of a 64-value group whose largest magnitude is m as q8
+// (quant.zig:209-288): their codes, and the group's scale by the lane that
+// has a place for it.
+__device__ __forceinline__ void store_q8x4_of(float m, const float (&v)[4], uint8_t *codes, uint16_t *scale) {
+    const uint16_t bits = dev::f32_to_f16_bits(__fmul_rn(m, 0.0078125f));  // (m / 128: the same rounding)
     const float stored = dev::f16_bits_to_f32(bits);
+    // The quotients as products with one reciprocal in f64, to 2^-50 of it.
+    // Rounded to f32 they are the f32 quotients: a value of 24 bits by a scale
+    // of 11 is 2^-37 or more of itself away from any middle of two f32.
+    double inverse = __builtin_amdgcn_rcp((double)stored);
+    inverse = fma(fma(-(double)stored, inverse, 1.0), inverse, inverse);
+    inverse = fma(fma(-(double)stored, inverse, 1.0), inverse, inverse);
     uint32_t word = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) word |= (uint32_t)(dev::quantize_one(v[i], stored, -128, 127) + 128) << (8 * i);
-    reinterpret_cast<uint32_t *>(codes)[lane] = word;
-    if ((lane & 15) == 0) scales[lane >> 4] = bits;
+    for (int i = 0; i < 4; ++i) {
+        const float scaled = stored == 0.0f ? 0.0f : (float)((double)v[i] * inverse);
+        word |= (uint32_t)(dev::round_code(scaled, -128, 127) + 128) << (8 * i);
+    }
+    *reinterpret_cast<uint32_t *>(codes) = word;
+    if (scale) *scale = bits;
+}
+
+// The same of a group that LANES aligned lanes hold.
+template <int LANES>
+__device__ __forceinline__ void store_q8x4(const float (&v)[4], uint8_t *codes, uint16_t *scale) {
+    store_q8x4_of(group_max<LANES>(quad_max(v)), v, codes, scale);
 }
 
 }  // namespace

@@ -14,88 +14,155 @@ namespace {
 // per query and key head, the rotation of its position, the query row out,
 // and key and value rows quantized into their page (quant.quantizeRow(.q8)).
 //
-// One wavefront a head row (a query head, a key head) or 256 values of the
+// A wavefront takes 8, 4, 2 or 2 (head_dim 64, 128, 192, 256) neighbouring
+// query or key heads of a row, a group of lanes each, or 512 values of the
 // value row: no wavefront waits for another, and a step's few rows still
-// spread over the device. The pair that the rotation mixes, dimensions d and
-// d + D/2, is one lane's, so norm and rotation need one reduction and no
-// exchange. Norm and rotation are in f64 (the square of an f32 is exact
-// there): a key's code is a rounding of its value, and 32-bit sums put about
-// one code in 10^5 on the other side of a border, by the order of the sum.
+// spread over the device. The values are asked for first; the way to the page
+// (the row's sequence, its position, its table) is a chain of loads of its own
+// meanwhile. A lane has four dimensions and the four that the rotation mixes
+// with them (D/2 further), so norm and rotation need one reduction over the
+// group, no exchange, and mostly neither do the 64 values of a scale. Norm and
+// rotation are in f64 (the square of an f32 is exact there): a key's code is a
+// rounding of its value, and 32-bit sums put about one code in 10^5 on the
+// other side of a border, by the order of the sum. Bound by instructions and
+// the stream of bytes about alike: 1608 tokens of 16 + 8 heads of 128 take 12.8
+// us (3.3 TB/s; a whole wavefront a head, 21), a step of up to 256 tokens the
+// 5 us of a launch.
+template <int MASK>
+__device__ __forceinline__ double xor_lane64(double v) {
+    const uint64_t x = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_bit_cast(uint32_t, dev::xor_lane<MASK>(__builtin_bit_cast(float, (uint32_t)x)));
+    const uint32_t hi = __builtin_bit_cast(uint32_t, dev::xor_lane<MASK>(__builtin_bit_cast(float, (uint32_t)(x >> 32))));
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// 1 / sqrt(x): the hardware's, about 2^-26 off, and two of Newton's steps.
+__device__ __forceinline__ double inverse_root(double x) {
+    const double r0 = __builtin_amdgcn_rsq(x);
+    double r = r0;
+    r = fma(r * 0.5, fma(-x * r, r, 1.0), r);
+    r = fma(r * 0.5, fma(-x * r, r, 1.0), r);
+    return r0 == 0.0 ? 0.0 : r;  // (of infinity)
+}
+
+typedef float Quad __attribute__((ext_vector_type(4), aligned(4)));
+
+// Lanes of a head, and heads and value quads of a wavefront.
+constexpr int head_lanes(int D) { return D == 64 ? 8 : D == 128 ? 16 : 32; }
+constexpr uint32_t kValues = 512;
+
 template <int D>
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs a) {
-    constexpr int H = D / 2;
-    constexpr int NP = (H + 63) / 64;  // pairs per lane
-    __shared__ float lds_k[4][D];
-    const uint32_t wave = threadIdx.x >> 6;
+    constexpr int H = D / 2, kLanes = head_lanes(D), kHeads = 64 / kLanes;
+    __shared__ float lds_k[D == 192 ? 4 : 1][D == 192 ? kHeads * D : 1];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
-    const uint64_t unit = (uint64_t)blockIdx.x * 4 + wave;
-    const uint32_t row = (uint32_t)(unit / a.units);
-    const uint32_t u = (uint32_t)(unit % a.units);
+    const uint32_t unit = blockIdx.x * 4 + wave;
+    const uint32_t row = unit / a.units, u = unit % a.units;
     if (row >= a.batch.rows) return;
+    const uint32_t kv_width = a.cache.kv_heads * D, normed = a.heads + a.cache.kv_heads;
+    const uint32_t head_units = (normed + kHeads - 1) / kHeads;
+    const float *src = a.qkv + (size_t)row * a.qkv_stride;
+    const bool is_value = u >= head_units;
+    const uint32_t first_head = u * kHeads, head = first_head + lane / kLanes, value = (u - head_units) * kValues + 4 * lane;
+    const int at = 4 * (lane % kLanes);  // of the head's dimensions
+    const bool there = head < normed && at < H;
+    float lo[4] = {}, hi[4] = {};
+    const auto take = [](float(&to)[4], const float *from) {
+        const Quad v = *reinterpret_cast<const Quad *>(from);
+        to[0] = v.x;
+        to[1] = v.y;
+        to[2] = v.z;
+        to[3] = v.w;
+    };
+    if (is_value) {
+        if (value < kv_width) take(lo, src + (size_t)normed * D + value);
+        if (value + 256 < kv_width) take(hi, src + (size_t)normed * D + value + 256);
+    } else if (there) {
+        take(lo, src + (size_t)head * D + at);
+        take(hi, src + (size_t)head * D + at + H);
+    }
     uint32_t b, t;
     if (!paged_row(a.batch, row, lane, b, t)) return;
     const uint64_t position = (uint64_t)a.batch.first[b] + t;
     if (position >= a.positions) return;
     const uint32_t pos = (uint32_t)position;
     const uint32_t pool_row = paged_pool_row(a.cache, a.batch.tables + (size_t)b * a.batch.table_pages, pos);
-    const float *src = a.qkv + (size_t)row * a.qkv_stride;
-    const uint32_t kv_width = a.cache.kv_heads * D;
     const uint32_t gpr = kv_width / 64;
-    if (u < a.heads + a.cache.kv_heads) {
-        const bool is_key = u >= a.heads;
-        if (is_key && pool_row == kNoRow) return;
-        const float *x = src + (size_t)u * D;
-        const float *w = is_key ? a.k_norm : a.q_norm;
-        float lo[NP], hi[NP], wl[NP], wh[NP], c[NP], s[NP];
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int j = lane + 64 * i;
-            const int jc = j < H ? j : 0;
-            lo[i] = x[jc];
-            hi[i] = x[jc + H];
-            wl[i] = w[jc];
-            wh[i] = w[jc + H];
-            c[i] = a.rope_cos[(size_t)pos * H + jc];
-            s[i] = a.rope_sin[(size_t)pos * H + jc];
-        }
-        double ss = 0.0;
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-            if (lane + 64 * i < H) ss += (double)lo[i] * lo[i] + (double)hi[i] * hi[i];
-#pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) ss += __shfl_xor(ss, m, 64);
-        const double inv = 1.0 / sqrt(ss / D + (double)a.eps);
-        float *q_out = a.query + (size_t)row * a.query_stride + (size_t)u * D;
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int j = lane + 64 * i;
-            if (j >= H) continue;
-            const double yl = (double)lo[i] * inv * wl[i], yh = (double)hi[i] * inv * wh[i];
-            const float rl = (float)(yl * c[i] - yh * s[i]), rh = (float)(yh * c[i] + yl * s[i]);
-            float *out = is_key ? &lds_k[wave][0] : q_out;
-            out[j] = rl;
-            out[j + H] = rh;
-        }
-        if (!is_key) return;
-        wave_fence();
-        const uint32_t col = (u - a.heads) * D;
-        if (lane * 4 < D) {
-            float v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = lds_k[wave][4 * lane + i];
-            store_q8x4(v, lane, a.cache.k_codes + (size_t)pool_row * kv_width + col,
-                       reinterpret_cast<uint16_t *>(a.cache.k_scales) + (size_t)pool_row * gpr + col / 64);
-        }
+    if (is_value) {
+        if (pool_row == kNoRow) return;
+        uint8_t *codes = a.cache.v_codes + (size_t)pool_row * kv_width + value;
+        uint16_t *scales = reinterpret_cast<uint16_t *>(a.cache.v_scales) + (size_t)pool_row * gpr + value / 64;
+        if (value < kv_width) store_q8x4<16>(lo, codes, lane % 16 == 0 ? scales : nullptr);  // (a multiple of 64)
+        if (value + 256 < kv_width) store_q8x4<16>(hi, codes + 256, lane % 16 == 0 ? scales + 4 : nullptr);
         return;
     }
-    if (pool_row == kNoRow) return;
-    const uint32_t col = (u - a.heads - a.cache.kv_heads) * 256;
-    const uint32_t left = kv_width - col;  // values from here on, a multiple of 64
-    if ((uint32_t)lane * 4 < left) {
-        const float4 f = *reinterpret_cast<const float4 *>(src + (size_t)(a.heads + a.cache.kv_heads) * D + col + 4 * lane);
-        const float v[4] = {f.x, f.y, f.z, f.w};
-        store_q8x4(v, lane, a.cache.v_codes + (size_t)pool_row * kv_width + col,
-                   reinterpret_cast<uint16_t *>(a.cache.v_scales) + (size_t)pool_row * gpr + col / 64);
+    // (first_head + kHeads - 1 may be a key where first_head is a query.)
+    if (pool_row == kNoRow && first_head >= a.heads) return;
+    const bool is_query = head < a.heads;
+    const float *w = (is_query ? a.q_norm : a.k_norm) + at;
+    float wl[4] = {}, wh[4] = {}, c[4] = {}, s[4] = {};
+    if (there) {
+        take(wl, w);
+        take(wh, w + H);
+        take(c, a.rope_cos + (size_t)pos * H + at);
+        take(s, a.rope_sin + (size_t)pos * H + at);
+    }
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss += (double)lo[i] * lo[i] + (double)hi[i] * hi[i];
+    if constexpr (kLanes >= 32) ss += xor_lane64<16>(ss);
+    if constexpr (kLanes >= 16) ss += xor_lane64<8>(ss);
+    ss += xor_lane64<4>(ss);
+    ss += xor_lane64<2>(ss);
+    ss += xor_lane64<1>(ss);
+    const double inv = inverse_root(ss * (1.0 / D) + (double)a.eps);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const double yl = (double)lo[i] * inv * wl[i], yh = (double)hi[i] * inv * wh[i];
+        lo[i] = (float)(yl * c[i] - yh * s[i]);
+        hi[i] = (float)(yh * c[i] + yl * s[i]);
+    }
+    if (there && is_query) {
+        float *out = a.query + (size_t)row * a.query_stride + (size_t)head * D + at;
+        *reinterpret_cast<float4 *>(out) = float4{lo[0], lo[1], lo[2], lo[3]};
+        *reinterpret_cast<float4 *>(out + H) = float4{hi[0], hi[1], hi[2], hi[3]};
+    }
+    if (pool_row == kNoRow || first_head + kHeads <= a.heads) return;
+    const bool is_key = there && !is_query;
+    uint8_t *codes = a.cache.k_codes + (size_t)pool_row * kv_width;
+    uint16_t *scales = reinterpret_cast<uint16_t *>(a.cache.k_scales) + (size_t)pool_row * gpr;
+    if constexpr (D == 192) {
+        // Scales' groups of 64 and halves of 96 do not fit: over LDS, 48
+        // lanes a head.
+        if (there) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                lds_k[wave][lane / kLanes * D + at + i] = lo[i];
+                lds_k[wave][lane / kLanes * D + at + H + i] = hi[i];
+            }
+        }
+        wave_fence();
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k) {
+            const uint32_t h = first_head + k;
+            if (h < a.heads || h >= normed || lane >= D / 4) continue;
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = lds_k[wave][k * D + 4 * lane + i];
+            const uint32_t col = (h - a.heads) * D + 4 * lane;
+            store_q8x4<16>(v, codes + col, lane % 16 == 0 ? scales + col / 64 : nullptr);
+        }
+    } else if (is_key) {
+        const uint32_t col = (head - a.heads) * D + at;
+        if constexpr (D == 64) {
+            const float m = group_max<8>(fmaxf(quad_max(lo), quad_max(hi)));
+            store_q8x4_of(m, lo, codes + col, at == 0 ? scales + col / 64 : nullptr);
+            store_q8x4_of(m, hi, codes + col + H, nullptr);
+        } else {
+            store_q8x4<16>(lo, codes + col, lane % 16 == 0 ? scales + col / 64 : nullptr);
+            store_q8x4<16>(hi, codes + col + H, lane % 16 == 0 ? scales + (col + H) / 64 : nullptr);
+        }
     }
 }
 
@@ -108,7 +175,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs
 // holds its kPieces pieces through a whole chain of steps (paged_plan.h): what
 // one step reads, an earlier or later step of the same thread writes, so
 // chains need no barrier, and a source that goes to several pages is read
-// once.
+// once. Bound by HBM: 300 pages of 16 positions in 28 layers, 283 MB read and
+// as much written, 119 us (4.8 TB/s; 8 pieces a thread, 157).
 constexpr int kPieces = 4;
 
 template <bool kNarrowScales>
@@ -176,7 +244,8 @@ __global__ __launch_bounds__(256) void paged_copy_kernel(const PagedCopyArgs a, 
 hipError_t launch_paged_append(hipStream_t s, const PagedAppendArgs &args) {
     PagedAppendArgs a = args;
     const uint32_t D = a.cache.head_dim;
-    a.units = a.heads + a.cache.kv_heads + (a.cache.kv_heads * D + 255) / 256;
+    const uint32_t heads = 64 / head_lanes((int)D);
+    a.units = (a.heads + a.cache.kv_heads + heads - 1) / heads + (a.cache.kv_heads * D + kValues - 1) / kValues;
     const uint64_t blocks = ((uint64_t)a.batch.rows * a.units + 3) / 4;
     if (blocks > 0xffffffu) return hipErrorInvalidValue;  // (x 256 threads: the grid's 32 bits)
     switch (D) {
