@@ -175,7 +175,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs
 // holds its kPieces pieces through a whole chain of steps (paged_plan.h): what
 // one step reads, an earlier or later step of the same thread writes, so
 // chains need no barrier, and a source that goes to several pages is read
-// once. Bound by HBM: 300 pages of 16 positions in 28 layers, 283 MB read and
+// once. Bound by HBM: 300 pages of 16 positions in 28 layers, 284 MB read and
 // as much written, 119 us (4.8 TB/s; 8 pieces a thread, 157).
 constexpr int kPieces = 4;
 

@@ -603,8 +603,8 @@ struct ManyLayout {
     static constexpr int kValues = kManyPositions * D * 2;           // [D][64] f16
     static constexpr int kScales = kValues + D * kManyPositions * 2;  // [2][64 / 4][G][4] f16: key scales, value scales
     static constexpr int kWeights = kScales + 2 * G * kManyPositions * 2;  // [2][64] f32: log2(vm), 2^12 / vm
-    static constexpr int kBad = kWeights + 2 * kManyPositions * 4;   // whether some value scale is no number
-    static constexpr int kBuffer = (kBad + 4 + 511) / 512 * 512;  // (row addresses are put together bit by bit)
+    static constexpr int kBad = kWeights + 2 * kManyPositions * 4;   // [G] u64: positions whose value scale is no number
+    static constexpr int kBuffer = (kBad + 8 * G + 511) / 512 * 512;  // (row addresses are put together bit by bit)
     static constexpr int kRows = 2 * kBuffer;                        // [4][64] pool rows in 16-byte pieces
     static constexpr int kPoolRows = kRows + 4 * kManyPositions * 4;  // [4][64] pool rows
     static constexpr int kThere = kPoolRows + 4 * kManyPositions * 4;  // [4] u64
@@ -774,39 +774,38 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
                 *reinterpret_cast<h8 *>(dst + (4 * quad + 3) * 128 + 16 * (eight ^ Lay::value_turn(4 * quad + 3))) = codes_across<3>(v_raw[j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            if (wave == 1) {
+                // Value scales that are no number count as 0 here, and the
+                // rows that see them are told apart in use(). (A position of
+                // zero scales counts as one of f16's least: its weight still
+                // belongs to the sum.)
+                float vm = 0x1p-24f;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const float vs = fabsf(dev::f16_bits_to_f32(scale_raw[g]));
+                    const bool bad = !(vs < INFINITY);
+                    const uint64_t some = __ballot(bad);
+                    if (lane == 0) reinterpret_cast<uint64_t *>(buf + Lay::kBad)[g] = some;
+                    if (bad) scale_raw[g] = 0;
+                    vm = fmaxf(vm, bad ? 0.0f : vs);
+                }
+                float *weights = reinterpret_cast<float *>(buf + Lay::kWeights);
+                weights[lane] = __builtin_amdgcn_logf(vm);
+                weights[kManyPositions + lane] = 4096.0f / vm;
+            }
             if (wave < 2) {
                 uint16_t *scales = reinterpret_cast<uint16_t *>(buf + Lay::kScales) + wave * G * kManyPositions + lane / 4 * (4 * G) + lane % 4;
 #pragma unroll
                 for (int g = 0; g < G; ++g) scales[4 * g] = scale_raw[g];
             }
-            if (wave == 1) {
-                // (A position of zero scales counts as one of f16's least:
-                // its weight still belongs to the sum.)
-                float vm = 0x1p-24f;
-                bool bad = false;
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const float vs = fabsf(dev::f16_bits_to_f32(scale_raw[g]));
-                    vm = fmaxf(vm, vs);
-                    bad |= !(vs < INFINITY);
-                }
-                const uint64_t some = __ballot(bad);
-                if (lane == 0) *reinterpret_cast<uint32_t *>(buf + Lay::kBad) = some != 0;
-                float *weights = reinterpret_cast<float *>(buf + Lay::kWeights);
-                weights[lane] = __builtin_amdgcn_logf(vm);
-                weights[kManyPositions + lane] = 4096.0f / vm;
-            }
         };
 
         // The query rows' two terms, times log2(e) / sqrt(D) and what brings
-        // products with the codes back. As they are where a wavefront's rows
-        // allow it (the largest value of each 2^-3 to 2^15, or zeros);
-        // otherwise scaled by a power of two a row to below 2^8, and the
-        // products by `fix` afterwards.
+        // products with the codes back, scaled by a power of two a row to
+        // below 2^8; the scores by `fix` afterwards.
         const size_t row = (size_t)start + t;
         h8 qh[G][4], ql[G][4];
-        float fix = 1.0f;
-        bool plain;
+        float fix;
         {
             f4 x[G][4][2];
             float top = 0.0f;
@@ -822,15 +821,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
                         top = fmaxf(top, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
                     }
             top = fmaxf(top, dev::xor_lane<32>(top));
-            float up = a.scaling * kCodeScale;
-            plain = __ballot(!(top == 0.0f || (top * up >= 0x1p-3f && top * up < 0x1p15f))) == 0;
-            if (!plain) {
-                int e = 0;
-                if (top > 0.0f && top < INFINITY) (void)__builtin_frexpf(top, &e);
-                e = e < -100 ? -100 : e;
-                up = a.scaling * __builtin_ldexpf(1.0f, 8 - e);
-                fix = __builtin_ldexpf(kCodeScale, e - 8);
-            }
+            int e = 0;
+            if (top > 0.0f && top < INFINITY) (void)__builtin_frexpf(top, &e);
+            e = e < -100 ? -100 : e;
+            const float up = a.scaling * __builtin_ldexpf(1.0f, 8 - e);
+            fix = __builtin_ldexpf(kCodeScale, e - 8);
 #pragma unroll
             for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -851,6 +846,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
         }
 
         float m = -INFINITY, l = 0.0f;
+        uint32_t not_numbers = 0;  // bit g: the row sees a value scale that is none
         f16v acc[G][2];
 #pragma unroll
         for (int g = 0; g < G; ++g)
@@ -875,34 +871,47 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
             // row 64 g + 32 k + col, whose turn is the column's and 4 g + 2 k.)
             const int key_at = (32 * blk + col) * (2 * D) + 16 * (half ^ Lay::key_turn(col));
             const int value_at = col * 128 + 16 * ((half ^ Lay::value_turn(col) ^ 4 * blk) & 7);
+            const auto key_chunk = [&](int g, int k) {
+                const int chunk = D % 128 == 0 ? key_at ^ 16 * (8 * g + 2 * k) : (key_at ^ 16 * (2 * k)) + 128 * g;
+                return *reinterpret_cast<const h8 *>(buf + Lay::kKeys + chunk);
+            };
+            uint64_t bad = 0;
+#pragma unroll
+            for (int g = 0; g < G; ++g) bad |= reinterpret_cast<const uint64_t *>(buf + Lay::kBad)[g];
+            const bool some_bad = uniform((uint32_t)(bad >> 32 * blk)) != 0;
+            // A group's chunks are read while the one before is multiplied.
+            h8 key[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) key[k] = key_chunk(0, k);
             float s[16];
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 f16v x = f16v{};
+                h8 next[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int chunk = D % 128 == 0 ? key_at ^ 16 * (8 * g + 2 * k) : (key_at ^ 16 * (2 * k)) + 128 * g;
-                    const h8 key = *reinterpret_cast<const h8 *>(buf + Lay::kKeys + chunk);
-                    x = mma32(key, ql[g][k], x);
-                    x = mma32(key, qh[g][k], x);
-                }
-                if (!plain) {
-                    asm volatile("");  // (a branch: seldom taken)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] *= fix;
+                    x = mma32(key[k], ql[g][k], x);
+                    x = mma32(key[k], qh[g][k], x);
+                    if (g + 1 < G) next[k] = key_chunk(g + 1, k);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const h4 ks = scale4(0, g, i);
-                    const f4 lv = g == 0 ? weight4(0, i) : f4{};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) s[4 * i + j] = fmaf((float)ks[j], x[4 * i + j], g == 0 ? lv[j] : s[4 * i + j]);
+                    for (int j = 0; j < 4; ++j) s[4 * i + j] = fmaf((float)ks[j], x[4 * i + j], g == 0 ? 0.0f : s[4 * i + j]);
                 }
-                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) key[k] = next[k];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f4 lv = weight4(0, i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[4 * i + j] = fmaf(s[4 * i + j], fix, lv[j]);
             }
             // (Branches around scores and weights only: one around the sums
             // would hold them twice, and spill.)
-            if (there != ~0u || base + 31 > common) {
+            if (there != ~0u || base + 31 > common || some_bad) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -910,7 +919,25 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
                         const uint32_t within = 8 * i + 4 * half + j;
                         if (!(there >> within & 1u) || base + within > limit) s[4 * i + j] = -INFINITY;
                     }
+                if (some_bad) {
+                    uint32_t seen = there;
+                    if (base + 31 > limit) seen &= base > limit ? 0u : ~0u >> (31 - (limit - base));
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const uint32_t none = (uint32_t)(reinterpret_cast<const uint64_t *>(buf + Lay::kBad)[g] >> 32 * blk);
+                        not_numbers |= (none & seen) != 0 ? 1u << g : 0u;
+                    }
+                }
             }
+            const auto value_chunk = [&](int g, int k, int i) {
+                return *reinterpret_cast<const h8 *>(buf + Lay::kValues + (64 * g + 32 * k) * 128 + (value_at ^ 16 * ((i ^ (4 * g + 2 * k)) & 7)));
+            };
+            h8 value[G][2];
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) value[g][k] = value_chunk(g, k, 0);
+            __builtin_amdgcn_sched_barrier(0);
             float mx = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
@@ -930,45 +957,36 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
                 m = to;
             }
             const float low = m == -INFINITY ? 0.0f : m;
-            const bool numbers = uniform(*reinterpret_cast<const uint32_t *>(buf + Lay::kBad)) == 0;
-            // 16 positions at a time: weights, then their products.
+            // 16 positions at a time: weights, then their products, the next
+            // ones' values on their way meanwhile.
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
+                const f4 rv[2] = {weight4(1, i), weight4(1, i + 1)};
+                h4 vs[G][2];
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) vs[g][k] = scale4(1, g, i + k);
                 float p[8];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const f4 rv = weight4(1, i + k);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        p[4 * k + j] = exp2_fast(s[4 * (i + k) + j] - low) * rv[j];
-                        l += p[4 * k + j];
-                    }
+                for (int j = 0; j < 8; ++j) {
+                    p[j] = exp2_fast(s[4 * i + j] - low) * rv[j / 4][j & 3];
+                    l += p[j];
                 }
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    float q[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) q[j] = p[j];
-                    h4 vs[2] = {scale4(1, g, i), scale4(1, g, i + 1)};
-                    if (!numbers) {
-                        asm volatile("");
-                        // (A scale that is no number must not reach rows that do not see it.)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) vs[j / 4][j & 3] = s[4 * i + j] == -INFINITY ? (_Float16)0.0f : vs[j / 4][j & 3];
-                    }
                     h8 hi, lo;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) hi[j] = (_Float16)(q[j] * (float)vs[j / 4][j & 3]);
+                    for (int j = 0; j < 8; ++j) hi[j] = (_Float16)fmaf(p[j], (float)vs[g][j / 4][j & 3], 0.0f);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) lo[j] = (_Float16)__builtin_fmaf(q[j], (float)vs[j / 4][j & 3], -(float)hi[j]);
+                    for (int j = 0; j < 8; ++j) lo[j] = (_Float16)fmaf(p[j], (float)vs[g][j / 4][j & 3], -(float)hi[j]);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) acc[g][k] = mma32(value[g][k], lo, acc[g][k]);
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        const h8 value = *reinterpret_cast<const h8 *>(buf + Lay::kValues + (64 * g + 32 * k) * 128 + (value_at ^ 16 * ((i ^ (4 * g + 2 * k)) & 7)));
-                        acc[g][k] = mma32(value, lo, acc[g][k]);
-                        acc[g][k] = mma32(value, hi, acc[g][k]);
+                        acc[g][k] = mma32(value[g][k], hi, acc[g][k]);
+                        if (i == 0) value[g][k] = value_chunk(g, k, 2);
                     }
-                    // (Reads moved up from the next round would cost
-                    // registers, and spill.)
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -1009,6 +1027,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
 
         if (!active) continue;
         l += dev::xor_lane<32>(l);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const float more = not_numbers >> g & 1u ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[g][i][j] += more;
+        }
         // Lane: dimensions 64 g + 32 k + 8 i + 4 half + 0..3 of its row.
         if (!alone) {
             const size_t rec = ((size_t)record * c.kv_heads + kvh) * kManyRows + 32 * wave + col;
