@@ -36,8 +36,18 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr uint32_t kUnit = 128;     // positions: one round of a workgroup
 constexpr uint32_t kTileRows = 8;   // query rows of a workgroup
 constexpr uint32_t kDies = 8;
-// Sequences of more query rows a key/value head take paged_many_kernel.
+// Sequences of more query rows a key/value head take paged_many_kernel, which
+// converts a code once for 128 rows instead of once for 8 (us, 8 key/value
+// heads of 128, 16 sequences of 2000 positions, few / many: 16 rows 37 / 61,
+// 32 rows 60 / 62, 64 rows 107 / 76). But its first answer comes 20 us after
+// its start against 6, so calls of little work in all take paged_few_kernel
+// alone: query rows of a key/value head times positions of the tables up to
+// kLittle (one sequence of 512 rows from position 0 on: 13 / 23; 4 of 256: 18
+// / 23; 8 of 256, twice the bound: 32 / 26), and up to kLittleNarrow of up to
+// 128 rows, which are one tile of paged_many_kernel (128 rows at 4000: 29 /
+// 41; at 16000, twice the bound: 84 / 68).
 constexpr uint32_t kFewRows = 32;
+constexpr uint64_t kLittle = 1 << 18, kLittleNarrow = 1 << 20;
 
 struct KernelArgs {
     PagedAttentionArgs p;
@@ -184,16 +194,27 @@ __device__ __forceinline__ h8 codes_across(const uint32_t (&w)[8]) {
     return h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
+// x as an f32 that is rounded here. A product that is converted to f16 may be
+// folded into the conversion and rounded once, or twice elsewhere: hi and what
+// it leaves would be of two numbers, half a step of hi apart.
+__device__ __forceinline__ float settled(float x) {
+    asm("" : "+v"(x));
+    return x;
+}
+
 // What a half leaves of x, as a half: one mixed multiply-add each.
 __device__ __forceinline__ _Float16 rest(float x, _Float16 hi) { return (_Float16)__builtin_fmaf((float)hi, -1.0f, x); }
 
 // x as hi + lo, both f16 (rounded to nearest, together 2^-22 of x).
 __device__ __forceinline__ void two_terms(const float (&x)[4], u2 &hi, u2 &lo) {
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = settled(x[i]);
     h4 h, l;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = (_Float16)x[i];
+    for (int i = 0; i < 4; ++i) h[i] = (_Float16)y[i];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) l[i] = rest(x[i], h[i]);
+    for (int i = 0; i < 4; ++i) l[i] = rest(y[i], h[i]);
     hi = __builtin_bit_cast(u2, h);
     lo = __builtin_bit_cast(u2, l);
 }
@@ -443,6 +464,16 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
             for (int i = 0; i < 4; ++i) largest = fmaxf(largest, fabsf(w[g][i]));
         }
         largest = row_max(largest);
+        if (__ballot(largest == INFINITY)) {
+            // (An infinite scale is its 64 dimensions' alone: the others keep
+            // their power of two.)
+            largest = 0.0f;
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) largest = fmaxf(largest, fabsf(w[g][i]) < INFINITY ? fabsf(w[g][i]) : 0.0f);
+            largest = row_max(largest);
+        }
         const float e_now = fmaxf(fmaxf(e_w + ceilf(turn), (float)((int)(__float_as_uint(largest) >> 23) - 126)), -100.0f);
         if (__ballot(turn != 0.0f || e_now != e_w)) {
             l *= exp2_fast(turn);
@@ -975,11 +1006,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
                 }
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
+                    float w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j] = settled(fmaf(p[j], (float)vs[g][j / 4][j & 3], 0.0f));
                     h8 hi, lo;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) hi[j] = (_Float16)fmaf(p[j], (float)vs[g][j / 4][j & 3], 0.0f);
+                    for (int j = 0; j < 8; ++j) hi[j] = (_Float16)w[j];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) lo[j] = (_Float16)fmaf(p[j], (float)vs[g][j / 4][j & 3], -(float)hi[j]);
+                    for (int j = 0; j < 8; ++j) lo[j] = rest(w[j], hi[j]);
 #pragma unroll
                     for (int k = 0; k < 2; ++k) acc[g][k] = mma32(value[g][k], lo, acc[g][k]);
 #pragma unroll
@@ -1148,9 +1182,10 @@ struct Forms {
 };
 
 Forms forms_of(const PagedAttentionArgs &a) {
-    const uint64_t ratio = a.heads / a.cache.kv_heads;
+    const uint64_t ratio = a.heads / a.cache.kv_heads, rows = ratio * (a.batch.row_starts ? a.batch.rows : a.batch.batch);
+    const uint64_t work = rows * a.batch.table_pages * a.cache.page_size;
+    if (rows <= kFewRows || work <= kLittle || (rows <= 128 && work <= kLittleNarrow)) return Forms{true, false};
     if (!a.batch.row_starts) return Forms{ratio <= kFewRows, ratio > kFewRows};
-    if (a.batch.rows * ratio <= kFewRows) return Forms{true, false};
     return Forms{a.batch.batch > 1, true};
 }
 

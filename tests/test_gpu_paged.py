@@ -214,6 +214,83 @@ def test_long_contexts(ctx, new, first):
     check(ctx, rng, (4, 2, 128), 16, new, first, one_row=max(new) == 1)
 
 
+# Tables far longer than the sequences: the kernel for many rows also takes
+# chunks that would otherwise be little work.
+WIDE = 70000
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_chunks_with_wide_tables(ctx, layout):
+    rng = np.random.default_rng(31)
+    check(ctx, rng, layout, 16, [1, 5, 0, 33, 70], [0, 200, 9, 0, 77], pad=3, spare=WIDE)
+
+
+@pytest.mark.parametrize("page_size", [1, 7, 16, 31, 64, 100])
+@pytest.mark.parametrize("n,first", [(31, 97), (64, 0), (65, 128), (130, 1)])
+def test_pages_that_end_inside_a_tile_with_wide_tables(ctx, page_size, n, first):
+    rng = np.random.default_rng(32)
+    check(ctx, rng, (4, 2, 64), page_size, [n, 3], [first, 129], spare=1100000 // page_size)
+
+
+@pytest.mark.parametrize("batch", [63, 64, 65, 130])
+def test_many_sequences_of_many_rows(ctx, batch):
+    rng = np.random.default_rng(33)
+    new = [(7 * b + 1) % 50 for b in range(batch)]
+    check(ctx, rng, (2, 1, 64), 16, new, [(37 * b) % 150 for b in range(batch)], pad=5)
+
+
+@pytest.mark.parametrize("spare", [2, WIDE])
+@pytest.mark.parametrize("scale", [np.inf, -np.inf, np.nan])
+def test_a_value_scale_that_is_no_number_reaches_the_rows_that_see_it(ctx, spare, scale):
+    """And of these only the 64 dimensions that it scales."""
+    rng = np.random.default_rng(34)
+    heads, kv_heads, D, n, f = 4, 2, 128, 50, 61
+    batch = Batch(rng, 16, [n], [f], spare=spare)
+    pool = Pool(ctx, rng, 1, batch.pages, 16, kv_heads, D)
+    owned = batch.owned()[0]
+    pool.fill(0, owned)
+    query = rng.standard_normal((n, heads * D)).astype(np.float32)
+    want, bound = reference(pool, 0, batch, query, heads)
+    at = 80  # seen by the tokens from 19 on
+    pool.scales[1][0, owned[at], 3] = scale  # key/value head 1, dimensions 64 on
+    got = attend(ctx, pool, 0, batch, query, heads).reshape(n, heads, 2, 64)
+    reached = np.zeros(got.shape, bool)
+    reached[at - f:, 2:, 1] = True
+    assert not np.isfinite(got[reached]).any()
+    assert np.all(np.abs(got - want.reshape(got.shape))[~reached] <= bound.reshape(got.shape)[~reached])
+
+
+@pytest.mark.parametrize("n,spare", [(1, 0), (33, 0), (33, WIDE)])
+def test_queries_whose_scaled_value_is_next_to_a_border_of_two_halves(ctx, n, spare):
+    """The query's two terms have to be of one number: x times the scaling,
+    rounded to f32 first or not, can round to two halves, a step apart (2^-11,
+    where both terms hold 2^-22). One dimension a head, so that the bound has
+    no sum of roundings to hide it in."""
+    rng = np.random.default_rng(36)
+    heads, kv_heads, D = 8, 2, 64
+    x = rng.uniform(4, 8, 1 << 22).astype(np.float32)
+    factor = np.float32(1.44269504088896340736) / np.sqrt(np.float32(D))
+    exact = x.astype(np.float64) * np.float64(factor) * 32
+    border = x[exact.astype(np.float16) != exact.astype(np.float32).astype(np.float16)]
+    assert len(border) > 100
+    batch = Batch(rng, 16, [n], [90], spare=spare, one_row=n == 1)
+    pool = Pool(ctx, rng, 1, batch.pages, 16, kv_heads, D)
+    pool.fill(0, batch.owned()[0])
+    query = np.zeros((n, heads, D), np.float32)
+    at = rng.integers(0, D, (n, heads, 1))
+    np.put_along_axis(query, at, border[rng.integers(0, len(border), at.shape)], 2)
+    query = query.reshape(n, heads * D)
+    got = attend(ctx, pool, 0, batch, query, heads)
+    want, bound = reference(pool, 0, batch, query, heads)
+    assert np.all(np.abs(got - want) <= bound)
+
+
+@pytest.mark.parametrize("n", [3, 40])
+def test_positions_without_a_page_with_wide_tables(ctx, n):
+    rng = np.random.default_rng(35)
+    check(ctx, rng, (4, 2, 128), 16, [n, n], [100, 37], spare=WIDE, holes=[(0, 0, NONE), (0, 5, NONE), (1, 1, NONE)])
+
+
 def test_other_layers_strides_and_spare_rows(ctx):
     rng = np.random.default_rng(6)
     check(ctx, rng, (16, 8, 128), 16, [3, 20], [50, 7], layers=3, layer=2, stride_extra=2052, pad=9)
