@@ -322,7 +322,8 @@ typedef struct {
  * +infinity, only those are drawn, evenly. A row with nothing but NaN and
  * -infinity gives 0. params_dev: one record per row. Weights and sums are held
  * in 64 bits and added in a fixed order; a token whose weight is below 2^-63 of
- * the largest is not drawn. At most 65535 rows and 2^26 logits a row. */
+ * the largest is not drawn. At most 65535 rows and 2^26 logits a row; takes
+ * about 1.2 bytes of the context's scratch memory per logit, up to 160 MB. */
 int32_t qwh_sample_rows(qwh_ctx *ctx, const float *logits_dev, uint32_t rows, uint32_t count,
                         const qwh_sampling *params_dev, const float *uniform_dev, uint32_t *ids_dev);
 
@@ -336,8 +337,8 @@ int32_t qwh_sample_rows(qwh_ctx *ctx, const float *logits_dev, uint32_t rows, ui
  * cache's layout (k / v scales [kv_heads*head_dim/64] f16, k / v codes
  * [kv_heads*head_dim] u8), device memory of the caller: code planes 16-byte,
  * scale planes 4-byte aligned. page_size is any number of positions from 1,
- * pages * page_size below 2^32 - 1, a layer's code plane below 64 GiB,
- * head_dim 64, 128, 192 or 256. */
+ * pages * page_size below 2^32 - 1, a layer's code plane below 64 GiB, at
+ * most 4096 kv_heads, head_dim 64, 128, 192 or 256. */
 typedef struct {
     uint32_t layers, pages, page_size, kv_heads, head_dim;
     uint8_t *k_scales, *k_codes, *v_scales, *v_codes;
@@ -355,8 +356,8 @@ typedef struct {
  * page tables[b][p / page_size]. `rows` is the number of rows the buffers
  * hold: rows behind the last sequence's are left as they are, and no row from
  * `rows` on is touched whatever row_starts holds. At most 65535 sequences,
- * 2^20 rows, 2^23 rows times query heads, 256 query heads per key/value head,
- * and page tables below 2^32 - 2^16 positions. */
+ * 2^20 rows, 4096 query heads, 2^23 rows times query heads, 256 query heads
+ * per key/value head, and page tables below 2^32 - 2^16 positions. */
 typedef struct {
     uint32_t batch, rows, table_pages;
     const uint32_t *row_starts; /* [batch + 1] or NULL */
@@ -390,8 +391,13 @@ int32_t qwh_paged_append(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t la
  * query_dev (query_stride floats apart, heads * head_dim values) gives row i
  * of out_dev (heads * head_dim values, back to back); rows of no sequence are
  * left as they are. Any number of new tokens per sequence, one among them,
- * and any heads / kv_heads ratio. query_dev and out_dev 16-byte aligned and
- * apart, query_stride a multiple of 4. */
+ * and any heads / kv_heads ratio, while rows times query heads per key/value
+ * head times the tables' positions stays below about 2^41 (else
+ * QWH_E_LIMIT_EXCEEDED). A value scale that is no finite number makes its own
+ * 64 dimensions of the rows that see it no numbers, and nothing else; a key
+ * scale its head's. query_dev and out_dev 16-byte aligned and apart,
+ * query_stride a multiple of 4. Records of split work are held in the
+ * context's scratch memory. */
 int32_t qwh_paged_attention(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t layer, const qwh_paged_batch *batch,
                             float *out_dev, const float *query_dev, uint32_t query_stride, uint32_t heads);
 
@@ -400,7 +406,8 @@ int32_t qwh_paged_attention(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t
  * read after the call returns). One source may go to several pages (a fork),
  * a page may be both source and destination (a compaction, a swap); a page
  * named as destination twice, or one from `pages` on, gives
- * QWH_E_INVALID_ARGUMENT, before any copy. */
+ * QWH_E_INVALID_ARGUMENT, before any copy. Pages of up to 8 GiB of codes a
+ * layer. */
 int32_t qwh_paged_copy(qwh_ctx *ctx, const qwh_paged_cache *cache, const uint32_t *src_pages,
                        const uint32_t *dst_pages, uint32_t count);
 

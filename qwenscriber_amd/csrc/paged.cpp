@@ -97,7 +97,7 @@ int32_t qwh_paged_copy(qwh_ctx *ctx, const qwh_paged_cache *cache, const uint32_
     QWH_REFUSE(paged::check_cache(cache));
     if (count == 0) return QWH_OK;
     if (!src_pages || !dst_pages) return fail(ctx, QWH_E_INVALID_ARGUMENT, "src_pages or dst_pages is null");
-    if (cache->layers > 65535) return fail(ctx, QWH_E_LIMIT_EXCEEDED, "more than 65535 layers");
+    QWH_REFUSE(paged::check_page(*cache));
     paged::CopyLaunches plan;
     try {
         paged::CopyPairs pairs;

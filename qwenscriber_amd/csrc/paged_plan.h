@@ -54,6 +54,13 @@ inline Refusal check_cache(const qwh_paged_cache *c) {
     return {};
 }
 
+// (A copy counts a page's pieces, of 16 bytes or of 2, in 32 bits.)
+inline Refusal check_page(const qwh_paged_cache &c) {
+    if ((uint64_t)c.page_size * c.kv_heads * c.head_dim > 8ull << 30)
+        return refuse(QWH_E_LIMIT_EXCEEDED, "a page of more than 8 GiB of codes a layer");
+    return {};
+}
+
 inline Refusal check_layer(const qwh_paged_cache &c, uint32_t layer) {
     if (layer >= c.layers) return refuse(QWH_E_INVALID_ARGUMENT, "layer is not one of the pool's");
     return {};

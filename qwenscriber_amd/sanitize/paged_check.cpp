@@ -131,6 +131,12 @@ void check_refusals() {
         change(c);
         expect(paged::check_cache(&c).status == status, what);
     };
+    qwh_paged_cache page = good;
+    page.pages = 2;
+    page.page_size = 1u << 23;
+    expect(paged::check_page(page).status == QWH_OK, "pages of 8 GiB");
+    page.page_size += 1;
+    expect(paged::check_page(page).status == QWH_E_LIMIT_EXCEEDED, "pages of more");
     cache(QWH_E_SHAPE_MISMATCH, "no layers", [](auto &c) { c.layers = 0; });
     cache(QWH_E_SHAPE_MISMATCH, "no pages", [](auto &c) { c.pages = 0; });
     cache(QWH_E_SHAPE_MISMATCH, "pages of no position", [](auto &c) { c.page_size = 0; });

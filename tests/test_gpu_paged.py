@@ -707,6 +707,49 @@ def test_refusals(ctx):
     batch.free()
 
 
+def test_two_contexts_at_once(ctx):
+    """Their streams run side by side on one pool that both only read."""
+    rng = np.random.default_rng(45)
+    other = qa.Context(0)
+    heads, kv_heads, D = 16, 8, 128
+    batches = [Batch(rng, 16, [1] * 9, [37 * i for i in range(9)]), Batch(rng, 16, [300, 2, 1], [1000, 700, 0])]
+    pools, query, out = [], [], []
+    for c, batch in zip((ctx, other), batches):
+        pool = Pool(c, rng, 1, batch.pages, 16, kv_heads, D)
+        pool.fill(0, np.concatenate(batch.owned()))
+        q = rng.standard_normal((batch.rows, heads * D)).astype(np.float32)
+        pools.append((pool, pool.upload(), batch.upload(c)))
+        query.append((q, c.to_device(q)))
+        out.append(c.buffer(q.nbytes))
+    for _ in range(20):
+        for c, (_, cache, desc), (_, q), o_ in zip((ctx, other), pools, query, out):
+            c.paged_attention(cache, 0, desc, o_.ptr, q.ptr, heads * D, heads)
+    for (pool, _, _), batch, (q, qbuf), o_ in zip(pools, batches, query, out):
+        want, bound = reference(pool, 0, batch, q, heads)
+        assert np.all(np.abs(o_.download(np.float32).reshape(want.shape) - want) <= bound)
+        for x in (qbuf, o_):
+            x.free()
+        pool.free()
+        batch.free()
+    other.close()
+
+
+def test_a_pool_s_last_page_and_the_same_page_in_two_tables(ctx):
+    """Sequences that share pages (a prompt's), the pool's last among them."""
+    rng = np.random.default_rng(46)
+    batch = Batch(rng, 16, [1, 4, 40], [50, 50, 50])
+    shared = np.setdiff1d(np.arange(batch.pages), batch.tables.reshape(-1))[:1]
+    for b in range(3):
+        batch.tables[b, 1] = batch.pages - 1
+        batch.tables[b, 0] = shared[0]
+    pool = Pool(ctx, rng, 1, batch.pages, 16, 2, 128)
+    pool.fill(0, np.unique(np.concatenate(batch.owned())))
+    query = rng.standard_normal((batch.rows, 4 * 128)).astype(np.float32)
+    got = attend(ctx, pool, 0, batch, query, 4)
+    want, bound = reference(pool, 0, batch, query, 4)
+    assert np.all(np.abs(got - want) <= bound)
+
+
 # ---------------------------------------------------------------------------
 def test_a_server_s_steps_with_a_fork(ctx):
     """A prompt appended and attended as one chunk, its pages shared by three

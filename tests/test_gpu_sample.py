@@ -148,6 +148,66 @@ def test_a_draw_follows_its_weights(ctx):
     assert np.all(np.abs(share - [0.5, 0.25, 0.125, 0.0625, 0.0625]) <= 2 / rows)
 
 
+def test_rows_of_many_parts(ctx):
+    """More parts of a row than the second pass has threads."""
+    rng = np.random.default_rng(8)
+    rules = [OFF, (1.0, 0, 0.7, 0.0), (1.5, 100000, 1.0, 0.0)]
+    logits = (2.0 * rng.standard_normal((3, 4300001))).astype(np.float32)
+    logits[:, rng.integers(0, logits.shape[1], 5)] += 6
+    check(ctx, logits, rules, rng.random(3, np.float32))
+
+
+def test_more_parts_than_one_launch_holds(ctx):
+    rng = np.random.default_rng(9)
+    logits = rng.standard_normal((40000, 5)).astype(np.float32)
+    check(ctx, logits, [RULES[r % len(RULES)] for r in range(40000)], rng.random(40000, np.float32))
+
+
+def test_two_contexts_at_once(ctx):
+    """Their streams run side by side; each has its own scratch memory."""
+    rng = np.random.default_rng(10)
+    other = qa.Context(0)
+    logits = (2.5 * rng.standard_normal((len(RULES), 50000))).astype(np.float32)
+    u = rng.random(len(RULES), np.float32)
+    params = np.frombuffer(b"".join(bytes(qa.Sampling(*r)) for r in RULES), np.uint8)
+    bufs = [[c.to_device(a) for a in (logits, params, u)] + [c.buffer(4 * len(RULES))] for c in (ctx, other)]
+    for _ in range(20):
+        for c, (l, p, n, ids) in zip((ctx, other), bufs):
+            c.sample_rows(l.ptr, len(RULES), logits.shape[1], p.ptr, n.ptr, ids.ptr)
+    want = [int(definition(logits[r], RULES[r], u[r])) for r in range(len(RULES))]
+    for b in bufs:
+        assert b[3].download(np.uint32).tolist() == want
+        for x in b:
+            x.free()
+    other.close()
+
+
+def test_a_decoder_s_steps_beside_larger_draws(ctx):
+    """A decoder's captured step between calls that grow the context's
+    scratch memory."""
+    config = dict(hidden=256, layers=2, heads=4, kv_heads=2, head_dim=128, ffn=512, vocab=1000, max_positions=32, eps=1e-6,
+                  theta=1e6)
+
+    def run(between):
+        c = qa.Context(0)
+        decoder = qa.Decoder(c, batch=3, **config)
+        decoder.init_synthetic(9)
+        set_norms(decoder, random_norms(config, 3), 2)
+        tokens, out = np.array([5, 6, 7], np.uint32), []
+        for step in range(6):
+            decoder.forward(tokens, want_logits=True)
+            if between:
+                big = np.zeros((8 << step, 30000), np.float32)
+                assert sample(c, big, [(0.0, 0, 1.0, 0.0)] * len(big), np.zeros(len(big))).tolist() == [0] * len(big)
+            out.append([decoder.logits(b) for b in range(3)])
+            tokens = decoder.sample(qa.Sampling(0.7, 40, 0.9, 0.0), [0.2, 0.5, 0.8])
+        decoder.close()
+        c.close()
+        return np.array(out)
+
+    assert np.array_equal(run(False), run(True))
+
+
 def test_greedy_is_the_argmax(ctx):
     rng = np.random.default_rng(6)
     logits = np.round(3 * rng.standard_normal((20, 5000))).astype(np.float32)
