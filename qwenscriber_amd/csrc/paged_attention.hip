@@ -256,6 +256,12 @@ __device__ __forceinline__ uint32_t take_other(uint32_t keep, uint32_t from) {
 //           l % 16's four dimensions of a group (one word a position), a
 //           product for each. The terms' sums are added at the end.
 // Two tiles of registers: one in flight while the other is used.
+//
+// Bound by HBM with a start and an end: 16 sequences at 4096 positions (138
+// MB, 28 us at the rate of a large copy) take 33 us here, 6 of them the chain
+// from the batch's arrays over a table to the first tile, and 4.7 in the join;
+// 61 of 1 to 5003 (325 MB, 66 us) 82 and 4.9. Loads alone take 36 in all, the
+// products alone 27.
 template <int D>
 __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
     constexpr int G = D / 64;
@@ -620,8 +626,19 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
 // P vs / vm = p vs. Both terms of 2^12 p vs then keep 2^-22 of the row's
 // largest; the sum is of 2^12 p = 2^12 P / vm.
 // Two LDS buffers and a barrier a tile: tile i + 1 is converted and tile i + 2
-// asked for at the start of tile i. Issue bound: of about 2600 cycles a
-// wavefront and tile (head_dim 128) the matrix cores work 2048.
+// asked for at the start of tile i. Units of 128 positions and at least one a
+// workgroup: a start costs 5 us, so units of 64 (402 rows x 2 from position 0
+// on: 27.4 us) or two a workgroup (33.6) lose to it (26.6).
+//
+// Bound by issue: 512 tokens of 16 heads over 8 x 128 at 7680 take 104 us and
+// the join 11 (33 GFLOP, 290 TFLOP/s; the two terms are twice that), in which
+// the vector unit is busy 60 % and the matrix cores 28 % of the cycles, with
+// two wavefronts a SIMD (256 registers) that overlap little. A tile of a
+// wavefront takes 8600 cycles: 2 x 1200 scores, 2 x 250 maximum, 2 x 1400
+// weights and values, 2800 for the next tile (rows, conversion, loads).
+// Converting between the products (spills), value chunks read a step earlier
+// (-3 %) and no read of the scores' chunks ahead (the same) did not change
+// that.
 constexpr int kManyRows = 128;
 constexpr int kManyPositions = 64;
 
@@ -671,7 +688,7 @@ __device__ __forceinline__ uint32_t tiles_units(const KernelArgs &a, uint32_t wh
 }
 
 template <int D>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const KernelArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void paged_many_kernel(const KernelArgs a) {
     using Lay = ManyLayout<D>;
     constexpr int G = D / 64;
     constexpr uint32_t kPieces = D / 16;                   // 16-byte pieces of a head row's codes
@@ -1101,6 +1118,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_many_kernel(const
 
 // Joins the records of a query row (one wavefront) in the order of its
 // positions. Rows whose tile one workgroup took whole were written by it.
+// Bound by latency: the chain row, plan, records; 3.6 us for one row of 16
+// heads, 11 for 512.
 template <int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(const KernelArgs a, uint32_t rows) {
     constexpr int G = D / 64;
@@ -1162,7 +1181,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const KernelArgs a, uin
 
 // Workgroups that a CU holds at once, by the kernels' registers.
 uint32_t resident_few(uint32_t head_dim) { return head_dim == 64 ? 3 : 2; }
-uint32_t resident_many(uint32_t head_dim) { return head_dim <= 128 ? 2 : 1; }
+uint32_t resident_many(uint32_t head_dim) { return head_dim == 64 ? 3 : head_dim == 128 ? 2 : 1; }
 
 // Stretches of a key/value head: as many workgroups as the device holds.
 uint32_t wanted_stretches(int cus, const PagedAttentionArgs &a, uint32_t resident) {
