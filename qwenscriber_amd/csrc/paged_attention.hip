@@ -636,9 +636,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
 // two wavefronts a SIMD (256 registers) that overlap little. A tile of a
 // wavefront takes 8600 cycles: 2 x 1200 scores, 2 x 250 maximum, 2 x 1400
 // weights and values, 2800 for the next tile (rows, conversion, loads).
-// Converting between the products (spills), value chunks read a step earlier
-// (-3 %) and no read of the scores' chunks ahead (the same) did not change
-// that.
+// Converting between the products instead takes the same (it spills).
 constexpr int kManyRows = 128;
 constexpr int kManyPositions = 64;
 
