@@ -71,22 +71,21 @@ __device__ __forceinline__ double rounded_product(double a, double b) {
     return a * b;
 }
 
-// 2^(f / 4) for f in [0, 1): e^t about the middle of the range, t = (f - 1/2)
-// ln(2) / 4 below 0.087 in magnitude, by its series to t^9 / 9! (the next term
-// is below 1e-17).
-__device__ __forceinline__ double quarter_power(double f) {
-    const double t = (f - 0.5) * 0.17328679513998633;
-    double e = 1.0 / 362880;
-    e = fma(e, t, 1.0 / 40320);
-    e = fma(e, t, 1.0 / 5040);
-    e = fma(e, t, 1.0 / 720);
-    e = fma(e, t, 1.0 / 120);
-    e = fma(e, t, 1.0 / 24);
-    e = fma(e, t, 1.0 / 6);
-    e = fma(e, t, 0.5);
-    e = fma(e, t, 1.0);
-    e = fma(e, t, 1.0);
-    return e * 1.0905077326652577;  // 2^(1/8)
+// 2^(f / 4) for f in [0, 1), times `scale` and plus `add`: e^t about the middle
+// of the range, t = (f - 1/2) ln(2) / 4 below 0.087 in magnitude, by its series
+// to t^7 / 7! (the next term is below 9e-14, a unit of a step's sum 7e-12).
+__device__ __forceinline__ double quarter_power(double f, double scale = 1.0, double add = 0.0) {
+    constexpr double kStep = 0.17328679513998633, kMiddle = 1.0905077326652577;  // ln(2) / 4, 2^(1/8)
+    const double t = fma(f, kStep, -0.5 * kStep), s = kMiddle * scale;
+    double e = s * (1.0 / 5040);
+    e = fma(e, t, s * (1.0 / 720));
+    e = fma(e, t, s * (1.0 / 120));
+    e = fma(e, t, s * (1.0 / 24));
+    e = fma(e, t, s * (1.0 / 6));
+    e = fma(e, t, s * 0.5);
+    e = fma(e, t, s);
+    e = fma(e, t, s);
+    return e + add;
 }
 
 // Weights against a reference step (infinite where the largest logit is: then
@@ -100,14 +99,19 @@ struct Weights {
     // A logit's step below the reference, at most kDead, and its weight
     // within the step.
     __device__ uint32_t bin(uint32_t key, double &within) const {
-        within = 1.0;
-        if (key <= kKeyMinusInf) return kDead;
-        if (infinite) return key == kKeyPlusInf ? 0 : kDead;
+        double f;
+        const uint32_t b = bin_and_rest(key, f);
+        within = quarter_power(f);
+        return b;
+    }
+    // The same with the place f within the step, 2^(f / 4) the weight.
+    __device__ __forceinline__ uint32_t bin_and_rest(uint32_t key, double &f) const {
         // (The product rounded first, as the reference's is: fused, the
         // largest finite logits would leave its rounding error.)
         const double y = rounded_product((double)key_logit(key), c), step = floor(y);
-        within = quarter_power(y - step);
-        return (uint32_t)fmin(reference - step, (double)kDead);
+        f = infinite ? 0.0 : y - step;
+        const uint32_t b = infinite ? (key == kKeyPlusInf ? 0 : kDead) : (uint32_t)fmin(reference - step, (double)kDead);
+        return key <= kKeyMinusInf ? kDead : b;
     }
     __device__ uint32_t bin(uint32_t key) const {
         if (key <= kKeyMinusInf) return kDead;
@@ -129,11 +133,10 @@ __device__ __forceinline__ double step_weight(uint32_t bin) {
     return ldexp(odd * half, -(int)(bin >> 2));
 }
 
-// A weight within a step as a whole number of units: the sum with 2^52 rounds
-// to one and holds it in its low bits.
-__device__ __forceinline__ uint64_t units_of(double within) {
-    const double v = within * (double)(1ull << kUnitBits) + 0x1p52;
-    return __builtin_bit_cast(uint64_t, v) & 0xfffffffffffffull;
+// A weight within a step, 2^(f / 4), as a whole number of units: the sum with
+// 2^52 rounds to one and holds it in its low bits.
+__device__ __forceinline__ uint64_t units_of(double f) {
+    return __builtin_bit_cast(uint64_t, quarter_power(f, (double)(1ull << kUnitBits), 0x1p52)) & 0xfffffffffffffull;
 }
 
 // What the first pass leaves of a part.
@@ -205,11 +208,19 @@ __global__ __launch_bounds__(256) void sample_parts_kernel(const float *logits, 
     const Weights w(steps_per_logit(p.temperature), top_key);
     uint8_t bin[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        double within;
-        const uint32_t b = w.bin(key[i], within);
-        bin[i] = (uint8_t)b;
-        if (b < kDead) atomicAdd(&sums[b], (unsigned long long)(1ull << kCountShift | units_of(within)));
+    for (int i0 = 0; i0 < 16; i0 += 8) {
+        // (Eight chains side by side, no branch between them.)
+        uint64_t add[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            double f;
+            bin[i0 + i] = (uint8_t)w.bin_and_rest(key[i0 + i], f);
+            add[i] = 1ull << kCountShift | units_of(f);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (bin[i0 + i] < kDead) atomicAdd(&sums[bin[i0 + i]], (unsigned long long)add[i]);
     }
     __syncthreads();
     // The steps whose tokens fit the short list.
