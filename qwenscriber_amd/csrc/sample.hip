@@ -71,22 +71,46 @@ __device__ __forceinline__ double rounded_product(double a, double b) {
     return a * b;
 }
 
+// A constant in scalar registers: as a literal it would be moved into the
+// result of each multiply-add first.
+__device__ __forceinline__ double held(double c) {
+    asm("" : "+s"(c));
+    return c;
+}
+
 // 2^(f / 4) for f in [0, 1), times `scale` and plus `add`: e^t about the middle
 // of the range, t = (f - 1/2) ln(2) / 4 below 0.087 in magnitude, by its series
 // to t^7 / 7! (the next term is below 9e-14, a unit of a step's sum 7e-12).
-__device__ __forceinline__ double quarter_power(double f, double scale = 1.0, double add = 0.0) {
-    constexpr double kStep = 0.17328679513998633, kMiddle = 1.0905077326652577;  // ln(2) / 4, 2^(1/8)
-    const double t = fma(f, kStep, -0.5 * kStep), s = kMiddle * scale;
-    double e = s * (1.0 / 5040);
-    e = fma(e, t, s * (1.0 / 720));
-    e = fma(e, t, s * (1.0 / 120));
-    e = fma(e, t, s * (1.0 / 24));
-    e = fma(e, t, s * (1.0 / 6));
-    e = fma(e, t, s * 0.5);
-    e = fma(e, t, s);
-    e = fma(e, t, s);
-    return e + add;
-}
+struct QuarterPower {
+    double step, half, c7, c6, c5, c4, c3, c2, c1, add;
+
+    __device__ __forceinline__ QuarterPower(double scale, double add_) {
+        constexpr double kStep = 0.17328679513998633, kMiddle = 1.0905077326652577;  // ln(2) / 4, 2^(1/8)
+        const double s = kMiddle * scale;
+        step = held(kStep);
+        half = held(-0.5 * kStep);
+        c7 = held(s * (1.0 / 5040));
+        c6 = held(s * (1.0 / 720));
+        c5 = held(s * (1.0 / 120));
+        c4 = held(s * (1.0 / 24));
+        c3 = held(s * (1.0 / 6));
+        c2 = held(s * 0.5);
+        c1 = held(s);
+        add = held(add_);
+    }
+    __device__ __forceinline__ double operator()(double f) const {
+        const double t = fma(f, step, half);
+        double e = fma(c7, t, c6);
+        e = fma(e, t, c5);
+        e = fma(e, t, c4);
+        e = fma(e, t, c3);
+        e = fma(e, t, c2);
+        e = fma(e, t, c1);
+        e = fma(e, t, c1);
+        return e + add;
+    }
+};
+__device__ __forceinline__ double quarter_power(double f) { return QuarterPower(1.0, 0.0)(f); }
 
 // Weights against a reference step (infinite where the largest logit is: then
 // such logits weigh 1 and others nothing).
@@ -99,19 +123,22 @@ struct Weights {
     // A logit's step below the reference, at most kDead, and its weight
     // within the step.
     __device__ uint32_t bin(uint32_t key, double &within) const {
+        within = 1.0;
+        if (key <= kKeyMinusInf) return kDead;
+        if (infinite) return key == kKeyPlusInf ? 0 : kDead;
         double f;
-        const uint32_t b = bin_and_rest(key, f);
+        const uint32_t b = finite_bin(key_logit(key), f);
         within = quarter_power(f);
         return b;
     }
-    // The same with the place f within the step, 2^(f / 4) the weight.
-    __device__ __forceinline__ uint32_t bin_and_rest(uint32_t key, double &f) const {
+    // A logit's step and place f within it, 2^(f / 4) the weight, where the
+    // largest is finite. (NaN and -infinity come out at kDead by themselves.)
+    __device__ __forceinline__ uint32_t finite_bin(float l, double &f) const {
         // (The product rounded first, as the reference's is: fused, the
         // largest finite logits would leave its rounding error.)
-        const double y = rounded_product((double)key_logit(key), c), step = floor(y);
-        f = infinite ? 0.0 : y - step;
-        const uint32_t b = infinite ? (key == kKeyPlusInf ? 0 : kDead) : (uint32_t)fmin(reference - step, (double)kDead);
-        return key <= kKeyMinusInf ? kDead : b;
+        const double y = rounded_product((double)l, c), step = floor(y);
+        f = y - step;
+        return (uint32_t)fmin(reference - step, (double)kDead);
     }
     __device__ uint32_t bin(uint32_t key) const {
         if (key <= kKeyMinusInf) return kDead;
@@ -131,12 +158,6 @@ struct Weights {
 __device__ __forceinline__ double step_weight(uint32_t bin) {
     const double odd = bin & 1 ? 0.8408964152537145 : 1.0, half = bin & 2 ? 0.7071067811865476 : 1.0;
     return ldexp(odd * half, -(int)(bin >> 2));
-}
-
-// A weight within a step, 2^(f / 4), as a whole number of units: the sum with
-// 2^52 rounds to one and holds it in its low bits.
-__device__ __forceinline__ uint64_t units_of(double f) {
-    return __builtin_bit_cast(uint64_t, quarter_power(f, (double)(1ull << kUnitBits), 0x1p52)) & 0xfffffffffffffull;
 }
 
 // What the first pass leaves of a part.
@@ -172,55 +193,67 @@ __global__ __launch_bounds__(256) void sample_parts_kernel(const float *logits, 
     if (tid == 0) kept_bins = 0;
     // Sixteen logits a thread, four in a row: 16-byte loads where the row
     // allows them.
-    uint32_t key[16];
+    float l[16];
     const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15u) == 0 && n == kPart;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const uint32_t at = 1024 * k + 4 * tid;
         if (aligned) {
             const float4 v = *reinterpret_cast<const float4 *>(row + first + at);
-            key[4 * k] = logit_key(v.x);
-            key[4 * k + 1] = logit_key(v.y);
-            key[4 * k + 2] = logit_key(v.z);
-            key[4 * k + 3] = logit_key(v.w);
+            l[4 * k] = v.x;
+            l[4 * k + 1] = v.y;
+            l[4 * k + 2] = v.z;
+            l[4 * k + 3] = v.w;
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) key[4 * k + j] = at + j < n ? logit_key(row[first + at + j]) : 0u;
+            for (int j = 0; j < 4; ++j) l[4 * k + j] = at + j < n ? row[first + at + j] : -INFINITY;
         }
     }
-    // The largest key, then the lowest index that has it.
-    uint32_t top_key = 0;
+    // The largest (NaN apart), then the lowest index that has it.
+    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top_key = max(top_key, key[i]);
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, l[i]);
     uint32_t at_top = 15;
 #pragma unroll
     for (int i = 15; i >= 0; --i)
-        if (key[i] == top_key) at_top = i;
-    uint64_t best = (uint64_t)top_key << 32 | (uint32_t) ~(first + 1024 * (at_top / 4) + 4 * tid + at_top % 4);
+        if (l[i] == top) at_top = i;
+    uint64_t best = (uint64_t)logit_key(top) << 32 | (uint32_t) ~(first + 1024 * (at_top / 4) + 4 * tid + at_top % 4);
     best = wave_largest(best);
     if (lane == 0) wave_best[wave] = best;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 4; ++w) best = wave_best[w] > best ? wave_best[w] : best;
-    top_key = (uint32_t)(best >> 32);
+    const uint32_t top_key = (uint32_t)(best >> 32);
     if (tid == 0) part.best = best;
     if (is_greedy(p) || top_key <= kKeyMinusInf) return;  // (nothing else of it is read)
     const Weights w(steps_per_logit(p.temperature), top_key);
     uint8_t bin[16];
+    if (w.infinite) {
 #pragma unroll
-    for (int i0 = 0; i0 < 16; i0 += 8) {
-        // (Eight chains side by side, no branch between them.)
-        uint64_t add[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            double f;
-            bin[i0 + i] = (uint8_t)w.bin_and_rest(key[i0 + i], f);
-            add[i] = 1ull << kCountShift | units_of(f);
+        for (int i = 0; i < 16; ++i) {
+            bin[i] = l[i] == INFINITY ? 0 : (uint8_t)kDead;
+            if (bin[i] == 0) atomicAdd(&sums[0], (unsigned long long)(1ull << kCountShift | 1ull << kUnitBits));
         }
-        __builtin_amdgcn_sched_barrier(0);
+    } else {
+        // A weight as a whole number of units: the sum with 2^52 rounds to
+        // one and holds it in its low bits. (Eight chains side by side, no
+        // branch between them.)
+        const QuarterPower units((double)(1ull << kUnitBits), 0x1p52);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (bin[i0 + i] < kDead) atomicAdd(&sums[bin[i0 + i]], (unsigned long long)add[i]);
+        for (int i0 = 0; i0 < 16; i0 += 8) {
+            uint64_t add[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                double f;
+                bin[i0 + i] = (uint8_t)w.finite_bin(l[i0 + i], f);
+                // (2^52's own bits give way to the count of 1.)
+                add[i] = __builtin_bit_cast(uint64_t, units(f)) - (0x433ull << 52) + (1ull << kCountShift);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (bin[i0 + i] < kDead) atomicAdd(&sums[bin[i0 + i]], (unsigned long long)add[i]);
+        }
     }
     __syncthreads();
     // The steps whose tokens fit the short list.
@@ -246,7 +279,7 @@ __global__ __launch_bounds__(256) void sample_parts_kernel(const float *logits, 
     for (int i = 0; i < 16; ++i)
         if (bin[i] < below) {
             const uint32_t at = atomicAdd(&place[bin[i]], 1u);
-            part.tokens[at] = (uint64_t)~key[i] << 32 | (first + 1024 * (i / 4) + 4 * tid + i % 4);
+            part.tokens[at] = (uint64_t)~logit_key(l[i]) << 32 | (first + 1024 * (i / 4) + 4 * tid + i % 4);
         }
     if (tid == 0) part.kept_bins = below;
 }
