@@ -23,11 +23,12 @@
 // in real numbers only where u falls within about 1e-12 of a border; with
 // 32-bit weights, about one draw in 1000 of an unfiltered row of 151936 would.
 //
-// The first launch is bound by its f64 instructions and LDS atomics (64 rows
-// of 151936, 39 MB: 18 us; one row 7), the second by latency: a chain of
-// rounds over one workgroup, 14 us where the kept tokens are few, up to 45
-// where a place lies in the bulk of an unfiltered row and the workgroup goes
-// over all its logits once more.
+// The first launch is bound by its vector instructions, f64 among them (64
+// rows of 151936, 39 MB: 20 us; one row 5.4; parts of 8192 logits, 27 and 12),
+// the second by latency: a chain of rounds over one workgroup, 14 us where the
+// kept tokens are few, up to 45 where a place lies in the bulk of an
+// unfiltered row and the workgroup goes over all its logits once more, 18 us
+// at what one CU can have in flight.
 #include <cmath>
 
 #include "common.h"
