@@ -142,13 +142,14 @@ __device__ __forceinline__ float f16_bits_to_f32(uint16_t bits) {
 }
 
 // quant.zig:280-288 `quantizeOne`: round half away from zero against the
-// stored scale, clamp to [min_code, max_code].
+// stored scale, clamp to [min_code, max_code]; round_code takes the quotient.
 __device__ __forceinline__ int round_code(float scaled, int min_code, int max_code) {
     float rounded = scaled >= 0.0f ? floorf(__fadd_rn(scaled, 0.5f)) : ceilf(__fsub_rn(scaled, 0.5f));
     if (rounded <= (float)min_code) return min_code;
     if (rounded >= (float)max_code) return max_code;
     return (int)rounded;
 }
+
 __device__ __forceinline__ int quantize_one(float value, float stored_scale, int min_code,
                                             int max_code) {
     if (stored_scale == 0.0f) return 0;

@@ -391,7 +391,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
         top = row_max(top);
         int e = 0;
         if (top > 0.0f && top < INFINITY) (void)__builtin_frexpf(top, &e);
-        e = e < -100 ? -100 : e;
+        e = e < -100 ? -100 : e > 126 ? 126 : e;  // (what undoes it is finite)
         const float up = __builtin_ldexpf(1.0f, 8 - e);
         qs = a.scaling * __builtin_ldexpf(kCodeScale, e - 8);
 #pragma unroll
@@ -437,7 +437,10 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float s0 = both[0][i] + dev::xor_lane<8>(both[0][i]), s1 = both[1][i] + dev::xor_lane<8>(both[1][i]);
-            s[i] = term ? s1 : s0;
+            // (Rounded here, in base 2: a multiply-add of the products against
+            // the scaled maximum would leave the maximum's own rounding error,
+            // which is no small number where scores are large.)
+            s[i] = settled((term ? s1 : s0) * qs);
         }
         const bool whole = tile.there == 0xffffffffu && base + 31 <= common;
         const int mine = 16 * term + 4 * quarter;  // this lane's first position of the tile
@@ -448,12 +451,12 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
         }
         const float mx = row_max(fmaxf(fmaxf(m, fmaxf(s[0], s[1])), fmaxf(s[2], s[3])));
         // A row that has seen nothing yet: weights of 0 against any maximum.
-        const float low = (mx == -INFINITY ? 0.0f : mx) * qs;
-        const float turn = fmaf(m, qs, -low);  // log2 of what earlier weights lose
+        const float low = mx == -INFINITY ? 0.0f : mx;
+        const float turn = m - low;  // log2 of what earlier weights lose
         m = mx;
         float p[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = exp2_fast(fmaf(s[i], qs, -low));
+        for (int i = 0; i < 4; ++i) p[i] = exp2_fast(s[i] - low);
         // The weights with their value scales, and the power of two that
         // brings the row's largest (of earlier ones too) near f16's top.
         float w[G][4], largest = 0.0f;
@@ -545,7 +548,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[g][i][j] = (acc[g][i][j] + dev::xor_lane<8>(acc[g][i][j])) * back;
-    float M = m == -INFINITY ? -INFINITY : m * qs;  // in base 2
+    float M = m;
     const int slot_row = n & 7;
     const bool writes = term == 0;
     // The four wavefronts' states into the first's: 2 and 3 hand theirs to 0
@@ -869,7 +872,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void paged_man
             top = fmaxf(top, dev::xor_lane<32>(top));
             int e = 0;
             if (top > 0.0f && top < INFINITY) (void)__builtin_frexpf(top, &e);
-            e = e < -100 ? -100 : e;
+            e = e < -100 ? -100 : e > 126 ? 126 : e;  // (what undoes it is finite)
             const float up = a.scaling * __builtin_ldexpf(1.0f, 8 - e);
             fix = __builtin_ldexpf(kCodeScale, e - 8);
 #pragma unroll

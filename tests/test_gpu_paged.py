@@ -361,6 +361,42 @@ def test_queries_of_any_size(ctx, query_scale):
     check(ctx, rng, (4, 2, 128), 16, [1, 20], [150, 60], query_scale=query_scale)
 
 
+@pytest.mark.parametrize("n,spare", [(1, 0), (40, 0), (40, WIDE)])
+def test_queries_next_to_the_largest_float(ctx, n, spare):
+    rng = np.random.default_rng(47)
+    heads, kv_heads, D = 4, 2, 128
+    batch = Batch(rng, 16, [n], [70], spare=spare, one_row=n == 1)
+    pool = Pool(ctx, rng, 1, batch.pages, 16, kv_heads, D)
+    pool.fill(0, batch.owned()[0], low=1e-4, high=5e-4)
+    query = np.zeros((n, heads, D), np.float32)
+    np.put_along_axis(query, rng.integers(0, D, (n, heads, 1)), np.float32(3.4e38), 2)
+    query = query.reshape(n, heads * D)
+    got = attend(ctx, pool, 0, batch, query, heads)
+    with np.errstate(all="ignore"):
+        want, _ = reference(pool, 0, batch, query, heads)
+    # One position has all the weight, or several of one code share it.
+    assert np.all(np.abs(got - want) <= 2.0**-20 * np.abs(want) + 1e-7)
+
+
+@pytest.mark.parametrize("n,spare", [(1, 0), (40, 0), (40, WIDE)])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+def test_a_query_row_that_is_no_number_stays_alone(ctx, n, spare, value):
+    rng = np.random.default_rng(48)
+    heads, kv_heads, D = 8, 2, 128
+    batch = Batch(rng, 16, [n] * 3, [70, 200, 5], spare=spare, one_row=n == 1)
+    pool = Pool(ctx, rng, 1, batch.pages, 16, kv_heads, D)
+    pool.fill(0, np.concatenate(batch.owned()))
+    query = rng.standard_normal((batch.rows, heads * D)).astype(np.float32)
+    want, bound = reference(pool, 0, batch, query, heads)
+    row, head = n + n // 2, 5
+    query[row, head * D + 7] = value
+    got = attend(ctx, pool, 0, batch, query, heads)
+    keep = np.ones((batch.rows, heads, D), bool)
+    keep[row, head] = False
+    keep = keep.reshape(batch.rows, heads * D)
+    assert np.all(np.abs(got - want)[keep] <= bound[keep])
+
+
 def test_rows_of_zeros_in_the_cache(ctx):
     rng = np.random.default_rng(13)
 
