@@ -1218,7 +1218,7 @@ uint64_t record_rows_many(int cus, const PagedAttentionArgs &a) {
 }
 
 template <int D>
-hipError_t launch_attention(hipStream_t s, int cus, const KernelArgs &k) {
+hipError_t launch_attention(hipStream_t s, const KernelArgs &k) {
     const qwh_paged_batch &b = k.p.batch;
     const Forms forms = forms_of(k.p);
     const uint32_t rows = b.row_starts ? b.rows : b.batch;
@@ -1268,10 +1268,10 @@ hipError_t launch_paged_attention(hipStream_t s, int cus, const PagedAttentionAr
     k.values_many = k.sums + record_rows_few(cus, a) * 2;
     k.sums_many = k.values_many + record_rows_many(cus, a) * D;
     switch (a.cache.head_dim) {
-    case 64: return launch_attention<64>(s, cus, k);
-    case 128: return launch_attention<128>(s, cus, k);
-    case 192: return launch_attention<192>(s, cus, k);
-    case 256: return launch_attention<256>(s, cus, k);
+    case 64: return launch_attention<64>(s, k);
+    case 128: return launch_attention<128>(s, k);
+    case 192: return launch_attention<192>(s, k);
+    case 256: return launch_attention<256>(s, k);
     default: return hipErrorNotSupported;
     }
 }
