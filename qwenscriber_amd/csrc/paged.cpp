@@ -98,7 +98,7 @@ int32_t qwh_paged_copy(qwh_ctx *ctx, const qwh_paged_cache *cache, const uint32_
     if (count == 0) return QWH_OK;
     if (!src_pages || !dst_pages) return fail(ctx, QWH_E_INVALID_ARGUMENT, "src_pages or dst_pages is null");
     QWH_REFUSE(paged::check_page(*cache));
-    paged::CopyLaunches plan;
+    paged::CopyLaunches plan(cache->pages <= paged::kShortPages);
     try {
         paged::CopyPairs pairs;
         QWH_REFUSE(paged::check_copies(src_pages, dst_pages, count, cache->pages, pairs));
@@ -108,8 +108,8 @@ int32_t qwh_paged_copy(qwh_ctx *ctx, const qwh_paged_cache *cache, const uint32_
     }
     OnDevice device(ctx->device);
     QWH_TRY(on_device(ctx, device));
-    for (const paged::CopySteps &steps : plan.launches)
-        QWH_TRY(check_hip(ctx, launch_paged_copy(ctx->stream, *cache, steps), "paged copy"));
+    for (const paged::CopyLaunch &launch : plan.launches)
+        QWH_TRY(check_hip(ctx, launch_paged_copy(ctx->stream, *cache, launch, plan.is_short), "paged copy"));
     return QWH_OK;
 }
 

@@ -40,7 +40,7 @@ struct PagedCopyArgs {
 };
 
 hipError_t launch_paged_append(hipStream_t s, const PagedAppendArgs &args);
-hipError_t launch_paged_copy(hipStream_t s, const qwh_paged_cache &cache, const paged::CopySteps &steps);
+hipError_t launch_paged_copy(hipStream_t s, const qwh_paged_cache &cache, const paged::CopyLaunch &launch, bool is_short);
 size_t paged_attention_scratch_bytes(int cus, const PagedAttentionArgs &a);
 hipError_t launch_paged_attention(hipStream_t s, int cus, const PagedAttentionArgs &a, void *scratch, size_t scratch_bytes);
 

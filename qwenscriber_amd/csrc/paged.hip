@@ -179,9 +179,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs
 // as much written, 119 us (4.8 TB/s; 8 pieces a thread, 157).
 constexpr int kPieces = 4;
 
-template <bool kNarrowScales>
-__global__ __launch_bounds__(256) void paged_copy_kernel(const PagedCopyArgs a, const paged::CopySteps steps) {
-    const uint32_t begin = steps.chain[blockIdx.y], end = steps.chain[blockIdx.y + 1];
+template <bool kNarrowScales, typename Steps>
+__global__ __launch_bounds__(256) void paged_copy_kernel(const PagedCopyArgs a, const Steps steps) {
+    static_assert(sizeof(a) + sizeof(steps) <= 4096, "a kernel's arguments");
+    const uint32_t begin = steps.begin(blockIdx.y), end = steps.end(blockIdx.y);
     const uint32_t per_layer = 2 * (a.code_pieces + a.scale_pieces);
     const uint64_t start = (uint64_t)blockIdx.x * (256 * kPieces);
     const uint32_t first_layer = (uint32_t)(start / per_layer), offset = (uint32_t)(start - (uint64_t)first_layer * per_layer);
@@ -228,10 +229,12 @@ __global__ __launch_bounds__(256) void paged_copy_kernel(const PagedCopyArgs a, 
     Piece v[kPieces] = {}, saved[kPieces] = {};
     uint32_t held = paged::kSaved;  // the page in v
     for (uint32_t i = begin; i < end; ++i) {
-        const uint32_t src = steps.src[i], dst = steps.dst[i];
+        const uint32_t src = steps.source(i), dst = steps.target(i);
         if (dst == paged::kSaved) load(saved, src);
-        else if (src == paged::kSaved) store(saved, dst);
-        else {
+        else if (src == paged::kSaved) {
+            store(saved, dst);
+            held = paged::kSaved;  // (dst may be the page in v)
+        } else {
             if (src != held) load(v, src);
             held = src;
             store(v, dst);
@@ -258,7 +261,7 @@ hipError_t launch_paged_append(hipStream_t s, const PagedAppendArgs &args) {
     return hipGetLastError();
 }
 
-hipError_t launch_paged_copy(hipStream_t s, const qwh_paged_cache &cache, const paged::CopySteps &steps) {
+hipError_t launch_paged_copy(hipStream_t s, const qwh_paged_cache &cache, const paged::CopyLaunch &launch, bool is_short) {
     PagedCopyArgs a{};
     a.cache = cache;
     const uint64_t width = (uint64_t)cache.kv_heads * cache.head_dim;
@@ -271,9 +274,13 @@ hipError_t launch_paged_copy(hipStream_t s, const qwh_paged_cache &cache, const 
     const uint64_t pieces = 2 * ((uint64_t)a.code_pieces + a.scale_pieces) * cache.layers;
     const uint64_t blocks = (pieces + 256 * kPieces - 1) / (256 * kPieces);
     if (blocks > 0xffffffu) return hipErrorInvalidValue;
-    const dim3 grid((uint32_t)blocks, steps.chains);
-    if (narrow) paged_copy_kernel<true><<<grid, 256, 0, s>>>(a, steps);
-    else paged_copy_kernel<false><<<grid, 256, 0, s>>>(a, steps);
+    const dim3 grid((uint32_t)blocks, launch.chains());
+    const auto run = [&](const auto &steps) {
+        if (narrow) paged_copy_kernel<true><<<grid, 256, 0, s>>>(a, steps);
+        else paged_copy_kernel<false><<<grid, 256, 0, s>>>(a, steps);
+    };
+    if (is_short) run(paged::pack_short(launch));
+    else run(paged::pack(launch));
     return hipGetLastError();
 }
 

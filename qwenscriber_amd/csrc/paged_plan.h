@@ -133,78 +133,166 @@ inline Refusal check_rows(const void *p, uint32_t stride, uint64_t width, const 
 constexpr uint32_t kSaved = 0xffffffffu;
 
 // Steps of one launch, handed over in the kernel's arguments (no upload, and
-// nothing that has to outlive the call): at most kMaxSteps, chains starting
-// at chain[0 .. chains - 1], chain[chains] their end.
+// nothing that has to outlive the call). In the short form, for pools of up to
+// kShortPages pages, a step is a word (its source below, its destination
+// above), and the chains' starts stand behind the steps, two a word, unless
+// every chain is one step.
 constexpr uint32_t kMaxSteps = 384;
 struct CopySteps {
     uint32_t chains;
     uint16_t chain[kMaxSteps + 1];
     uint32_t src[kMaxSteps], dst[kMaxSteps];
+
+    constexpr uint32_t begin(uint32_t c) const { return chain[c]; }
+    constexpr uint32_t end(uint32_t c) const { return chain[c + 1]; }
+    constexpr uint32_t source(uint32_t i) const { return src[i]; }
+    constexpr uint32_t target(uint32_t i) const { return dst[i]; }
 };
 
-// The pairs over the pages that they name: page[] in ascending order, and for
-// each of them the place in page[] of its source (kSaved: not a destination).
+constexpr uint32_t kShortPages = 0xffff, kShortWords = 990;
+struct CopyStepsShort {
+    uint32_t chains, steps;
+    uint32_t words[kShortWords];
+
+    constexpr uint32_t at(uint32_t c) const { return chains == steps ? c : words[steps + c / 2] >> (c % 2 * 16) & 0xffff; }
+    constexpr uint32_t begin(uint32_t c) const { return at(c); }
+    constexpr uint32_t end(uint32_t c) const { return at(c + 1); }
+    constexpr uint32_t page(uint32_t p) const { return p == kShortPages ? kSaved : p; }
+    constexpr uint32_t source(uint32_t i) const { return page(words[i] & 0xffff); }
+    constexpr uint32_t target(uint32_t i) const { return page(words[i] >> 16); }
+};
+
+// The pairs, and over the pages that they name: page[] in ascending order,
+// and for each of them the place in page[] of its source (kSaved: not a
+// destination). `apart`: no page is both (but for pages onto themselves), so
+// that any order does; the rest is then left out.
 struct CopyPairs {
+    const uint32_t *src, *dst;
+    uint32_t count;
+    bool apart;
     std::vector<uint32_t> page, source, order;  // order: the destinations' places, as given
 };
 
 inline Refusal check_copies(const uint32_t *src, const uint32_t *dst, uint32_t count, uint32_t pages, CopyPairs &out) {
+    out.src = src;
+    out.dst = dst;
+    out.count = count;
+    out.apart = false;
     out.page.clear();
-    for (uint32_t i = 0; i < count; ++i) {
+    out.order.clear();
+    for (uint32_t i = 0; i < count; ++i)
         if (src[i] >= pages || dst[i] >= pages) return refuse(QWH_E_INVALID_ARGUMENT, "a page is not one of the pool's");
-        out.page.push_back(src[i]);
-        out.page.push_back(dst[i]);
+    const char *twice = "a page is named as destination twice";
+    // A bit a page, where the pool is not far larger than the call: the
+    // ordering below costs the host about 0.1 us a pair.
+    if (pages <= (1u << 20) + 256ull * count) {
+        std::vector<uint64_t> written((pages + 63ull) / 64);
+        for (uint32_t i = 0; i < count; ++i) {
+            uint64_t &word = written[dst[i] / 64];
+            const uint64_t bit = 1ull << dst[i] % 64;
+            if (word & bit) return refuse(QWH_E_INVALID_ARGUMENT, twice);
+            word |= bit;
+        }
+        out.apart = true;
+        for (uint32_t i = 0; i < count && out.apart; ++i) out.apart = src[i] == dst[i] || !(written[src[i] / 64] >> src[i] % 64 & 1);
+        if (out.apart) return {};
     }
-    std::sort(out.page.begin(), out.page.end());
-    out.page.erase(std::unique(out.page.begin(), out.page.end()), out.page.end());
+    const bool all = pages <= 1024 + 4ull * count;  // every page has its own number as its place
+    if (all) {
+        out.page.resize(pages);
+        for (uint32_t p = 0; p < pages; ++p) out.page[p] = p;
+    } else {
+        out.page.insert(out.page.end(), src, src + count);
+        out.page.insert(out.page.end(), dst, dst + count);
+        std::sort(out.page.begin(), out.page.end());
+        out.page.erase(std::unique(out.page.begin(), out.page.end()), out.page.end());
+    }
     const auto place = [&](uint32_t p) {
-        return (uint32_t)(std::lower_bound(out.page.begin(), out.page.end(), p) - out.page.begin());
+        return all ? p : (uint32_t)(std::lower_bound(out.page.begin(), out.page.end(), p) - out.page.begin());
     };
     out.source.assign(out.page.size(), kSaved);
-    out.order.clear();
     for (uint32_t i = 0; i < count; ++i) {
         const uint32_t d = place(dst[i]);
-        if (out.source[d] != kSaved) return refuse(QWH_E_INVALID_ARGUMENT, "a page is named as destination twice");
+        if (out.source[d] != kSaved) return refuse(QWH_E_INVALID_ARGUMENT, twice);
         out.source[d] = place(src[i]);
         out.order.push_back(d);
     }
     return {};
 }
 
-// Appends steps to launches of at most kMaxSteps.
+// Steps in launches that hold as many as their form takes.
+struct CopyLaunch {
+    std::vector<uint32_t> chain{0}, src, dst;
+
+    uint32_t chains() const { return (uint32_t)chain.size() - 1; }
+    uint32_t steps() const { return (uint32_t)src.size(); }
+};
+
 class CopyLaunches {
   public:
-    std::vector<CopySteps> launches;
+    explicit CopyLaunches(bool is_short) : is_short(is_short) {}
+    const bool is_short;
+    std::vector<CopyLaunch> launches;
 
     // Starts a new chain.
     void chain() { fresh_ = true; }
     // One step of the current chain; `keep`: steps from here on that have to
     // be in one launch (this one first).
     void step(uint32_t src, uint32_t dst, uint32_t keep = 1) {
-        if (launches.empty() || used_ + keep > kMaxSteps) {
+        if (launches.empty() || !fits(launches.back(), keep)) {
             launches.emplace_back();
-            launches.back().chains = 0;
-            launches.back().chain[0] = 0;
-            used_ = 0;
+            launches.back().src.reserve(kShortWords);
+            launches.back().dst.reserve(kShortWords);
+            launches.back().chain.reserve(kShortWords + 1);
             fresh_ = true;
         }
-        CopySteps &l = launches.back();
-        if (fresh_) {
-            ++l.chains;
-            fresh_ = false;
-        }
-        l.src[used_] = src;
-        l.dst[used_] = dst;
-        l.chain[l.chains] = (uint16_t)++used_;
+        CopyLaunch &l = launches.back();
+        if (fresh_) l.chain.push_back(l.steps());
+        fresh_ = false;
+        l.src.push_back(src);
+        l.dst.push_back(dst);
+        l.chain.back() = l.steps();
     }
 
   private:
-    uint32_t used_ = 0;
+    bool fits(const CopyLaunch &l, uint32_t more) const {
+        const uint32_t steps = l.steps() + more, chains = l.chains() + (fresh_ ? 1 : 0);
+        if (!is_short) return steps <= kMaxSteps;
+        return steps + (chains == steps ? 0 : (chains + 2) / 2) <= kShortWords;
+    }
     bool fresh_ = true;
 };
 
+inline CopySteps pack(const CopyLaunch &l) {
+    CopySteps s{};
+    s.chains = l.chains();
+    for (uint32_t c = 0; c <= s.chains; ++c) s.chain[c] = (uint16_t)l.chain[c];
+    std::copy(l.src.begin(), l.src.end(), s.src);
+    std::copy(l.dst.begin(), l.dst.end(), s.dst);
+    return s;
+}
+
+inline CopyStepsShort pack_short(const CopyLaunch &l) {
+    CopyStepsShort s{};
+    s.chains = l.chains();
+    s.steps = l.steps();
+    const auto half = [](uint32_t p) { return p == kSaved ? kShortPages : p; };
+    for (uint32_t i = 0; i < s.steps; ++i) s.words[i] = half(l.src[i]) | half(l.dst[i]) << 16;
+    if (s.chains != s.steps)
+        for (uint32_t c = 0; c <= s.chains; ++c) s.words[s.steps + c / 2] |= l.chain[c] << (c % 2 * 16);
+    return s;
+}
+
 // The pairs' steps, a chain for each set of pages that copies connect.
 inline void order_copies(const CopyPairs &pairs, CopyLaunches &out) {
+    if (pairs.apart) {
+        for (uint32_t i = 0; i < pairs.count; ++i) {
+            if (pairs.src[i] == pairs.dst[i]) continue;
+            if (i == 0 || pairs.src[i] != pairs.src[i - 1]) out.chain();
+            out.step(pairs.src[i], pairs.dst[i]);
+        }
+        return;
+    }
     const std::vector<uint32_t> &source = pairs.source;
     const uint32_t n_pages = (uint32_t)source.size();
     const auto is_copied = [&](uint32_t p) { return source[p] != kSaved && source[p] != p; };

@@ -24,25 +24,27 @@ void expect(bool ok, const char *what, long a = 0, long b = 0) {
     if (++failures <= 20) std::printf("FAIL %s (%ld, %ld)\n", what, a, b);
 }
 
-// The launches, as paged_copy_kernel runs them.
-void run(const paged::CopyLaunches &plan, std::vector<uint64_t> &pool, std::mt19937 &rng) {
-    for (const paged::CopySteps &s : plan.launches) {
-        std::vector<uint32_t> chains(s.chains);
-        std::iota(chains.begin(), chains.end(), 0u);
-        std::shuffle(chains.begin(), chains.end(), rng);
-        for (uint32_t c : chains) {
-            uint64_t v = ~0ull, saved = ~0ull;
-            uint32_t held = paged::kSaved;
-            for (uint32_t i = s.chain[c]; i < s.chain[c + 1]; ++i) {
-                if (s.src[i] == paged::kSaved) v = saved;
-                else if (s.src[i] != held) v = pool[s.src[i]];
-                held = s.src[i];
-                if (s.dst[i] == paged::kSaved) {
-                    saved = v;
-                    held = paged::kSaved;
-                    continue;
-                }
-                pool[s.dst[i]] = v;
+// A launch, as paged_copy_kernel runs it.
+template <typename Steps>
+void run(const Steps &s, std::vector<uint64_t> &pool, std::mt19937 &rng) {
+    std::vector<uint32_t> chains(s.chains);
+    std::iota(chains.begin(), chains.end(), 0u);
+    std::shuffle(chains.begin(), chains.end(), rng);
+    for (uint32_t c : chains) {
+        uint64_t v = ~0ull, saved = ~0ull;
+        uint32_t held = paged::kSaved;
+        expect(s.begin(c) < s.end(c), "empty chain", c);
+        for (uint32_t i = s.begin(c); i < s.end(c); ++i) {
+            const uint32_t src = s.source(i), dst = s.target(i);
+            if (dst == paged::kSaved) {
+                saved = pool[src];
+            } else if (src == paged::kSaved) {
+                pool[dst] = saved;
+                held = paged::kSaved;
+            } else {
+                if (src != held) v = pool[src];
+                held = src;
+                pool[dst] = v;
             }
         }
     }
@@ -54,22 +56,28 @@ void copies(const std::vector<uint32_t> &src, const std::vector<uint32_t> &dst, 
     const paged::Refusal r = paged::check_copies(src.data(), dst.data(), (uint32_t)src.size(), pages, pairs);
     expect(r.status == QWH_OK, what, (long)src.size(), pages);
     if (r.status != QWH_OK) return;
-    paged::CopyLaunches plan;
-    paged::order_copies(pairs, plan);
-    std::vector<uint64_t> pool(pages);
-    std::iota(pool.begin(), pool.end(), 1000ull);
-    std::vector<uint64_t> want = pool;
-    for (size_t i = 0; i < src.size(); ++i) want[dst[i]] = pool[src[i]];
-    size_t steps = 0, moved = 0;
-    for (const paged::CopySteps &s : plan.launches) {
-        expect(s.chains >= 1 && s.chain[0] == 0 && s.chain[s.chains] <= paged::kMaxSteps, "launch size", s.chains);
-        for (uint32_t c = 0; c < s.chains; ++c) expect(s.chain[c] < s.chain[c + 1], "empty chain", c);
-        steps += s.chain[s.chains];
-    }
+    size_t moved = 0;
     for (size_t i = 0; i < src.size(); ++i) moved += src[i] != dst[i];
-    expect(steps <= 2 * moved, "more than two steps a page", (long)steps, (long)moved);
-    run(plan, pool, rng);
-    expect(pool == want, what, (long)src.size(), pages);
+    for (const bool is_short : {false, true}) {
+        if (is_short && pages > paged::kShortPages) continue;
+        paged::CopyLaunches plan(is_short);
+        paged::order_copies(pairs, plan);
+        std::vector<uint64_t> pool(pages);
+        std::iota(pool.begin(), pool.end(), 1000ull);
+        std::vector<uint64_t> want = pool;
+        for (size_t i = 0; i < src.size(); ++i) want[dst[i]] = pool[src[i]];
+        size_t steps = 0;
+        for (const paged::CopyLaunch &l : plan.launches) {
+            expect(l.chains() >= 1 && l.chain[l.chains()] == l.steps(), "launch size", l.chains());
+            expect(is_short ? l.steps() + (l.chains() == l.steps() ? 0 : (l.chains() + 2) / 2) <= paged::kShortWords
+                            : l.steps() <= paged::kMaxSteps, "launch size", l.steps());
+            steps += l.steps();
+            if (is_short) run(paged::pack_short(l), pool, rng);
+            else run(paged::pack(l), pool, rng);
+        }
+        expect(steps <= 2 * moved, "more than two steps a page", (long)steps, (long)moved);
+        expect(pool == want, what, (long)src.size(), pages);
+    }
 }
 
 void check_copies() {
@@ -83,7 +91,7 @@ void check_copies() {
     copies({0, 1}, {1, 0}, 2, rng, "swap");
     copies({0, 0, 0, 0}, {1, 2, 3, 4}, 5, rng, "fork");
     copies({0, 0, 1, 1, 0}, {1, 2, 3, 4, 0}, 5, rng, "fork and chain");
-    for (uint32_t n : {2u, 3u, 17u, 381u, 382u, 383u, 384u, 385u, 386u, 767u, 768u, 2000u}) {
+    for (uint32_t n : {2u, 3u, 17u, 381u, 382u, 383u, 384u, 385u, 386u, 767u, 768u, 988u, 989u, 990u, 991u, 2000u}) {
         // A cycle through n pages, with readers hanging off it, and a chain.
         std::vector<uint32_t> src = range(n, 0), dst = range(n, 1);
         dst[n - 1] = 0;
@@ -113,8 +121,15 @@ void check_copies() {
         for (size_t i = 0; i < dst.size(); ++i) src.push_back(permuted ? order[i] : rng() % pages);
         copies(src, dst, pages, rng, "random pairs");
     }
+    // Few pages of a large pool, and a pool so large that no bit a page is kept.
+    for (uint32_t pages : {100000u, (1u << 20) + 256 * 5 + 1}) {
+        const uint32_t p = pages - 6;
+        copies({p, p + 1, p + 2, 7, 7}, {p + 1, p + 2, p, p + 4, p + 5}, pages, rng, "high pages");
+        copies({p, p + 1, 3}, {p + 2, p + 3, p + 4}, pages, rng, "high pages apart");
+    }
     paged::CopyPairs pairs;
     const uint32_t a[] = {1, 2}, b[] = {3, 3}, c[] = {1, 9};
+    expect(paged::check_copies(a, b, 2, 1u << 31, pairs).status == QWH_E_INVALID_ARGUMENT, "a destination twice in a large pool");
     expect(paged::check_copies(a, b, 2, 9, pairs).status == QWH_E_INVALID_ARGUMENT, "a destination twice");
     expect(paged::check_copies(c, a, 2, 9, pairs).status == QWH_E_INVALID_ARGUMENT, "a source past the pool");
     expect(paged::check_copies(a, c, 2, 9, pairs).status == QWH_E_INVALID_ARGUMENT, "a destination past the pool");

@@ -660,6 +660,30 @@ def test_copies_of_many_pages(ctx):
     pool.free()
 
 
+@pytest.mark.parametrize("pages", [65534, 65535, 65536, 70000])
+def test_copies_in_pools_of_many_pages(ctx, pages):
+    """Either side of the pools whose page numbers fit 16 bits."""
+    rng = np.random.default_rng(49)
+    pool = Pool(ctx, rng, 1, pages, 1, 1, 64)
+    for k in range(2):
+        pool.codes[k][:] = rng.integers(0, 256, pool.codes[k].shape)
+        pool.scales[k].view(np.uint16)[:] = rng.integers(0, 65536, pool.scales[k].shape)
+    cache = pool.upload()
+    last = np.arange(pages - 5, pages)
+    order = rng.permutation(pages)
+    for src, dst in ((last, np.roll(last, 1)), (order[:2500], order[2500:5000]), (np.repeat(order[:300], 5), order[300:1800]),
+                     (order[:1300], np.roll(order[:1300], 1))):
+        ctx.paged_copy(cache, src, dst)
+        for k in range(2):
+            for planes in (pool.codes, pool.scales):
+                whole = planes[k].reshape(1, pages, -1)
+                whole[:, dst] = whole[:, src]
+    codes, scales = pool.download()
+    for k in range(2):
+        assert np.array_equal(codes[k], pool.codes[k]) and np.array_equal(scales[k], pool.scales[k].view(np.uint16))
+    pool.free()
+
+
 def test_copies_from_scale_planes_on_four_bytes(ctx):
     rng = np.random.default_rng(33)
     pages, size = 6, 16 * 64 // 32
