@@ -396,8 +396,8 @@ int32_t qwh_paged_append(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t la
  * QWH_E_LIMIT_EXCEEDED). A value scale that is no finite number makes its own
  * 64 dimensions of the rows that see it no numbers, and nothing else; a key
  * scale its head's. query_dev and out_dev 16-byte aligned and apart,
- * query_stride a multiple of 4. Records of split work are held in the
- * context's scratch memory. */
+ * query_stride a multiple of 4. Records of split work take about 100 MB of the
+ * context's scratch memory, or 2.3 MB a key/value head where that is more. */
 int32_t qwh_paged_attention(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t layer, const qwh_paged_batch *batch,
                             float *out_dev, const float *query_dev, uint32_t query_stride, uint32_t heads);
 
