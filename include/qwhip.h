@@ -355,9 +355,11 @@ typedef struct {
  * first[b], first[b] + 1, ...; its position p lives in row p % page_size of
  * page tables[b][p / page_size]. `rows` is the number of rows the buffers
  * hold: rows behind the last sequence's are left as they are, and no row from
- * `rows` on is touched whatever row_starts holds. At most 65535 sequences,
- * 2^20 rows, 4096 query heads, 2^23 rows times query heads, 256 query heads
- * per key/value head, and page tables below 2^32 - 2^16 positions. */
+ * `rows` on is touched whatever row_starts holds. (Launches and their forms
+ * go by `rows` and table_pages: spare ones cost time.) At most 65535
+ * sequences, 2^20 rows, 4096 query heads, 2^23 rows times query heads, 256
+ * query heads per key/value head, and page tables below 2^32 - 2^16
+ * positions. */
 typedef struct {
     uint32_t batch, rows, table_pages;
     const uint32_t *row_starts; /* [batch + 1] or NULL */
