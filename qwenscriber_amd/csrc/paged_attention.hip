@@ -624,11 +624,16 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
 //   values  [dimension][row] += V^T P^T, 16 positions at a time, counted in
 //           that order, so that weights stay in their lane.
 // Value scales: with vm the largest of a position's, the softmax runs over
-// score + log2(vm), so its weights P = p vm are at most 1 (2^3: the maximum
-// they are taken against moves only when it is passed by more) and so are
-// P vs / vm = p vs. Both terms of 2^12 p vs then keep 2^-22 of the row's
-// largest; the sum is of 2^12 p = 2^12 P / vm. (vs / vm and 1 / vm are worked
-// out once a tile: 133 -> 131 us in a long run of the chunk below.)
+// score + log2(vm), so its weights P = p vm are at most 1 (2^3: what they are
+// taken against moves only when it is passed by more) and so are P vs / vm =
+// p vs. Both terms of 2^12 p vs then keep 2^-22 of the row's largest; the sum
+// is of 2^12 p = 2^12 P / vm. (vs / vm and 1 / vm are worked out once a tile:
+// 133 -> 131 us in a long run of the chunk below.) Score and log2(vm) are one
+// f32: its rounding is as large as the score's own, half a step.
+// What weights are taken against is held as `low`, 12 below the largest score
+// of the time: scores less `low` stay below 16, f16's range, and `low` itself,
+// not the maximum, is what sums and records are relative to. From 2^26 on,
+// where f32 cannot hold the maximum less 12, it is the maximum.
 // Two LDS buffers and a barrier a tile: tile i + 1 is converted and tile i + 2
 // asked for at the start of tile i. Units of 128 positions and at least one a
 // workgroup: a start costs 5 us, so units of 64 (402 rows x 2 from position 0
@@ -900,7 +905,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void paged_man
                     }
         }
 
-        float m = -INFINITY, l = 0.0f;
+        float low = -INFINITY, l = 0.0f;
         uint32_t not_numbers = 0;  // bit g: the row sees a value scale that is none
         f16v acc[G][2];
 #pragma unroll
@@ -1000,11 +1005,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void paged_man
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
             mx = fmaxf(mx, dev::xor_lane<32>(mx));
-            // The maximum moves when some row's is passed by 2^3, or it has
-            // none yet.
-            if (__ballot(mx > m + 3.0f)) {
-                const float to = fmaxf(m, mx);
-                const float less = exp2_fast(m - (to == -INFINITY ? 0.0f : to));
+            // `low` moves when some row's maximum is past it by 2^15, 2^3
+            // more than it was put below one, or the row has none yet.
+            if (__ballot(mx - low > 15.0f)) {
+                const float below = mx - 12.0f;
+                const float to = fmaxf(low, mx - below > 14.0f ? mx : below);  // (16 and more: f32's steps there)
+                const float less = exp2_fast(low - (to == -INFINITY ? 0.0f : to));
                 l *= less;
 #pragma unroll
                 for (int g = 0; g < G; ++g)
@@ -1012,9 +1018,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void paged_man
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int j = 0; j < 16; ++j) acc[g][i][j] *= less;
-                m = to;
+                low = to;
             }
-            const float low = (m == -INFINITY ? 0.0f : m) - 12.0f;
+            const float against = low == -INFINITY ? 0.0f : low;
             // 16 positions at a time: weights, then their products, the next
             // ones' values on their way meanwhile.
 #pragma unroll
@@ -1028,7 +1034,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void paged_man
                 float p[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    p[j] = exp2_fast(s[4 * i + j] - low);
+                    p[j] = exp2_fast(s[4 * i + j] - against);
                     l = fmaf(p[j], rv[j / 4][j & 3], l);
                 }
 #pragma unroll
@@ -1101,7 +1107,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void paged_man
         if (!alone) {
             const size_t rec = ((size_t)record * c.kv_heads + kvh) * kManyRows + 32 * wave + col;
             if (half == 0) {
-                a.sums_many[2 * rec] = m;
+                a.sums_many[2 * rec] = low;
                 a.sums_many[2 * rec + 1] = l;
             }
 #pragma unroll
