@@ -417,7 +417,12 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
 
     const auto use = [&](const Tile &tile, uint32_t base) {
 #pragma unroll
-        for (int g = 0; g < G; ++g) lds_scale[wave][lane >> 5][g][lane & 31] = dev::f16_bits_to_f32(tile.scale[g]);
+        for (int g = 0; g < G; ++g) {
+            // (No finite number: NaN. An infinite key scale would else make
+            // scores of one sign, and weights of 0 where that is below.)
+            const float scale = dev::f16_bits_to_f32(tile.scale[g]);
+            lds_scale[wave][lane >> 5][g][lane & 31] = fmaf(scale, 0.0f, scale);
+        }
         wave_fence();
         f4 both[2];
 #pragma unroll
@@ -472,17 +477,8 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(const KernelArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) largest = fmaxf(largest, fabsf(w[g][i]));
         }
+        // (Of numbers: a scale that is none is its 64 dimensions' alone.)
         largest = row_max(largest);
-        if (__ballot(largest == INFINITY)) {
-            // (An infinite scale is its 64 dimensions' alone: the others keep
-            // their power of two.)
-            largest = 0.0f;
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) largest = fmaxf(largest, fabsf(w[g][i]) < INFINITY ? fabsf(w[g][i]) : 0.0f);
-            largest = row_max(largest);
-        }
         const float e_now = fmaxf(fmaxf(e_w + ceilf(turn), (float)((int)(__float_as_uint(largest) >> 23) - 126)), -100.0f);
         if (__ballot(turn != 0.0f || e_now != e_w)) {
             l *= exp2_fast(turn);
@@ -856,7 +852,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) void paged_man
             if (wave == 0) {
                 uint16_t *scales = reinterpret_cast<uint16_t *>(buf + Lay::kScales) + lane / 4 * (4 * G) + lane % 4;
 #pragma unroll
-                for (int g = 0; g < G; ++g) scales[4 * g] = scale_raw[g];
+                for (int g = 0; g < G; ++g)  // (an infinity: NaN, as in the few rows' form)
+                    scales[4 * g] = (scale_raw[g] & 0x7c00u) == 0x7c00u ? (uint16_t)0x7e00u : scale_raw[g];
             }
         };
 

@@ -1,5 +1,6 @@
-"""Attention over the paged cache where scores are large. Tolerances are derived per test, from constructions in which few
-roundings take part."""
+"""Attention over the paged cache where scores are large or no numbers.
+Tolerances are derived per test, from constructions in which few roundings
+take part."""
 import numpy as np
 import pytest
 
@@ -39,3 +40,24 @@ def test_equal_scores_of_any_size_share_their_row(ctx, n, spare, log2_score):
             v = pool.values(1, 0, seen, h // 2)
             bound = np.abs(v).mean(0) * (2 * (len(owned) + 64) * 2.0**-24 + 2.0**-21) + 1e-30
             assert np.all(np.abs(got[t, h] - v.mean(0)) <= bound), (t, h, got[t, h, :4], v.mean(0)[:4])
+
+
+@pytest.mark.parametrize("n,spare", [(1, 0), (50, 2), (50, WIDE)])
+@pytest.mark.parametrize("scale", [np.inf, -np.inf, np.nan])
+def test_a_key_scale_that_is_no_number_reaches_its_head_s_rows_that_see_it(ctx, n, spare, scale):
+    """Whatever sign the products with it have."""
+    rng = np.random.default_rng(63)
+    heads, kv_heads, D, f = 8, 2, 128, 61
+    batch = Batch(rng, 16, [n], [f], spare=spare, one_row=n == 1)
+    pool = Pool(ctx, rng, 1, batch.pages, 16, kv_heads, D)
+    owned = batch.owned()[0]
+    pool.fill(0, owned)
+    query = rng.standard_normal((n, heads * D)).astype(np.float32)
+    at = f - 5 if n == 1 else f + 19
+    plain = attend(ctx, pool, 0, batch, query, heads).reshape(n, heads, D)
+    pool.scales[0][0, owned[at], 3] = scale  # key/value head 1, dimensions 64 on
+    got = attend(ctx, pool, 0, batch, query, heads).reshape(n, heads, D)
+    reached = np.zeros(got.shape, bool)
+    reached[max(0, at - f):, heads // kv_heads:] = True
+    assert np.isnan(got[reached]).all()
+    assert np.array_equal(got[~reached], plain[~reached])
