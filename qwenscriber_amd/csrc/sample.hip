@@ -33,6 +33,7 @@
 
 #include "common.h"
 #include "device.h"
+#include "sample_plan.h"
 
 namespace qwh {
 namespace {
@@ -296,7 +297,7 @@ struct RowShared {
     uint32_t raw[kThreads];
     uint16_t shift[kThreads], kept[kThreads];  // of the first parts
     double wave_m[16];
-    uint32_t wave_n[16];
+    uint32_t wave_n[16], wave_step[kBins / 64];
     uint64_t wave_best[16];
     uint32_t listed, raw_parts, found, found_index, edge[2], last_live;
     uint32_t found_count, counted, tie;
@@ -519,21 +520,23 @@ __device__ uint32_t reach(RowShared &sh, uint32_t n, double at, bool past) {
 }
 
 // The step in which the count (`by_mass`: the sum) reaches `at` (past:
-// exceeds it): the last step with tokens if none does.
+// exceeds it): the first with tokens of which that holds (may_hold), the last
+// step with tokens if none does.
 __device__ uint32_t step_of(RowShared &sh, bool by_mass, double at, bool past) {
-    // (The sums never fall, and step 0 has the largest: where they pass `at`
-    // is a step with tokens. That none does is left to the sums' last bits.)
-    const auto passes = [&](uint32_t b) {
-        const double v = by_mass ? sh.mass[b + 1] : (double)sh.count[b + 1];
-        return past ? v > at : v >= at;
-    };
-    __syncthreads();
-    if (threadIdx.x == 0) sh.found = sh.last_live;
-    __syncthreads();
     const uint32_t b = threadIdx.x;
-    if (b < kDead && passes(b) && (b == 0 || !passes(b - 1))) sh.found = b;
+    bool here = false;
+    if (b < kDead) {
+        const double upto = by_mass ? sh.mass[b + 1] : (double)sh.count[b + 1];
+        here = sample::may_hold(sh.count[b], sh.count[b + 1], upto, at, past);
+    }
+    const uint64_t all = __ballot(here);
     __syncthreads();
-    return sh.found;
+    if (b < kBins && b % 64 == 0) sh.wave_step[b / 64] = all ? b + (uint32_t)__builtin_ctzll(all) : kDead;
+    __syncthreads();
+    uint32_t first = sh.last_live;
+#pragma unroll
+    for (uint32_t w = 0; w < kBins / 64; ++w) first = min(first, sh.wave_step[w]);
+    return first;
 }
 
 // A place in step `bin`: the entry where the count (by_mass: sum) reaches
