@@ -36,18 +36,6 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr uint32_t kUnit = 128;     // positions: one round of a workgroup
 constexpr uint32_t kTileRows = 8;   // query rows of a workgroup
 constexpr uint32_t kDies = 8;
-// Sequences of more query rows a key/value head take paged_many_kernel, which
-// converts a code once for 128 rows instead of once for 8 (us, 8 key/value
-// heads of 128, 16 sequences of 2000 positions, few / many: 16 rows 37 / 61,
-// 32 rows 60 / 62, 64 rows 107 / 76). But its first answer comes 20 us after
-// its start against 6, so calls of little work in all take paged_few_kernel
-// alone: query rows of a key/value head times positions of the tables up to
-// kLittle (one sequence of 512 rows from position 0 on: 13 / 23; 4 of 256: 18
-// / 23; 8 of 256, twice the bound: 32 / 26), and up to kLittleNarrow of up to
-// 128 rows, which are one tile of paged_many_kernel (128 rows at 4000: 29 /
-// 41; at 16000, twice the bound: 84 / 68).
-constexpr uint32_t kFewRows = 32;
-constexpr uint64_t kLittle = 1 << 18, kLittleNarrow = 1 << 20;
 
 struct KernelArgs {
     PagedAttentionArgs p;
@@ -59,9 +47,8 @@ struct KernelArgs {
     float inverse_stretches;
     float scaling;          // log2(e) / sqrt(head_dim)
     float *values, *sums;   // records: [record][row][D] and [record][row][2]
-    // Sequences of up to few_rows query rows a kv head take paged_few_kernel,
-    // the others paged_many_kernel.
-    uint32_t few_rows, stretches_most_many;
+    uint32_t few_rows;      // query rows a kv head up to which a sequence takes paged_few_kernel (paged::few_rows)
+    uint32_t stretches_most_many;
     float inverse_stretches_many;
     float *values_many, *sums_many;
     u4 *plan;               // per sequence: units of a stretch, its first unit, units of a tile (many: whole_units), 1: many
@@ -122,7 +109,7 @@ struct WorkLine {
         const qwh_paged_batch &batch = a.p.batch;
         const uint32_t b = base + lane;
         n = new_tokens(batch, b);
-        if ((n * a.ratio > a.few_rows) != (rows != kTileRows)) n = 0;
+        if (paged::takes_many(n * a.ratio, a.few_rows) != (rows != kTileRows)) n = 0;
         first = b < batch.batch ? batch.first[b] : 0;
         const uint32_t tiles = row_tiles(a, n, rows);
         if (rows == kTileRows) {
@@ -1148,9 +1135,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const KernelArgs a, uin
     const u4 plan = a.plan[b];
     const uint64_t seen64 = (uint64_t)a.p.batch.first[b] + t + 1;
     const uint32_t seen = seen64 < a.held ? (uint32_t)seen64 : a.held;
-    // (Starts that fall can leave a sequence without a plan: whatever stands
-    // there, only records are read.)
-    const bool many = plan.w == 1;
+    // (Starts that fall can leave a sequence without a plan. Whatever an
+    // earlier call left there, the form is one that this call runs, and
+    // stretches are held to that form's records.)
+    const bool many = paged::joins_many(plan.w, a.few_rows);
     const uint32_t per = max(plan.x, 1u), tile_rows = many ? kManyRows : kTileRows;
     const uint32_t kvh = h / a.ratio, f = t * a.ratio + (h - kvh * a.ratio);
     const uint32_t tile = f / tile_rows, slot = f - tile * tile_rows;
@@ -1208,18 +1196,8 @@ uint32_t most_stretches(int cus, const PagedAttentionArgs &a, uint32_t resident)
     return (wanted_stretches(cus, a, resident) + 2 + kDies - 1) / kDies * kDies;
 }
 
-// Which kernels a call needs: by the most query rows that a sequence may have
-// (one sequence: as if it had all rows of the buffer).
-struct Forms {
-    bool few, many;
-};
-
-Forms forms_of(const PagedAttentionArgs &a) {
-    const uint64_t ratio = a.heads / a.cache.kv_heads, rows = ratio * (a.batch.row_starts ? a.batch.rows : a.batch.batch);
-    const uint64_t work = rows * a.batch.table_pages * a.cache.page_size;
-    if (rows <= kFewRows || work <= kLittle || (rows <= 128 && work <= kLittleNarrow)) return Forms{true, false};
-    if (!a.batch.row_starts) return Forms{ratio <= kFewRows, ratio > kFewRows};
-    return Forms{a.batch.batch > 1, true};
+paged::Forms forms_of(const PagedAttentionArgs &a) {
+    return paged::forms_of(a.batch, a.heads / a.cache.kv_heads, (uint64_t)a.batch.table_pages * a.cache.page_size);
 }
 
 // Two records a stretch and head, each of a tile's rows.
@@ -1233,7 +1211,7 @@ uint64_t record_rows_many(int cus, const PagedAttentionArgs &a) {
 template <int D>
 hipError_t launch_attention(hipStream_t s, const KernelArgs &k) {
     const qwh_paged_batch &b = k.p.batch;
-    const Forms forms = forms_of(k.p);
+    const paged::Forms forms = forms_of(k.p);
     const uint32_t rows = b.row_starts ? b.rows : b.batch;
     const uint64_t join = ((uint64_t)rows * k.p.heads + 3) / 4;
     const uint64_t few = (uint64_t)k.stretches_most * k.p.cache.kv_heads, many = (uint64_t)k.stretches_most_many * k.p.cache.kv_heads;
@@ -1268,8 +1246,7 @@ hipError_t launch_paged_attention(hipStream_t s, int cus, const PagedAttentionAr
     k.ratio = a.heads / a.cache.kv_heads;
     k.ratio_magic = k.ratio == 1 ? 0 : (uint32_t)((1ull << 32) / k.ratio) + 1;
     k.page_shift = (a.cache.page_size & (a.cache.page_size - 1)) ? 32 : (uint32_t)__builtin_ctz(a.cache.page_size);
-    const Forms forms = forms_of(a);
-    k.few_rows = !forms.many ? 0xffffffffu : !forms.few ? 0 : kFewRows;
+    k.few_rows = paged::few_rows(forms_of(a));
     k.stretches_most = most_stretches(cus, a, resident_few(D));
     k.inverse_stretches = 1.0f / (float)wanted_stretches(cus, a, resident_few(D));
     k.stretches_most_many = most_stretches(cus, a, resident_many(D));

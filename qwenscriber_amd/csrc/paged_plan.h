@@ -1,6 +1,6 @@
 // Host arithmetic of the paged cache's entry points (no device code): what a
-// pool and a batch have to satisfy, and the order in which a set of page
-// copies runs. paged.cpp calls it; sanitize/plan_check.cpp checks it on the CPU.
+// pool and a batch have to satisfy, which kernels of the attention a call
+// needs, and the order in which a set of page copies runs. paged.cpp calls it; sanitize/paged_check.cpp checks it on the CPU.
 #pragma once
 
 #include <algorithm>
@@ -119,6 +119,43 @@ inline Refusal check_rows(const void *p, uint32_t stride, uint64_t width, const 
         return refuse(QWH_E_INVALID_ARGUMENT, "rows must be 16-byte aligned, strides a multiple of 4 floats");
     return {};
 }
+
+// ---- the attention's forms ----
+//
+// Sequences of more query rows a key/value head take paged_many_kernel, which
+// converts a code once for 128 rows instead of once for 8 (us, 8 key/value
+// heads of 128, 16 sequences of 2000 positions, few / many: 16 rows 37 / 61,
+// 32 rows 60 / 62, 64 rows 107 / 76). But its first answer comes 20 us after
+// its start against 6, so calls of little work in all take paged_few_kernel
+// alone: query rows of a key/value head times positions of the tables up to
+// kLittle (one sequence of 512 rows from position 0 on: 13 / 23; 4 of 256: 18
+// / 23; 8 of 256, twice the bound: 32 / 26), and up to kLittleNarrow of up to
+// 128 rows, which are one tile of paged_many_kernel (128 rows at 4000: 29 /
+// 41; at 16000, twice the bound: 84 / 68).
+constexpr uint32_t kFewRows = 32;
+constexpr uint64_t kLittle = 1 << 18, kLittleNarrow = 1 << 20;
+
+// The kernels that a call needs (at least one): by the most query rows that a
+// sequence may have (one sequence: as if it had all rows of the buffer).
+struct Forms {
+    bool few, many;
+};
+
+inline Forms forms_of(const qwh_paged_batch &b, uint64_t ratio, uint64_t positions) {
+    const uint64_t rows = ratio * (b.row_starts ? b.rows : b.batch), work = rows * positions;
+    if (rows <= kFewRows || work <= kLittle || (rows <= 128 && work <= kLittleNarrow)) return Forms{true, false};
+    if (!b.row_starts) return Forms{ratio <= kFewRows, ratio > kFewRows};
+    return Forms{b.batch > 1, true};
+}
+
+// Whether a sequence of `rows` query rows a key/value head takes the form for
+// many rows, in a call whose forms have the border few_rows; and whether its
+// records are of that form, by the word that the form left in the sequence's
+// plan (1: many) or, where it left none, any word. Neither is ever a form that
+// the call does not run: that has no records.
+constexpr uint32_t few_rows(const Forms &f) { return !f.many ? 0xffffffffu : !f.few ? 0 : kFewRows; }
+constexpr bool takes_many(uint32_t rows, uint32_t border) { return rows > border; }
+constexpr bool joins_many(uint32_t word, uint32_t border) { return border == 0 || (border != 0xffffffffu && word == 1); }
 
 // ---- page copies ----
 //

@@ -216,10 +216,36 @@ void check_refusals() {
     expect(paged::check_rows(nullptr, 2048, 2048, "", "").status == QWH_E_INVALID_ARGUMENT, "null rows");
 }
 
+// Every sequence that a call may hold takes a form that the call runs: the
+// other form's records are not reserved.
+void check_forms() {
+    static uint32_t words[4];
+    for (uint32_t ratio : {1u, 2u, 3u, 8u, 31u, 32u, 33u, 64u, 128u, 256u})
+        for (uint32_t rows : {1u, 2u, 4u, 31u, 33u, 100u, 129u, 5000u, 1u << 15})
+            for (uint32_t batch : {1u, 2u, 40u, 5000u})
+                for (uint64_t positions : {1ull, 16ull, 130ull, 1024ull, 8192ull, 70000ull, 0xfffeffffull})
+                    for (bool ragged : {false, true}) {
+                        const qwh_paged_batch b{batch, ragged ? rows : batch, 1, ragged ? words : nullptr, words, words};
+                        const paged::Forms forms = paged::forms_of(b, ratio, positions);
+                        expect(forms.few || forms.many, "no form", ratio, rows);
+                        const uint32_t border = paged::few_rows(forms);
+                        // (Words that an earlier call, or nothing, left.)
+                        for (uint32_t word : {0u, 1u, 2u, 0xffffffffu})
+                            expect(paged::joins_many(word, border) ? forms.many : forms.few, "records that are not there", word, ratio);
+                        for (uint32_t n = 1; n <= (ragged ? b.rows : 1); n += 1 + n / 5) {
+                            const bool many = paged::takes_many(n * ratio, border);
+                            expect(many ? forms.many : forms.few, "a form that does not run", n * ratio, ragged);
+                            expect(paged::joins_many(many, border) == many, "records of the other form", n * ratio, ragged);
+                            expect(!forms.few || !forms.many || many == (n * ratio > paged::kFewRows), "the border of two forms", n * ratio);
+                        }
+                    }
+}
+
 }  // namespace
 
 int main() {
     check_refusals();
+    check_forms();
     check_copies();
     std::printf("paged: %ld cases, %ld failures\n", cases, failures);
     return failures ? 1 : 0;
