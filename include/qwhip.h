@@ -349,7 +349,7 @@ typedef struct {
 #define QWH_PAGE_NONE 0xffffffffu
 
 /* One call's new tokens: rows of the row buffers, ragged over `batch`
- * sequences (device arrays, read when the call's kernels run). Sequence b's
+ * sequences (device arrays, 4-byte aligned, read when the call's kernels run). Sequence b's
  * new tokens are the rows row_starts[b] .. row_starts[b + 1] - 1 (row_starts:
  * batch + 1 values that never fall; NULL: row b alone), at its positions
  * first[b], first[b] + 1, ...; its position p lives in row p % page_size of
@@ -380,7 +380,8 @@ typedef struct {
  * a sum is split. A token whose position has no page gets its query row
  * only; a token at or past the end of its page table or of the tables' rows
  * is left out. Two tokens of a call must not share a pool row. qkv_dev and
- * query_dev 16-byte aligned, strides multiples of 4. */
+ * query_dev 16-byte aligned, strides multiples of 4; norms and rotation tables
+ * 4-byte aligned. */
 int32_t qwh_paged_append(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t layer, const qwh_paged_batch *batch,
                          const float *qkv_dev, uint32_t qkv_stride, uint32_t heads, const float *q_norm_dev,
                          const float *k_norm_dev, float eps, const float *rope_cos_dev, const float *rope_sin_dev,

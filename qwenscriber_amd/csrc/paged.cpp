@@ -41,8 +41,7 @@ int32_t qwh_paged_append(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t la
     QWH_REFUSE(paged::check_rows(query_dev, query_stride, heads * D, "query is null", "query_stride is smaller than a row"));
     if (query_dev == qkv_dev && query_stride != qkv_stride)
         return fail(ctx, QWH_E_INVALID_ARGUMENT, "a query written in place takes qkv's stride");
-    if (!q_norm_dev || !k_norm_dev || !rope_cos_dev || !rope_sin_dev)
-        return fail(ctx, QWH_E_INVALID_ARGUMENT, "a norm or rotation table is null");
+    QWH_REFUSE(paged::check_floats(q_norm_dev, k_norm_dev, rope_cos_dev, rope_sin_dev));
     OnDevice device(ctx->device);
     QWH_TRY(on_device(ctx, device));
     PagedAppendArgs a{};

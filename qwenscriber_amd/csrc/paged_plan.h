@@ -75,6 +75,8 @@ inline Refusal check_batch(const qwh_paged_batch *b) {
         return refuse(QWH_E_SHAPE_MISMATCH, "fewer rows than sequences of one row each");
     if (b->table_pages == 0) return refuse(QWH_E_SHAPE_MISMATCH, "page tables of no entry");
     if (!b->first || !b->tables) return refuse(QWH_E_INVALID_ARGUMENT, "first or tables is null");
+    if (!aligned(b->row_starts, 4) || !aligned(b->first, 4) || !aligned(b->tables, 4))
+        return refuse(QWH_E_INVALID_ARGUMENT, "row_starts, first and tables must be 4-byte aligned");
     return {};
 }
 
@@ -109,6 +111,15 @@ inline Refusal check_units(const qwh_paged_cache &c, const qwh_paged_batch &b, u
     const uint64_t units = ((uint64_t)b.table_pages * c.page_size + 127) / 128 + b.rows / 128 + 3;
     if (tiles * units >= 0x7fffffffull)
         return refuse(QWH_E_LIMIT_EXCEEDED, "rows times heads per kv head times positions past 2^41");
+    return {};
+}
+
+// The append's vectors and tables.
+inline Refusal check_floats(const float *q_norm, const float *k_norm, const float *rope_cos, const float *rope_sin) {
+    for (const float *p : {q_norm, k_norm, rope_cos, rope_sin}) {
+        if (!p) return refuse(QWH_E_INVALID_ARGUMENT, "a norm or rotation table is null");
+        if (!aligned(p, 4)) return refuse(QWH_E_INVALID_ARGUMENT, "norms and rotation tables must be 4-byte aligned");
+    }
     return {};
 }
 

@@ -189,6 +189,17 @@ void check_refusals() {
     batch(QWH_E_SHAPE_MISMATCH, "empty tables", [](auto &b) { b.table_pages = 0; });
     batch(QWH_E_INVALID_ARGUMENT, "null first", [](auto &b) { b.first = nullptr; });
     batch(QWH_E_INVALID_ARGUMENT, "null tables", [](auto &b) { b.tables = nullptr; });
+    const auto off = [](const uint32_t *p) { return reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(p) + 2); };
+    batch(QWH_E_INVALID_ARGUMENT, "starts' alignment", [&](auto &b) { b.row_starts = off(b.row_starts); });
+    batch(QWH_E_INVALID_ARGUMENT, "first's alignment", [&](auto &b) { b.first = off(b.first); });
+    batch(QWH_E_INVALID_ARGUMENT, "tables' alignment", [&](auto &b) { b.tables = off(b.tables); });
+    batch(QWH_OK, "no row, whatever its arrays", [&](auto &b) { b.rows = 0, b.first = off(b.first); });
+    const float *good_floats = reinterpret_cast<const float *>(plane), *bad_floats = reinterpret_cast<const float *>(plane + 2);
+    expect(paged::check_floats(good_floats, good_floats + 1, good_floats + 2, good_floats + 3).status == QWH_OK, "norms and tables");
+    for (int which = 0; which < 4; ++which)
+        for (const float *p : {bad_floats, (const float *)nullptr})
+            expect(paged::check_floats(which == 0 ? p : good_floats, which == 1 ? p : good_floats, which == 2 ? p : good_floats,
+                                       which == 3 ? p : good_floats).status == QWH_E_INVALID_ARGUMENT, "a norm or table", which);
     batch(QWH_E_LIMIT_EXCEEDED, "sequences", [](auto &b) { b.batch = 65536; });
     batch(QWH_E_LIMIT_EXCEEDED, "rows", [](auto &b) { b.rows = (1u << 20) + 1; });
 

@@ -10,6 +10,32 @@ from test_gpu_paged import WIDE, Batch, Pool, reference
 pytestmark = pytest.mark.gpu
 
 
+def test_arrays_off_four_bytes_are_refused(ctx):
+    """On the host: nothing is launched."""
+    buf = ctx.buffer(1 << 16)
+    cache = qa.PagedCache(1, 4, 16, 2, 64, *[buf.ptr] * 4)
+
+    def refused(arrays=(0, 0, 0), floats=(0, 0, 0, 0), appends=True, attends=True):
+        desc = qa.PagedBatch(1, 2, 4, *[buf.ptr + at for at in arrays])
+        norms = [buf.ptr + at for at in floats]
+        calls = []
+        if appends:
+            calls.append(lambda: ctx.paged_append(cache, 0, desc, buf.ptr, 512, 4, norms[0], norms[1], 1e-6, norms[2], norms[3], 64,
+                                                  buf.ptr + 8192, 256))
+        if attends:
+            calls.append(lambda: ctx.paged_attention(cache, 0, desc, buf.ptr, buf.ptr + 8192, 256, 4))
+        for call in calls:
+            with pytest.raises(qa.QwhError) as e:
+                call()
+            assert e.value.status == -1 and "4-byte" in str(e.value)
+
+    for k in range(3):
+        refused(arrays=[2 * (i == k) for i in range(3)])
+    for k in range(4):
+        refused(floats=[(i == k) for i in range(4)], attends=False)
+    buf.free()
+
+
 class Call:
     """A batch over its own pool, its rows between guard rows."""
 
