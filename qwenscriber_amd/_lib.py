@@ -72,6 +72,18 @@ STATUS = {
 }
 
 
+def _page_numbers(pages) -> np.ndarray:
+    """Page numbers as 32-bit words; ValueError for what is not one, instead
+    of another page (numpy's conversion drops fractions and upper bits)."""
+    pages = np.asarray(pages)
+    if pages.dtype != np.uint32 and pages.size:
+        if pages.dtype.kind not in "iu":
+            raise ValueError("page numbers are whole numbers")
+        if pages.min() < 0 or pages.max() > PAGE_NONE:
+            raise ValueError("a page number is not one of 32 bits")
+    return np.ascontiguousarray(pages, np.uint32)
+
+
 def library_path() -> str:
     return os.environ.get("QWHIP_LIBRARY", os.path.join(HERE, "build", "libqwhip.so"))
 
@@ -567,8 +579,7 @@ class Context:
     def paged_copy(self, cache: "PagedCache", src_pages, dst_pages) -> None:
         """Page dst_pages[i] receives what page src_pages[i] held before the
         call, in every layer (qwh_paged_copy)."""
-        src = np.ascontiguousarray(src_pages, np.uint32)
-        dst = np.ascontiguousarray(dst_pages, np.uint32)
+        src, dst = _page_numbers(src_pages), _page_numbers(dst_pages)
         if src.ndim != 1 or src.shape != dst.shape:
             raise ValueError("one destination page for each source page")
         self._check(self.lib.qwh_paged_copy(self.handle, cache, _ptr(src), _ptr(dst), src.size))

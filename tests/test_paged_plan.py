@@ -14,6 +14,7 @@ import numpy as np
 import pytest
 
 import qwenscriber_amd as qa
+from qwenscriber_amd import _lib
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CHECK = os.path.join(ROOT, "qwenscriber_amd", "build", "paged_check")
@@ -36,6 +37,21 @@ def test_null_context_is_refused_without_a_device():
     assert lib.qwh_rope_tables(None, 64, 1, 1e6, None, None) == -1
     assert lib.qwh_sample_rows(None, None, 1, 1, None, None, None) == -1
     assert lib.qwh_decoder_sample(None, None, None, None) == -1
+
+
+@pytest.mark.parametrize("pages", [[2**32 + 1], [-1], np.array([3, 2**40], np.int64), np.array([-2**31], np.int32), [1.5], np.ones(2),
+                                   [2**70], ["1"], [None], [True]])
+def test_what_is_no_page_number_is_refused(pages):
+    """Not taken as the page that its low 32 bits or its whole part name."""
+    with pytest.raises(ValueError):
+        _lib._page_numbers(pages)
+
+
+@pytest.mark.parametrize("pages", [[], [0, 5, 2**32 - 1], (1, 2), np.arange(6)[::-2], np.arange(4, dtype=np.uint8),
+                                   np.array([7, 2**32 - 1], np.uint32), np.array([2**31], np.uint64)])
+def test_page_numbers_of_any_whole_type(pages):
+    got = _lib._page_numbers(pages)
+    assert got.dtype == np.uint32 and got.flags.c_contiguous and got.tolist() == [int(p) for p in pages]
 
 
 def test_descriptors_have_the_header_s_layout():
