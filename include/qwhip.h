@@ -679,7 +679,8 @@ int32_t qwh_decoder_generate_until(qwh_decoder *decoder, const uint32_t *tokens,
 /* Draws a token for every sequence from its last logits (those that
  * qwh_decoder_forward, _forward_rows with want_logits or _step left on the
  * device) by qwh_sample_rows: params and uniform are host arrays of batch
- * records and numbers, ids_out receives batch ids. The decoder's state does
+ * records and numbers, ids_out receives batch ids; its limits (rows: the
+ * batch, logits: the vocabulary) give QWH_E_LIMIT_EXCEEDED. The decoder's state does
  * not change: the caller feeds the ids to its next forward. */
 int32_t qwh_decoder_sample(qwh_decoder *decoder, const qwh_sampling *params, const float *uniform,
                            uint32_t *ids_out);

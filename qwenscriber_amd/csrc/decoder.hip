@@ -1978,6 +1978,9 @@ int32_t qwh_decoder_generate_until(qwh_decoder *d, const uint32_t *tokens, uint3
 int32_t qwh_decoder_sample(qwh_decoder *d, const qwh_sampling *params, const float *uniform, uint32_t *ids_out) {
     if (!d || !params || !uniform || !ids_out) return QWH_E_INVALID_ARGUMENT;
     qwh_ctx *ctx = d->ctx;
+    // (qwh_sample_rows' limits: sums of more logits pass 64 bits.)
+    if (d->batch > 65535) return fail(ctx, QWH_E_LIMIT_EXCEEDED, "batch %u > 65535", d->batch);
+    if (d->c.vocab > kSampleMaxCount) return fail(ctx, QWH_E_LIMIT_EXCEEDED, "vocab %u > 2^26", d->c.vocab);
     OnDevice device(ctx->device);
     QWH_TRY(on_device(ctx, device));
     // The records, the numbers and the ids in the context's scratch, before

@@ -263,3 +263,13 @@ def test_decoder_sample(ctx):
     with pytest.raises(ValueError):
         decoder.sample(qa.Sampling(1.0, 0, 1.0, 0.0), [0.5])
     decoder.close()
+
+
+@pytest.mark.parametrize("batch,vocab", [(1, 2**26 + 64), (65536, 64)])
+def test_decoder_sample_refuses_what_sample_rows_refuses(ctx, batch, vocab):
+    config = dict(hidden=64, layers=1, heads=1, kv_heads=1, head_dim=64, ffn=64, vocab=vocab, max_positions=1, eps=1e-6, theta=1e6)
+    decoder = qa.Decoder(ctx, batch=batch, **config)
+    with pytest.raises(qa.QwhError) as e:
+        decoder.sample(qa.Sampling(1.0, 0, 1.0, 0.0), np.zeros(batch))
+    assert e.value.status == -9
+    decoder.close()
