@@ -583,10 +583,18 @@ KINDS = {"attend": (prepare_attend, attend_plain, attend_own, exact_attend, work
 
 
 def prepare(case, seed):
-    return KINDS[case["kind"]][0](case, seed)
+    s = KINDS[case["kind"]][0](case, seed)
+    if own:
+        # The package's context has a stream of its own, which does not wait
+        # for what torch's still has queued for the inputs.
+        torch.cuda.synchronize()
+    return s
 
 
 def run(state):
+    """One pass. With `own` set its outputs are written on the context's
+    stream: whoever reads them on another waits for the context
+    (`context().sync()`) or the device first."""
     return KINDS[state.case["kind"]][2 if own else 1](state)
 
 
