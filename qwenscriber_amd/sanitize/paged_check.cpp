@@ -217,6 +217,19 @@ void check_refusals() {
     expect(paged::check_heads(good, 0).status == QWH_E_SHAPE_MISMATCH, "no query head");
     expect(paged::check_heads(good, 12).status == QWH_E_SHAPE_MISMATCH, "12 over 8");
     expect(paged::check_heads(good, 4104).status == QWH_E_LIMIT_EXCEEDED, "4104 heads");
+    // 2^15 rows of 8 heads in one sequence: 32769 tiles of 8 query rows, and
+    // 259 units beside the tables'. 32769 * 65534 is 2^31 - 2.
+    qwh_paged_cache wide = good;
+    wide.page_size = 128;
+    qwh_paged_batch units{1, 1u << 15, 65534 - 259, words, words, words};
+    expect(paged::check_units(wide, units, 64).status == QWH_OK, "2^31 - 2 units");
+    ++units.table_pages;
+    expect(paged::check_units(wide, units, 64).status == QWH_E_LIMIT_EXCEEDED, "more units");
+    // A tile more for each sequence, as many as there are rows.
+    units = qwh_paged_batch{65535, 1u << 15, (uint32_t)(0x7ffffffeu / (2u << 15)) - 259, words, words, words};
+    expect(paged::check_units(wide, units, 64).status == QWH_OK, "units of short sequences");
+    ++units.table_pages;
+    expect(paged::check_units(wide, units, 64).status == QWH_E_LIMIT_EXCEEDED, "more units of short sequences");
     const qwh_paged_cache narrow{1, 1, 1, 1, 64, plane, plane, plane, plane};
     expect(paged::check_heads(narrow, 256).status == QWH_OK, "256 over 1");
     expect(paged::check_heads(narrow, 257).status == QWH_E_LIMIT_EXCEEDED, "257 over 1");
