@@ -323,7 +323,8 @@ typedef struct {
  * -infinity gives 0. params_dev: one record per row. Weights and sums are held
  * in 64 bits and added in a fixed order; a token whose weight is below 2^-63 of
  * the largest is not drawn. At most 65535 rows and 2^26 logits a row; takes
- * about 1.2 bytes of the context's scratch memory per logit, up to 160 MB. */
+ * 4.6 KB of the context's scratch memory for every 4096 logits of a row, whole
+ * or begun, up to 152 MB (allocated as the paged attention's is). */
 int32_t qwh_sample_rows(qwh_ctx *ctx, const float *logits_dev, uint32_t rows, uint32_t count,
                         const qwh_sampling *params_dev, const float *uniform_dev, uint32_t *ids_dev);
 
@@ -395,12 +396,15 @@ int32_t qwh_paged_append(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t la
  * of out_dev (heads * head_dim values, back to back); rows of no sequence are
  * left as they are. Any number of new tokens per sequence, one among them,
  * and any heads / kv_heads ratio, while rows times query heads per key/value
- * head times the tables' positions stays below about 2^41 (else
- * QWH_E_LIMIT_EXCEEDED). A value scale that is no finite number makes its own
+ * head times the sum of rows and the tables' positions stays below about 2^41
+ * (else QWH_E_LIMIT_EXCEEDED). A value scale that is no finite number makes its own
  * 64 dimensions of the rows that see it no numbers, and nothing else; a key
  * scale its head's. query_dev and out_dev 16-byte aligned and apart,
- * query_stride a multiple of 4. Records of split work take about 100 MB of the
- * context's scratch memory, or 2.3 MB a key/value head where that is more. */
+ * query_stride a multiple of 4. Weights times value scales are held to 2^-22
+ * of the largest of their row's head, products and sums in f32. Records of
+ * split work take about 100 MB of the context's scratch memory, or 2.3 MB a
+ * key/value head where that is more: the first call that needs more than
+ * the context has waits for its stream and allocates. */
 int32_t qwh_paged_attention(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t layer, const qwh_paged_batch *batch,
                             float *out_dev, const float *query_dev, uint32_t query_stride, uint32_t heads);
 

@@ -47,7 +47,7 @@ constexpr uint32_t kOrder = 256;       // and of these, puts in order
 constexpr int kThreads = 1024;
 constexpr int kUnitBits = 37;          // of a weight of 1 in a step's sum
 constexpr int kCountShift = 50;        // 4096 * 2^(1/4) * 2^37 < 2^50: the count stands above the sum
-constexpr uint32_t kPartsAtOnce = 32768;  // of a launch (160 MB of scratch)
+constexpr uint32_t kPartsAtOnce = 32768;  // of a launch (152 MB of scratch)
 
 // Order-preserving bits of a logit (0: NaN, never drawn); -0 counts as 0.
 __device__ __forceinline__ uint32_t logit_key(float l) {
