@@ -175,8 +175,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendArgs
 // holds its kPieces pieces through a whole chain of steps (paged_plan.h): what
 // one step reads, an earlier or later step of the same thread writes, so
 // chains need no barrier, and a source that goes to several pages is read
-// once. Bound by HBM: 300 pages of 16 positions in 28 layers, 284 MB read and
-// as much written, 119 us (4.8 TB/s; 8 pieces a thread, 157).
+// once. Bound by HBM where chains are short: 300 pages of 16 positions in 28
+// layers, 284 MB read and as much written, 117 us (4.9 TB/s; 8 pieces a thread,
+// 157). A long chain is bound by its round trips, a load and the store of it
+// a step: the same 300 pages each to the page before it, 394 us.
 constexpr int kPieces = 4;
 
 template <bool kNarrowScales, typename Steps>

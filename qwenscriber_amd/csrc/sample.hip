@@ -20,8 +20,10 @@
 // of 2^-37: integers, so the order of the LDS atomics does not matter, and
 // count and sum share one 64-bit word and one atomic. Running sums over steps
 // and tokens are 64-bit floats in a fixed order. A draw so differs from one
-// in real numbers only where u falls within about 1e-12 of a border; with
-// 32-bit weights, about one draw in 1000 of an unfiltered row of 151936 would.
+// in real numbers only where u falls within about 1e-12 of a border (logits of
+// more than 10^4 temperatures, whose y has fewer bits behind the point: in
+// proportion more); with 32-bit weights, about one draw in 1000 of an
+// unfiltered row of 151936 would.
 //
 // The first launch is bound by its vector instructions, f64 among them (64
 // rows of 151936, 39 MB: 20 us; one row 5.4; parts of 8192 logits, 27 and 12),
