@@ -397,14 +397,15 @@ int32_t qwh_paged_append(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t la
  * left as they are. Any number of new tokens per sequence, one among them,
  * and any heads / kv_heads ratio, while rows times query heads per key/value
  * head times the sum of rows and the tables' positions stays below about 2^41
- * (else QWH_E_LIMIT_EXCEEDED). A value scale that is no finite number makes its own
- * 64 dimensions of the rows that see it no numbers, and nothing else; a key
+ * (else QWH_E_LIMIT_EXCEEDED). A value scale that is no finite number makes its
+ * own 64 dimensions of the rows that see it no numbers, and nothing else; a key
  * scale its head's. query_dev and out_dev 16-byte aligned and apart,
  * query_stride a multiple of 4. Weights times value scales are held to 2^-22
- * of the largest of their row's head, products and sums in f32. Records of
- * split work take about 100 MB of the context's scratch memory, or 2.3 MB a
- * key/value head where that is more: the first call that needs more than
- * the context has waits for its stream and allocates. */
+ * of the largest of their row's head (a scale of 0 counting as 2^-24, f16's
+ * least), products and sums in f32. Records of split work take about 100 MB of
+ * the context's scratch memory, or 2.3 MB a key/value head where that is more:
+ * the first call that needs more than the context has waits for its stream and
+ * allocates. */
 int32_t qwh_paged_attention(qwh_ctx *ctx, const qwh_paged_cache *cache, uint32_t layer, const qwh_paged_batch *batch,
                             float *out_dev, const float *query_dev, uint32_t query_stride, uint32_t heads);
 
