@@ -320,9 +320,11 @@ typedef struct {
  * as 0, from 1 on the last kept token with a weight). A NaN logit is never
  * drawn, nor one of -infinity beside a larger one; where the largest is
  * +infinity, only those are drawn, evenly. A row with nothing but NaN and
- * -infinity gives 0. params_dev: one record per row. Weights and sums are held
- * in 64 bits and added in a fixed order; a token whose weight is below 2^-63 of
- * the largest is not drawn. At most 65535 rows and 2^26 logits a row; takes
+ * -infinity gives 0. params_dev: one record per row. Weights are rounded to
+ * 2^-38 of themselves, alike for equal logits, and summed in 64 bits; where
+ * tokens with the largest logit are all that is summed, top_p and a number that
+ * fall on a border of two of them fall on the definition's side. A token whose
+ * weight is below 2^-63 of the largest is not drawn. At most 65535 rows and 2^26 logits a row; takes
  * 4.6 KB of the context's scratch memory for every 4096 logits of a row, whole
  * or begun, up to 152 MB (allocated as the paged attention's is). */
 int32_t qwh_sample_rows(qwh_ctx *ctx, const float *logits_dev, uint32_t rows, uint32_t count,

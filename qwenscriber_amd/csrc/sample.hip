@@ -15,15 +15,20 @@
 //
 // Steps and weights: y = l * 4 / (T ln 2) in 64 bits; step floor(y), the same
 // grid in every part; within a step a token weighs 2^((y - floor(y)) / 4), 1
-// to 2^(1/4), and the step itself is a power of 2^(1/4) that comes in when
-// steps are added. Within a step the sums are of weights in whole multiples
-// of 2^-37: integers, so the order of the LDS atomics does not matter, and
-// count and sum share one 64-bit word and one atomic. Running sums over steps
-// and tokens are 64-bit floats in a fixed order. A draw so differs from one
-// in real numbers only where u falls within about 1e-12 of a border (logits of
-// more than 10^4 temperatures, whose y has fewer bits behind the point: in
-// proportion more); with 32-bit weights, about one draw in 1000 of an
-// unfiltered row of 151936 would.
+// to 2^(1/4), in whole multiples of 2^-37, and the step itself is a power of
+// 2^(1/4) that comes in when steps are added. Within a step sums are integers,
+// so the order of the LDS atomics does not matter, and count and sum share one
+// 64-bit word and one atomic. Running sums over steps and tokens are 64-bit
+// floats in a fixed order. Every sum, of a histogram, a step's split or a list,
+// is of the same multiples, and the largest logit's step weighs 1: sums of
+// tokens that share it are whole numbers of one weight, however they are added,
+// and where top_p's or u's part of the whole is such a sum, the token is the one
+// that the definition says. (Sums are compared as equal within 2^-47, which is
+// what 64-bit additions may leave of larger ones: kReach, kPast.) Otherwise a
+// draw differs from one in real numbers only where u falls within 4e-12 of a
+// border (half a multiple; logits of more than 10^4 temperatures, whose y has
+// fewer bits behind the point: in proportion more); with 32-bit weights, about
+// one draw in 1000 of an unfiltered row of 151936 would.
 //
 // The first launch is bound by its vector instructions, f64 among them (64
 // rows of 151936, 39 MB: 20 us; one row 5.4; parts of 8192 logits, 27 and 12),
@@ -49,6 +54,7 @@ constexpr uint32_t kOrder = 256;       // and of these, puts in order
 constexpr int kThreads = 1024;
 constexpr int kUnitBits = 37;          // of a weight of 1 in a step's sum
 constexpr int kCountShift = 50;        // 4096 * 2^(1/4) * 2^37 < 2^50: the count stands above the sum
+constexpr double kReach = 1.0 - 0x1p-47, kPast = 1.0 + 0x1p-47;  // what a sum has to reach, or pass, for a part of it
 constexpr uint32_t kPartsAtOnce = 32768;  // of a launch (152 MB of scratch)
 
 // Order-preserving bits of a logit (0: NaN, never drawn); -0 counts as 0.
@@ -114,7 +120,10 @@ struct QuarterPower {
         return e + add;
     }
 };
-__device__ __forceinline__ double quarter_power(double f) { return QuarterPower(1.0, 0.0)(f); }
+
+// The same in whole units of 2^-kUnitBits: the sum with 2^52 rounds to them.
+constexpr double kUnits = (double)(1ull << kUnitBits);
+__device__ __forceinline__ double quarter_power(double f) { return (QuarterPower(kUnits, 0x1p52)(f) - 0x1p52) * (1.0 / kUnits); }
 
 // Weights against a reference step (infinite where the largest logit is: then
 // such logits weigh 1 and others nothing).
@@ -242,7 +251,7 @@ __global__ __launch_bounds__(256) void sample_parts_kernel(const float *logits, 
         // A weight as a whole number of units: the sum with 2^52 rounds to
         // one and holds it in its low bits. (Eight chains side by side, no
         // branch between them.)
-        const QuarterPower units((double)(1ull << kUnitBits), 0x1p52);
+        const QuarterPower units(kUnits, 0x1p52);
 #pragma unroll
         for (int i0 = 0; i0 < 16; i0 += 8) {
             uint64_t add[8];
@@ -558,9 +567,9 @@ __device__ __noinline__ void place_in(RowShared &sh, const Row &row, uint32_t bi
         high = sh.edge[1];
     }
     // The range of keys split into up to 1024 equal ones, and the one that
-    // has the place again, until it has few tokens or one key. (Sums in units
-    // of 2^-36: 2^26 weights fit 64 bits.)
-    const double unit = step_weight(bin) * 0x1p-36;
+    // has the place again, until it has few tokens or one key. (Sums in units:
+    // 2^26 weights of up to 2^(1/4) fit 64 bits.)
+    const double unit = step_weight(bin) * (1.0 / kUnits);
     while (true) {
         if (!listed && n <= kList) {
             collect(sh, row, bin, bin, whole, low, high);
@@ -577,7 +586,7 @@ __device__ __noinline__ void place_in(RowShared &sh, const Row &row, uint32_t bi
             double within;
             (void)row.w.bin(key, within);
             atomicAdd(&sh.split_n[d], 1u);
-            atomicAdd(&sh.split_m[d], (unsigned long long)rint(within * 0x1p36));
+            atomicAdd(&sh.split_m[d], (unsigned long long)(within * kUnits));
         };
         if (listed) {
             const uint32_t all = min(sh.listed, kList);
@@ -730,7 +739,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
                 m += sh.split_m[g * kBins + b];
             }
             run_n = n;
-            run_m = (double)m * (step_weight(b) / (double)(1ull << kUnitBits));
+            run_m = (double)m * (step_weight(b) * (1.0 / kUnits));
         }
         block_scan(sh, run_n, run_m);
         if (group == 0) {
@@ -760,7 +769,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
     // The last step that any rule can keep a token of.
     uint32_t last = sh.last_live;
     if (by_k) last = min(last, step_of(sh, false, (double)p.top_k, false));
-    else if (by_p) last = min(last, step_of(sh, true, (double)p.top_p * sh.mass[kDead], false));
+    else if (by_p) last = min(last, step_of(sh, true, (double)p.top_p * kReach * sh.mass[kDead], false));
     else if (least > 0.0 && !row.w.infinite) last = min(last, (uint32_t)fmin(row.w.reference - floor(top * row.w.c + 4.0 * log2(least)) + 1.0, (double)(kDead - 1)));
     // All that may be kept, if it fits the list.
     const uint32_t n = sh.count[last + 1];
@@ -774,7 +783,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
         uint32_t tokens = by_k ? min(p.top_k, n) : n;
         if (by_p) {
             const double whole = by_k ? sh.run[tokens - 1] : sh.mass[kDead];
-            tokens = min(tokens, reach(sh, tokens, (double)p.top_p * whole, false) + 1);
+            tokens = min(tokens, reach(sh, tokens, (double)p.top_p * kReach * whole, false) + 1);
         }
         if (least > 0.0) {
             __syncthreads();
@@ -787,7 +796,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
             tokens = max(sh.counted, 1u);
         }
         const double kept = sh.run[tokens - 1];
-        const uint32_t k = draw >= 1.0 ? tokens - 1 : reach(sh, tokens, draw * kept, true);
+        const uint32_t k = draw >= 1.0 ? tokens - 1 : reach(sh, tokens, draw * kPast * kept, true);
         __syncthreads();
         if (tid == 0) ids[blockIdx.x] = (uint32_t)sh.ordered[min(k, tokens - 1)];
         return;
@@ -801,7 +810,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
         kept = sh.found_mass;
     }
     if (by_p) {
-        const double at = (double)p.top_p * kept;
+        const double at = (double)p.top_p * kReach * kept;
         place_in(sh, row, step_of(sh, true, at, false), true, at, false, listed);
         tokens = sh.found_count;
         kept = sh.found_mass;
@@ -825,7 +834,10 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(const float *logi
         }
     }
     if (draw >= 1.0) place_in(sh, row, step_of(sh, false, (double)tokens, false), false, (double)tokens, false, listed);
-    else place_in(sh, row, step_of(sh, true, draw * kept, true), true, draw * kept, true, listed);
+    else {
+        const double at = draw * kPast * kept;
+        place_in(sh, row, step_of(sh, true, at, true), true, at, true, listed);
+    }
     if (tid == 0) ids[blockIdx.x] = sh.found_index;
 }
 
