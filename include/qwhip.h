@@ -377,10 +377,10 @@ typedef struct {
  * k_norm_dev, head_dim weights) and the rotation of its position (row p of
  * rope_cos_dev / rope_sin_dev, [rope_positions][head_dim/2], qwh_rope_tables);
  * the query goes to row i of query_dev (query_stride floats apart; query_dev
- * may be qkv_dev with its stride), key and value to layer `layer`'s row of the
- * position, as qwh_kv_append_q8 stores them. Norm and rotation are held in 64
- * bits and rounded to f32 once, so that a stored code does not depend on how
- * a sum is split. A token whose position has no page gets its query row
+ * may be qkv_dev with its stride, else they are apart), key and value to layer
+ * `layer`'s row of the position, as qwh_kv_append_q8 stores them. Norm and
+ * rotation are held in 64 bits and rounded to f32 once, so that a stored code
+ * does not depend on how a sum is split. A token whose position has no page gets its query row
  * only; a token at or past the end of its page table or of the tables' rows
  * is left out. Two tokens of a call must not share a pool row. qkv_dev and
  * query_dev 16-byte aligned, strides multiples of 4; norms and rotation tables
