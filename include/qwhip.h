@@ -684,11 +684,12 @@ int32_t qwh_decoder_generate_until(qwh_decoder *decoder, const uint32_t *tokens,
                                    const uint32_t *stop_tokens, uint32_t stop_count, uint32_t *ids_out,
                                    uint32_t *counts_out);
 /* Draws a token for every sequence from its last logits (those that
- * qwh_decoder_forward, _forward_rows with want_logits or _step left on the
- * device) by qwh_sample_rows: params and uniform are host arrays of batch
+ * qwh_decoder_forward or _forward_rows with want_logits, _step, _generate or,
+ * for its sequence, _prefill left on the device; zeros before the first of
+ * these) by qwh_sample_rows: params and uniform are host arrays of batch
  * records and numbers, ids_out receives batch ids; its limits (rows: the
- * batch, logits: the vocabulary) give QWH_E_LIMIT_EXCEEDED. The decoder's state does
- * not change: the caller feeds the ids to its next forward. */
+ * batch, logits: the vocabulary) give QWH_E_LIMIT_EXCEEDED. The decoder's state
+ * does not change: the caller feeds the ids to its next forward. */
 int32_t qwh_decoder_sample(qwh_decoder *decoder, const qwh_sampling *params, const float *uniform,
                            uint32_t *ids_out);
 /* Copies sequence `seq`'s last logits (vocab f32) to the host. */
