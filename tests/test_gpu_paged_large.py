@@ -118,3 +118,36 @@ def test_steps_of_many_heads_over_wide_tables(ctx):
 def test_a_chunk_of_more_than_64_tiles(ctx, first):
     rng = np.random.default_rng(66)
     check(ctx, rng, (16, 1, 64), 16, [7, 600, 5], [40, first, 3], pad=2)
+
+
+@pytest.mark.parametrize("n,spare", FORMS)
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("log2_score", [12.0, 26.5, 27.5, 60.0])
+def test_a_maximum_that_moves_over_a_long_context(ctx, n, spare, sign, log2_score):
+    """Keys that rise, or fall, along a context that several workgroups take:
+    a row is the mean of the values at the last key's positions (the next key's
+    score is 32 and more away in base 2, or 2^-32 of the weights), with the
+    same roundings as above."""
+    rng = np.random.default_rng(67)
+    heads, kv_heads, D, first = 4, 2, 128, 1500
+    batch = Batch(rng, 16, [n], [first], spare=spare, one_row=n == 1)
+    pool = Pool(ctx, rng, 1, batch.pages, 16, kv_heads, D)
+    owned = batch.owned()[0]
+    pool.fill(0, owned)
+    pool.scales[0][0, owned] = 2.0**-6
+    pool.scales[1][0, owned] = 2.0**-4
+    step = np.arange(len(owned)) * 120 // len(owned)
+    code = step if sign > 0 else -step - 1
+    dim = 37
+    for g in range(kv_heads):
+        pool.codes[0][0, owned, g * D + dim] = 128 + code
+    query = np.zeros((n, heads, D), np.float32)
+    query[:, :, dim] = 2.0**log2_score / (127 * 2.0**-6 * np.log2(np.e) / np.sqrt(D))
+    got = attend(ctx, pool, 0, batch, query.reshape(n, heads * D), heads).reshape(n, heads, D)
+    for t in range(n):
+        seen = owned[:first + t + 1]
+        best = seen[code[:first + t + 1] == code[:first + t + 1].max()]
+        for h in range(heads):
+            v, others = pool.values(1, 0, best, h // 2), np.abs(pool.values(1, 0, seen, h // 2)).max()
+            bound = np.abs(v).mean(0) * (2 * (len(owned) + 64) * 2.0**-24 + 2.0**-21) + len(owned) * 2.0**-32 * others
+            assert np.all(np.abs(got[t, h] - v.mean(0)) <= bound), (t, h)
